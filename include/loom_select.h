@@ -18,6 +18,9 @@
  *                      no counterpart there and follows the semantics written beside it below.
  *   loom_sample_shard_partial / loom_sample_shard_merge
  *                      the same chain with the vocabulary split across GPUs; no counterpart.
+ *   loom_token_logprobs / loom_token_logprobs_grad
+ *                      log-probabilities of given tokens, with entropy, rank and top alternatives, and
+ *                      their gradient; no counterpart (loom.cpp scores no tokens).
  *   loom_lm_head_argmax
  *                      the text model's last ggml_mul_mat(lm_head, hidden) followed by
  *                      Generator::argmax (src/core/generation.cpp:64-74), fused: the logits stay on chip.
@@ -266,6 +269,54 @@ LOOM_SELECT_API size_t loom_lm_head_workspace_size(int64_t rows, int64_t n_vocab
 LOOM_SELECT_API int loom_lm_head_argmax(const void* hidden, const void* weight, int64_t rows, int64_t hidden_dim,
                                         int64_t n_vocab, int32_t* out_ids, float* out_logit, float* out_lse,
                                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* Most alternatives one loom_token_logprobs call returns per row. */
+#define LOOM_SELECT_MAX_TOP_LOGPROBS 32
+
+/*
+ * Log-probabilities of given tokens. No loom.cpp counterpart: it is what a host that scores text asks of
+ * the logits -- the log-probability and alternatives an API reports beside each token, the log-likelihood
+ * of a prompt, the policy's log-probabilities and entropy in training. Per row x[0..V), y = x / T:
+ *   out_lse     = log sum_v exp(y_v)
+ *   out_logp    = y_t - out_lse for t = ids[r]
+ *   out_entropy = -sum_v p_v log p_v, p_v = exp(y_v - out_lse) (nats)
+ *   out_rank    = number of ids v ahead of t: x_v > x_t, or x_v == x_t and v < t (0: t is the greedy id)
+ *   out_top_ids, out_top_logp ([rows][n_top]) = the first n_top ids by x descending, then id ascending, and
+ *                 their log-probabilities.
+ * Every output may be NULL, not all of them; ids may be NULL when out_logp and out_rank are. n_top is 0 .. min(V,
+ * LOOM_SELECT_MAX_TOP_LOGPROBS), positive exactly when one of out_top_ids and out_top_logp is given. T is a
+ * positive, finite, normal float (LOOM_SELECT_EPARAM otherwise, as for n_top out of range). Log-probabilities are
+ * accurate to 1e-5 absolute or relative, whichever is larger. The comparisons are exact: -0 == +0.
+ *   - A negative id means "no token in this row" (padding): out_logp = 0, out_rank = -1, the rest as usual.
+ *     An id >= V: out_logp = NaN, out_rank = -1.
+ *   - -inf logits have probability 0 (masked ids). A row of nothing else: out_lse = -inf, out_logp, out_entropy and
+ *     out_top_logp NaN.
+ *   - A NaN or +inf logit makes out_lse, out_logp, out_entropy and out_top_logp of its row NaN; a NaN is never an
+ *     alternative (id -1, NaN, once nothing else is left), never ahead of a token, and has out_rank -1 itself.
+ * Needs no workspace and keeps no state: calls on several streams, and graphs replayed at once, do not meet.
+ * LOOM_SELECT_ESHAPE for rows beyond 2^27 - 1 or V beyond 2^31 - 1.
+ */
+LOOM_SELECT_API int loom_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t n_vocab,
+                                        int64_t row_stride, const int32_t* ids, float temperature, int32_t n_top,
+                                        float* out_logp, float* out_entropy, float* out_lse, int32_t* out_rank,
+                                        int32_t* out_top_ids, float* out_top_logp, void* stream);
+
+/*
+ * The gradient of  L = sum_r grad_logp[r] * out_logp[r] + grad_entropy[r] * out_entropy[r]  with respect to the logits,
+ * from the forward call's lse and entropy, in the logits' type:
+ *   out_grad[r, v] = (1 / T) * (grad_logp[r] * ([v == t] - p_v) - grad_entropy[r] * p_v * (log p_v + entropy[r]))
+ * grad_logp or grad_entropy may be NULL (all zeros), not both; entropy may be NULL without grad_entropy, ids without
+ * grad_logp. A negative id takes no part (its grad_logp counts as 0), an id >= V with a non-zero grad_logp makes its
+ * row NaN. A row whose two weights are 0 gets zeros, whatever its logits hold; otherwise a row whose lse is NaN or
+ * -inf gets NaN. -inf logits get 0. out_grad rows are grad_stride >= V elements apart; out_grad may be the logits
+ * themselves (same pointer, same stride: LOOM_SELECT_EINVAL otherwise), and must not overlap them in another way.
+ * No workspace, no atomics: the result does not depend on timing.
+ */
+LOOM_SELECT_API int loom_token_logprobs_grad(const void* logits, int dtype, int64_t rows, int64_t n_vocab,
+                                             int64_t row_stride, const int32_t* ids, float temperature,
+                                             const float* lse, const float* entropy, const float* grad_logp,
+                                             const float* grad_entropy, void* out_grad, int64_t grad_stride,
+                                             void* stream);
 
 #ifdef __cplusplus
 } /* extern "C" */

@@ -10,6 +10,7 @@ loom.cpp names on CUDA tensors:
     ctc_greedy_decode(logits, blank_id)      loom::ctc_greedy_decode          src/core/ctc_decode.cpp:7-31
     sample_rows(logits, ...)                 the sampling chain (no loom.cpp counterpart)
     shard_partial / shard_merge              the vocabulary-sharded chain (no loom.cpp counterpart)
+    token_logprobs / token_logprobs_grad     log-probabilities of given tokens, and their gradient (none)
 
 Errors raise SelectError, as loom.cpp raises loom::Error (include/loom/loom_errors.h:10) and its
 Lua bindings turn that into a Lua error (lua_bridge.cpp:26-32). The library must be present: there
@@ -17,6 +18,8 @@ is no fallback of any kind, and importing this module on a machine without it fa
 
 torch is used for device memory, streams and host<->device copies only.
 """
+import collections
+import contextlib
 import ctypes
 import os
 
@@ -27,6 +30,7 @@ F32 = 0
 BF16 = 1
 MAX_TOP_K = 1024
 MAX_WINDOWS = 8
+MAX_TOP_LOGPROBS = 32
 
 OK = 0
 EINVAL = 1
@@ -60,6 +64,8 @@ EXPORTS = (
     "loom_ctc_greedy",
     "loom_lm_head_workspace_size",
     "loom_lm_head_argmax",
+    "loom_token_logprobs",
+    "loom_token_logprobs_grad",
 )
 
 
@@ -89,6 +95,7 @@ def _lib():
             raise RuntimeError(f"{LIB_PATH} is missing: build it with `python {os.path.join(_HERE, 'build.py')}`")
         lib = ctypes.CDLL(LIB_PATH)
         vp, i32, i64, sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t
+        f32 = ctypes.c_float
         sig = {
             "loom_select_strerror": (ctypes.c_char_p, [ctypes.c_int]),
             "loom_select_abi_version": (ctypes.c_int, []),
@@ -113,6 +120,10 @@ def _lib():
             "loom_ctc_greedy": (ctypes.c_int, [vp, ctypes.c_int, i64, i64, i64, i32, vp, vp, vp, vp, vp, vp, sz, vp]),
             "loom_lm_head_workspace_size": (sz, [i64, i64]),
             "loom_lm_head_argmax": (ctypes.c_int, [vp, vp, i64, i64, i64, vp, vp, vp, vp, sz, vp]),
+            "loom_token_logprobs": (ctypes.c_int, [vp, ctypes.c_int, i64, i64, i64, vp, f32, i32, vp, vp, vp, vp, vp,
+                                                   vp, vp]),
+            "loom_token_logprobs_grad": (ctypes.c_int, [vp, ctypes.c_int, i64, i64, i64, vp, f32, vp, vp, vp, vp, vp,
+                                                        i64, vp]),
         }
         for name, (res, args) in sig.items():
             f = getattr(lib, name)
@@ -429,3 +440,112 @@ def lm_head_argmax(hidden, weight, want_logit=True, want_lse=True, workspace=Non
     lse = torch.empty(rows, dtype=torch.float32, device=dev) if want_lse else None
     lm_head_argmax_into(hidden, weight, ids, logit, lse, workspace, stream)
     return ids, logit, lse
+
+
+# ----------------------------------------------------------------------------------------------
+# log-probabilities of given tokens
+
+def _check_tensor(t, name, dtype, shape, device):
+    """A contiguous tensor of this type and shape on `device`, or None."""
+    if t is None:
+        return
+    if t.dtype != dtype:
+        raise SelectError(EDTYPE, f"{name} is {t.dtype}, expected {dtype}")
+    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise SelectError(EINVAL, f"{name} must be contiguous, of shape {tuple(shape)}")
+    if t.device != device:
+        raise SelectError(EINVAL, f"{name} is on {t.device}, expected {device}")
+
+
+def _check_device(t, name):
+    """The kernels run on the current device: a tensor elsewhere is an error, not a fault."""
+    if t.device.type != "cuda" or t.device.index != _torch().cuda.current_device():
+        raise SelectError(EINVAL, f"{name} is on {t.device}, not on the current CUDA device")
+
+
+def _on(stream):
+    """New tensors belong to the stream that fills them."""
+    return contextlib.nullcontext() if stream is None else _torch().cuda.stream(stream)
+
+
+def token_logprobs_into(logits, ids, out_logp=None, out_entropy=None, out_lse=None, out_rank=None, out_top_ids=None,
+                        out_top_logp=None, temperature=1.0, stream=None):
+    """Log-probabilities of ids [rows] (int32; negative: no token) under logits [rows, n_vocab] (asynchronous).
+
+    out_logp, out_entropy, out_lse f32 [rows], out_rank int32 [rows], out_top_ids int32 and out_top_logp f32
+    [rows, n] (n alternatives, at most MAX_TOP_LOGPROBS), each of them or None. See loom_token_logprobs."""
+    torch = _torch()
+    rows, n_vocab, stride = _rows_view(logits)
+    code, dev = _dtype_code(logits), logits.device
+    _check_device(logits, "logits")
+    n_top = 0
+    for t in (out_top_ids, out_top_logp):
+        if t is not None:
+            if t.dim() == 0:
+                raise SelectError(EINVAL, "alternatives must be [rows, n]")
+            n_top = t.shape[-1]
+    top = (rows, n_top) if logits.dim() == 2 else (n_top,)
+    per_row = (rows,)
+    for t, name, dtype, shape in ((ids, "ids", torch.int32, per_row), (out_logp, "out_logp", torch.float32, per_row),
+                                  (out_entropy, "out_entropy", torch.float32, per_row),
+                                  (out_lse, "out_lse", torch.float32, per_row),
+                                  (out_rank, "out_rank", torch.int32, per_row),
+                                  (out_top_ids, "out_top_ids", torch.int32, top),
+                                  (out_top_logp, "out_top_logp", torch.float32, top)):
+        _check_tensor(t, name, dtype, shape, dev)
+    check(_lib().loom_token_logprobs(_ptr(logits), code, rows, n_vocab, stride, _ptr(ids), temperature, n_top,
+                                     _ptr(out_logp), _ptr(out_entropy), _ptr(out_lse), _ptr(out_rank),
+                                     _ptr(out_top_ids), _ptr(out_top_logp), _stream_handle(stream)),
+          "loom_token_logprobs")
+
+
+TokenLogprobs = collections.namedtuple("TokenLogprobs", "logp entropy lse rank top_ids top_logp")
+
+
+def token_logprobs(logits, ids=None, temperature=1.0, n_top=0, want_entropy=True, want_rank=False, stream=None):
+    """TokenLogprobs(logp, entropy, lse, rank, top_ids, top_logp) as CUDA tensors, None for what is not asked for
+    (logp and rank without ids, alternatives with n_top == 0)."""
+    torch = _torch()
+    rows, _, _ = _rows_view(logits)
+    dev = logits.device
+    if want_rank and ids is None:
+        raise SelectError(EINVAL, "a rank needs ids")
+    with _on(stream):
+        f32 = [torch.empty(rows, dtype=torch.float32, device=dev) if w else None
+               for w in (ids is not None, want_entropy, True)]
+        rank = torch.empty(rows, dtype=torch.int32, device=dev) if want_rank else None
+        top = (rows, n_top) if logits.dim() == 2 else (n_top,)
+        top_ids = torch.empty(top, dtype=torch.int32, device=dev) if n_top else None
+        top_logp = torch.empty(top, dtype=torch.float32, device=dev) if n_top else None
+    token_logprobs_into(logits, ids, f32[0], f32[1], f32[2], rank, top_ids, top_logp, temperature, stream)
+    return TokenLogprobs(f32[0], f32[1], f32[2], rank, top_ids, top_logp)
+
+
+def token_logprobs_grad_into(logits, ids, lse, out_grad, grad_logp=None, grad_entropy=None, entropy=None,
+                             temperature=1.0, stream=None):
+    """d/dlogits of sum(grad_logp * logp + grad_entropy * entropy) into out_grad, of the logits' shape and type
+    (rows may be strided; out_grad may be the logits themselves). lse and entropy are the forward call's."""
+    torch = _torch()
+    rows, n_vocab, stride = _rows_view(logits)
+    code, dev = _dtype_code(logits), logits.device
+    _check_device(logits, "logits")
+    if out_grad.dtype != logits.dtype:
+        raise SelectError(EDTYPE, f"out_grad is {out_grad.dtype}, expected {logits.dtype}")
+    if out_grad.shape != logits.shape or out_grad.device != dev:
+        raise SelectError(EINVAL, "out_grad must have the logits' shape and device")
+    _, _, grad_stride = _rows_view(out_grad)
+    for t, name, dtype in ((ids, "ids", torch.int32), (lse, "lse", torch.float32), (entropy, "entropy", torch.float32),
+                           (grad_logp, "grad_logp", torch.float32), (grad_entropy, "grad_entropy", torch.float32)):
+        _check_tensor(t, name, dtype, (rows,), dev)
+    check(_lib().loom_token_logprobs_grad(_ptr(logits), code, rows, n_vocab, stride, _ptr(ids), temperature, _ptr(lse),
+                                          _ptr(entropy), _ptr(grad_logp), _ptr(grad_entropy), _ptr(out_grad),
+                                          grad_stride, _stream_handle(stream)), "loom_token_logprobs_grad")
+    return out_grad
+
+
+def token_logprobs_grad(logits, ids, lse, grad_logp=None, grad_entropy=None, entropy=None, temperature=1.0,
+                        stream=None):
+    """token_logprobs_grad_into a new tensor."""
+    with _on(stream):
+        out = _torch().empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    return token_logprobs_grad_into(logits, ids, lse, out, grad_logp, grad_entropy, entropy, temperature, stream)
