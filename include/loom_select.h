@@ -21,6 +21,9 @@
  *   loom_token_logprobs / loom_token_logprobs_grad
  *                      log-probabilities of given tokens, with entropy, rank and top alternatives, and
  *                      their gradient; no counterpart (loom.cpp scores no tokens).
+ *   loom_rms_norm_i8, loom_quantize_rows_i8, loom_lm_head_logits_i8
+ *                      the text model's final norm and ggml_mul_mat(lm_head, hidden) with the LM head in
+ *                      8-bit integers, a scale per token and per vocabulary id; no counterpart for the format.
  *   loom_lm_head_argmax
  *                      the text model's last ggml_mul_mat(lm_head, hidden) followed by
  *                      Generator::argmax (src/core/generation.cpp:64-74), fused: the logits stay on chip.
@@ -317,6 +320,44 @@ LOOM_SELECT_API int loom_token_logprobs_grad(const void* logits, int dtype, int6
                                              const float* lse, const float* entropy, const float* grad_logp,
                                              const float* grad_entropy, void* out_grad, int64_t grad_stride,
                                              void* stream);
+
+/*
+ * The LM head in 8-bit integers, three calls. A text model's last norm makes 8-bit hidden states with a scale per
+ * row (loom_rms_norm_i8); its LM-head weight was made 8-bit once, with a scale per vocabulary id
+ * (loom_quantize_rows_i8); the product of the two (loom_lm_head_logits_i8) is what loom_argmax_rows,
+ * loom_sample_rows and loom_token_logprobs take.
+ *
+ * loom_rms_norm_i8, per row of D = dim elements (rows x_stride apart, the residual's and out_sum's by their own):
+ *   h = x + residual, rounded to `dtype`, stored to out_sum when given (h = x when residual is NULL)
+ *   y = (h * inv) * weight,  inv = (float)(1 / sqrt(sum h^2 / D + eps)) computed in double, the products in f32
+ *   out_scale = a / 127,  out_q = rint(y * ((1 / a) * 127)),  a = max |y|     (f32 steps, round to nearest even)
+ * so out_q * out_scale stands for y; out_q is in [-127, 127], rows packed. A row with a below 2^-100 gives zeros and
+ * scale 0; a NaN or infinity anywhere in y gives zeros and scale NaN. weight is [dim], of its own type. eps is a
+ * positive finite number (LOOM_SELECT_EPARAM). out_sum may be x or residual themselves (same pointer and stride) and
+ * must not overlap them in another way. loom_quantize_rows_i8 is the same with y = x. dim <= 32768 and
+ * rows <= 2^31 - 1 (LOOM_SELECT_ESHAPE). No workspace.
+ */
+LOOM_SELECT_API int loom_rms_norm_i8(const void* x, int dtype, int64_t rows, int64_t dim, int64_t x_stride,
+                                     const void* residual, int64_t residual_stride, const void* weight,
+                                     int weight_dtype, double eps, int8_t* out_q, float* out_scale, void* out_sum,
+                                     int64_t sum_stride, void* stream);
+LOOM_SELECT_API int loom_quantize_rows_i8(const void* x, int dtype, int64_t rows, int64_t dim, int64_t x_stride,
+                                          int8_t* out_q, float* out_scale, void* stream);
+
+/*
+ * out_logits[r, v] = ((float)(sum_k hidden[r, k] * weight[v, k]) * hidden_scale[r]) * weight_scale[v]
+ * in out_dtype (f32, or rounded once more to bf16), rows out_stride >= n_vocab elements apart; what lies between them
+ * stays as it was. The integer sum is exact, each product above is one f32 rounding: the logits do not depend on the
+ * device or the launch. hidden [rows, hidden_dim] and weight [n_vocab, hidden_dim] (ggml's lm_head layout) are packed
+ * and 16-byte aligned; hidden_dim is a multiple of 16, at most 65536 (LOOM_SELECT_ESHAPE otherwise). The workspace
+ * holds only the status word read by loom_select_read_status (a bounded wait that gave up), so calls on several
+ * streams may share it.
+ */
+LOOM_SELECT_API size_t loom_lm_head_logits_i8_workspace_size(int64_t rows, int64_t n_vocab);
+LOOM_SELECT_API int loom_lm_head_logits_i8(const int8_t* hidden, const float* hidden_scale, const int8_t* weight,
+                                           const float* weight_scale, int64_t rows, int64_t hidden_dim,
+                                           int64_t n_vocab, void* out_logits, int out_dtype, int64_t out_stride,
+                                           void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 } /* extern "C" */

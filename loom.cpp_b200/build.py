@@ -27,7 +27,9 @@ SOURCES = [("select_capi.cu", "select_capi.o", []),
            ("select_noalloc.cu", "select_noalloc.o", []),
            ("select_windows.cu", "select_windows.o", []),
            ("select_lmhead.cu", "select_lmhead.o", []),
-           ("select_logprobs.cu", "select_logprobs.o", [])]
+           ("select_logprobs.cu", "select_logprobs.o", []),
+           ("select_quant.cu", "select_quant.o", []),
+           ("select_lmhead_i8.cu", "select_lmhead_i8.o", [])]
 
 # sm_100a only. --fmad=false: no multiply-add contraction anywhere, so every float expression
 # rounds as written (the decision arithmetic also spells its operations as explicit intrinsics).

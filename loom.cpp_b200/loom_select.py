@@ -11,6 +11,8 @@ loom.cpp names on CUDA tensors:
     sample_rows(logits, ...)                 the sampling chain (no loom.cpp counterpart)
     shard_partial / shard_merge              the vocabulary-sharded chain (no loom.cpp counterpart)
     token_logprobs / token_logprobs_grad     log-probabilities of given tokens, and their gradient (none)
+    rms_norm_i8, quantize_rows_i8, lm_head_logits_i8
+                                             the final norm and the LM head in 8-bit integers (none)
 
 Errors raise SelectError, as loom.cpp raises loom::Error (include/loom/loom_errors.h:10) and its
 Lua bindings turn that into a Lua error (lua_bridge.cpp:26-32). The library must be present: there
@@ -66,6 +68,10 @@ EXPORTS = (
     "loom_lm_head_argmax",
     "loom_token_logprobs",
     "loom_token_logprobs_grad",
+    "loom_rms_norm_i8",
+    "loom_quantize_rows_i8",
+    "loom_lm_head_logits_i8_workspace_size",
+    "loom_lm_head_logits_i8",
 )
 
 
@@ -124,6 +130,12 @@ def _lib():
                                                    vp, vp]),
             "loom_token_logprobs_grad": (ctypes.c_int, [vp, ctypes.c_int, i64, i64, i64, vp, f32, vp, vp, vp, vp, vp,
                                                         i64, vp]),
+            "loom_rms_norm_i8": (ctypes.c_int, [vp, ctypes.c_int, i64, i64, i64, vp, i64, vp, ctypes.c_int,
+                                                ctypes.c_double, vp, vp, vp, i64, vp]),
+            "loom_quantize_rows_i8": (ctypes.c_int, [vp, ctypes.c_int, i64, i64, i64, vp, vp, vp]),
+            "loom_lm_head_logits_i8_workspace_size": (sz, [i64, i64]),
+            "loom_lm_head_logits_i8": (ctypes.c_int, [vp, vp, vp, vp, i64, i64, i64, vp, ctypes.c_int, i64, vp, sz,
+                                                      vp]),
         }
         for name, (res, args) in sig.items():
             f = getattr(lib, name)
@@ -549,3 +561,134 @@ def token_logprobs_grad(logits, ids, lse, grad_logp=None, grad_entropy=None, ent
     with _on(stream):
         out = _torch().empty(logits.shape, dtype=logits.dtype, device=logits.device)
     return token_logprobs_grad_into(logits, ids, lse, out, grad_logp, grad_entropy, entropy, temperature, stream)
+
+
+# ----------------------------------------------------------------------------------------------
+# the LM head in 8-bit integers
+
+def _matrix_view(t, name):
+    """(rows, dim, row_stride) of a 1-D or 2-D tensor with unit column stride."""
+    if t.dim() == 1:
+        return 1, t.shape[0], t.shape[0]
+    if t.dim() != 2 or t.stride(1) != 1:
+        raise SelectError(EINVAL, f"{name} must be [rows, dim] with contiguous rows")
+    return t.shape[0], t.shape[1], t.stride(0)
+
+
+def rms_norm_i8_into(x, weight, out_q, out_scale, residual=None, out_sum=None, eps=1e-6, stream=None):
+    """RMS norm of x (+ residual) [rows, dim] with weight [dim], as 8-bit integers with a scale per row (asynchronous).
+
+    out_q int8 [rows, dim], out_scale f32 [rows]; residual and out_sum (x + residual, which may be x or residual
+    itself) are like x or None. out_q * out_scale stands for the normed rows. See loom_rms_norm_i8."""
+    torch = _torch()
+    rows, dim, stride = _matrix_view(x, "x")
+    code, dev = _dtype_code(x), x.device
+    _check_device(x, "x")
+    wcode = _dtype_code(weight)
+    _check_tensor(weight, "weight", weight.dtype, (dim,), dev)
+    strides = []
+    for t, name in ((residual, "residual"), (out_sum, "out_sum")):
+        if t is not None:
+            if t.dtype != x.dtype:
+                raise SelectError(EDTYPE, f"{name} is {t.dtype}, expected {x.dtype}")
+            if t.shape != x.shape or t.device != dev:
+                raise SelectError(EINVAL, f"{name} must have x's shape and device")
+        strides.append(0 if t is None else _matrix_view(t, name)[2])
+    _check_tensor(out_q, "out_q", torch.int8, x.shape, dev)
+    _check_tensor(out_scale, "out_scale", torch.float32, (rows,), dev)
+    check(_lib().loom_rms_norm_i8(_ptr(x), code, rows, dim, stride, _ptr(residual), strides[0], _ptr(weight), wcode, eps,
+                                  _ptr(out_q), _ptr(out_scale), _ptr(out_sum), strides[1], _stream_handle(stream)),
+          "loom_rms_norm_i8")
+    return out_q, out_scale
+
+
+def rms_norm_i8(x, weight, residual=None, eps=1e-6, stream=None):
+    """(q int8, scale f32, x + residual or None) in new tensors."""
+    torch = _torch()
+    rows, _, _ = _matrix_view(x, "x")
+    with _on(stream):
+        q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+        total = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rms_norm_i8_into(x, weight, q, scale, residual, total, eps, stream)
+    return q, scale, total
+
+
+def quantize_rows_i8_into(x, out_q, out_scale, stream=None):
+    """Rows of x [rows, dim] as 8-bit integers with a scale per row (asynchronous): q * scale stands for x."""
+    torch = _torch()
+    rows, dim, stride = _matrix_view(x, "x")
+    code, dev = _dtype_code(x), x.device
+    _check_device(x, "x")
+    _check_tensor(out_q, "out_q", torch.int8, x.shape, dev)
+    _check_tensor(out_scale, "out_scale", torch.float32, (rows,), dev)
+    check(_lib().loom_quantize_rows_i8(_ptr(x), code, rows, dim, stride, _ptr(out_q), _ptr(out_scale),
+                                       _stream_handle(stream)), "loom_quantize_rows_i8")
+    return out_q, out_scale
+
+
+def quantize_rows_i8(x, stream=None):
+    """(q int8, scale f32) in new tensors: an LM-head weight [n_vocab, hidden_dim] for lm_head_logits_i8, say."""
+    torch = _torch()
+    rows, _, _ = _matrix_view(x, "x")
+    with _on(stream):
+        q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    return quantize_rows_i8_into(x, q, scale, stream)
+
+
+_STATUS_WS = {}
+
+
+def _status_workspace(stream):
+    """The workspace of a call that needs only the status word: one per device, never replaced. A captured call
+    gets one of its own (zeroed by the graph), which the graph's memory pool keeps."""
+    torch = _torch()
+    with _on(stream):
+        dev = torch.cuda.current_device()
+        capturing = torch.cuda.is_current_stream_capturing()
+        if not capturing and dev in _STATUS_WS:
+            return _STATUS_WS[dev]
+        ws = Workspace(torch.device("cuda", dev))
+        ws.get(256, stream)
+        if not capturing:
+            torch.cuda.current_stream().synchronize()  # zeroed before another stream's call reads it
+            _STATUS_WS[dev] = ws
+    return ws
+
+
+def lm_head_logits_i8_into(hidden, hidden_scale, weight, weight_scale, out, workspace=None, stream=None):
+    """out[r, v] = (hidden[r] . weight[v]) * hidden_scale[r] * weight_scale[v] (asynchronous).
+
+    hidden int8 [rows, hidden_dim] with hidden_scale f32 [rows], weight int8 [n_vocab, hidden_dim] with weight_scale
+    f32 [n_vocab], all contiguous; out f32 or bf16 [rows, n_vocab], rows of any stride. See loom_lm_head_logits_i8."""
+    torch = _torch()
+    if hidden.dim() not in (1, 2) or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+        raise SelectError(EINVAL, "hidden must be [rows, hidden_dim] and weight [n_vocab, hidden_dim]")
+    rows = 1 if hidden.dim() == 1 else hidden.shape[0]
+    n_vocab, hdim = weight.shape
+    dev = hidden.device
+    _check_device(hidden, "hidden")
+    _check_tensor(hidden, "hidden", torch.int8, hidden.shape, dev)
+    _check_tensor(hidden_scale, "hidden_scale", torch.float32, (rows,), dev)
+    _check_tensor(weight, "weight", torch.int8, weight.shape, dev)
+    _check_tensor(weight_scale, "weight_scale", torch.float32, (n_vocab,), dev)
+    code = _dtype_code(out)
+    if tuple(out.shape) != ((n_vocab,) if hidden.dim() == 1 else (rows, n_vocab)) or out.device != dev:
+        raise SelectError(EINVAL, "out must be [rows, n_vocab] on the hidden states' device")
+    _, _, stride = _rows_view(out)
+    ws = workspace or _status_workspace(stream)
+    buf = ws.get(256, stream)
+    check(_lib().loom_lm_head_logits_i8(_ptr(hidden), _ptr(hidden_scale), _ptr(weight), _ptr(weight_scale), rows, hdim,
+                                        n_vocab, _ptr(out), code, stride, _ptr(buf), buf.numel(),
+                                        _stream_handle(stream)), "loom_lm_head_logits_i8")
+    return out
+
+
+def lm_head_logits_i8(hidden, hidden_scale, weight, weight_scale, dtype=None, workspace=None, stream=None):
+    """lm_head_logits_i8_into a new tensor of `dtype` (f32 by default, or bf16)."""
+    torch = _torch()
+    shape = (weight.shape[0],) if hidden.dim() == 1 else (hidden.shape[0], weight.shape[0])
+    with _on(stream):
+        out = torch.empty(shape, dtype=dtype or torch.float32, device=hidden.device)
+    return lm_head_logits_i8_into(hidden, hidden_scale, weight, weight_scale, out, workspace, stream)

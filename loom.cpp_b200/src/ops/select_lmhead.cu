@@ -28,14 +28,13 @@
 // role winds down: the producer waits (again bounded) for the copies it issued, the MMA warp for the
 // MMAs it issued, then TMEM is freed.
 #include <cstdint>
-#include <cuda.h>
-#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 #include <mutex>
 
 #include "loom_select.h"
 #include "select_device.cuh"
 #include "select_internal.h"
+#include "select_tcgen05.cuh"
 
 namespace loom_select {
 namespace {
@@ -70,90 +69,6 @@ struct LmTile {
         (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(BN >> 3) << 17) | (uint32_t(kBM >> 4) << 24);
 };
 
-template <int kStages>
-struct LmBars {
-    uint64_t full[kStages];    // TMA -> MMA
-    uint64_t empty[kStages];   // MMA -> TMA
-    uint64_t tfull[2];         // MMA -> epilogue
-    uint64_t tempty[2];        // epilogue -> MMA (4 arrivals: one per epilogue warp)
-    uint64_t drain;            // the MMA warp's final commit
-    uint32_t tmem_base;
-    int abort;
-};
-
-// ---- tcgen05 / TMA wrappers ----
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
-            smem_addr(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(x), "r"(y)
-        : "memory");
-}
-
-// Shared-memory matrix descriptor of a K-major tile written by TMA with the 128-byte swizzle: rows of
-// 128 bytes, groups of 8 rows 1024 bytes apart (stride byte offset), descriptor version 1, layout
-// type 2 (128-byte swizzle). Stepping K by 16 elements inside the span adds 32 bytes to the start.
-__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr) {
-    uint64_t d = 0;
-    d |= uint64_t((saddr >> 4) & 0x3FFF);
-    d |= uint64_t(1) << 16;                    // leading byte offset (unused for swizzled K-major)
-    d |= uint64_t((1024 >> 4) & 0x3FFF) << 32; // stride byte offset
-    d |= uint64_t(1) << 46;                    // version
-    d |= uint64_t(2) << 61;                    // 128-byte swizzle
-    return d;
-}
-
-__device__ __forceinline__ void tc_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                       uint32_t accumulate) {
-    asm volatile(
-        "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-                 : "memory");
-}
-
-__device__ __forceinline__ void tc_ld32(uint32_t taddr, float (&v)[32]) {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-}
-
-__device__ __forceinline__ void tc_ld16(uint32_t taddr, float (&v)[16]) {
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-        "[%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
-}
-
-template <int W>
-__device__ __forceinline__ void tc_ld(uint32_t taddr, float (&v)[W]) {
-    if constexpr (W == 32) tc_ld32(taddr, v);
-    else tc_ld16(taddr, v);
-}
-
 // The running (maximum, lowest id) of one row over W logits at tile columns [c0, c0 + W).
 template <int W>
 __device__ __forceinline__ void scan_chunk(const float (&v)[W], int c0, int valid, float& bv, int& bi) {
@@ -183,22 +98,6 @@ __device__ __forceinline__ void sum_chunk(const float (&v)[W], int c0, int valid
         const int col = c0 + j;
         if (col < valid) s0 += fast_exp2(__fsub_rn(__fmul_rn(v[j], l2e), mb));
         if (col + 1 < valid) s1 += fast_exp2(__fsub_rn(__fmul_rn(v[j + 1], l2e), mb));
-    }
-}
-
-// Bounded wait that also gives up as soon as another role of the CTA has aborted.
-__device__ __forceinline__ bool lm_wait(uint64_t* bar, uint32_t parity, int* status, volatile int* abort_flag,
-                                        uint64_t limit_ns) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = global_timer_ns();
-    for (;;) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if (*abort_flag) return false;
-        if (global_timer_ns() - t0 > limit_ns) {
-            record_status(status, LOOM_SELECT_ETIMEOUT);
-            *abort_flag = 1;
-            return false;
-        }
     }
 }
 
@@ -469,20 +368,6 @@ __global__ void __launch_bounds__(256) lm_merge_kernel(const float4* __restrict_
         if (out_logit) out_logit[r] = zero ? qnan : p.m;
         if (out_lse && want_lse) out_lse[r] = zero ? qnan : p.m + logf(p.s);
     }
-}
-
-// cuTensorMapEncodeTiled through the runtime's driver entry point (no link against libcuda).
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    });
-    return fn;
 }
 
 bool make_map(CUtensorMap* m, const void* base, uint64_t inner, uint64_t outer, uint32_t box_outer) {
