@@ -297,7 +297,7 @@ LOOM_SELECT_API int loom_lm_head_argmax(const void* hidden, const void* weight, 
  *   - A NaN or +inf logit makes out_lse, out_logp, out_entropy and out_top_logp of its row NaN; a NaN is never an
  *     alternative (id -1, NaN, once nothing else is left), never ahead of a token, and has out_rank -1 itself.
  * Needs no workspace and keeps no state: calls on several streams, and graphs replayed at once, do not meet.
- * LOOM_SELECT_ESHAPE for rows beyond 2^27 - 1 or V beyond 2^31 - 1.
+ * LOOM_SELECT_ESHAPE for rows beyond 2^27 - 1 or V beyond 2^30.
  */
 LOOM_SELECT_API int loom_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t n_vocab,
                                         int64_t row_stride, const int32_t* ids, float temperature, int32_t n_top,

@@ -15,6 +15,7 @@
 // warps, of their lists' ceil(n_top / warps)-th values, seeded from the first elements' lane maxima.
 #include <cfloat>
 #include <cmath>
+#include <cooperative_groups.h>
 #include <cstdint>
 #include <cuda_runtime.h>
 
@@ -23,11 +24,14 @@
 #include "select_internal.h"
 #include "select_rows.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace loom_select {
 namespace {
 
 constexpr int kLpWarps = 8;
 constexpr int kLpNT = kLpWarps * 32;
+constexpr int64_t kMaxVocab = int64_t(1) << 30;  // ids, and steps past the last one, in 32 bits
 constexpr int kMaxTop = LOOM_SELECT_MAX_TOP_LOGPROBS;
 static_assert(kMaxTop <= 32, "a warp's list is one key per lane");
 constexpr float kLog2e = 1.4426950408889634f;
@@ -67,16 +71,10 @@ __device__ __forceinline__ SoftAcc soft_move(SoftAcc p, float M, float c) {
     return {M, p.s * f, f * __fmaf_rn(d, p.s, p.a)};
 }
 
-__device__ __forceinline__ SoftAcc soft_merge(SoftAcc p, SoftAcc q, float c) {
-    const float M = fmaxf(p.m, q.m);
-    p = soft_move(p, M, c);
-    q = soft_move(q, M, c);
-    return {M, p.s + q.s, p.a + q.a};
-}
-
 struct LpDev {
     const unsigned char* base;
-    int64_t width, row_stride;
+    int32_t width;
+    int64_t row_stride;
     const int32_t* ids;
     float T, c;
     int32_t n_top;
@@ -93,7 +91,10 @@ struct LpShared {
     int32_t ahead[kLpWarps];
     uint64_t list[kLpWarps][32];
     uint32_t wq[kLpWarps];  // per warp: order key of a value that ceil(n_top / warps) of its elements reach
-    float lns, m;
+    // the block's results, read by the cluster's first block
+    SoftAcc block_acc;
+    int32_t block_ahead;
+    uint64_t block_list[32];
 };
 
 // Descending bitonic sort of one float per lane.
@@ -123,6 +124,19 @@ __device__ __forceinline__ uint64_t merge_lists(uint64_t a, uint64_t b) {
     return a;
 }
 
+// The states of the warp's first `n` lanes (a power of two) as one, in every one of them: one rescale per
+// lane to the common maximum, then plain sums.
+__device__ __forceinline__ SoftAcc soft_reduce(SoftAcc p, int n, float c) {
+    float M = p.m;
+    for (int o = n >> 1; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    p = soft_move(p, M, c);
+    for (int o = n >> 1; o > 0; o >>= 1) {
+        p.s += __shfl_xor_sync(0xffffffffu, p.s, o);
+        p.a += __shfl_xor_sync(0xffffffffu, p.a, o);
+    }
+    return p;
+}
+
 // One thread's running state over its elements of a row.
 struct LpScan {
     SoftAcc acc;
@@ -131,32 +145,53 @@ struct LpScan {
     float own;      // smallest float that an element must reach to enter the warp's own list
 };
 
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+
 // Adds NE elements: x[j] has id id0 + (j / kPer) * step + j % kPer; elements whose id is not in
 // [0, limit) hold -inf and are neither counted nor listed. All lanes of the warp call it together.
 template <int NE, int kPer, bool kTop>
-__device__ __forceinline__ void scan_elems(const LpDev& p, LpShared* sh, LpScan& st, const float (&x)[NE], int64_t id0,
-                                           int64_t step, int64_t limit, float xt, int64_t t, bool rank) {
+__device__ __forceinline__ void scan_elems(const LpDev& p, LpShared* sh, LpScan& st, const float (&x)[NE], int32_t id0,
+                                           int32_t step, int32_t limit, float xt, int32_t t, bool rank) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     float mx = x[0];
 #pragma unroll
     for (int j = 1; j < NE; ++j) mx = fmaxf(mx, x[j]);
     if (mx > st.acc.m) st.acc = soft_move(st.acc, mx, p.c);
-    // (summed apart first: a thread's chain is one addition per call, not one per element)
-    const float m = st.acc.m;
-    float s = 0.0f, a = 0.0f;
+    // Two elements per instruction (f32x2); summed apart first: a thread's chain is one addition per
+    // call, not one per element.
+    const uint64_t mm = pack2(st.acc.m, st.acc.m), cc = pack2(p.c, p.c);
+    uint64_t s2 = 0, a2 = 0;
 #pragma unroll
-    for (int j = 0; j < NE; ++j) {
-        const float d = max_nan(__fmul_rn(__fsub_rn(x[j], m), p.c), kMinExp2);
-        const float e = ex2(d);
-        s += e;
-        a = __fmaf_rn(e, d, a);
+    for (int j = 0; j < NE; j += 2) {
+        uint64_t d = pack2(x[j], x[j + 1]);
+        asm("sub.rn.f32x2 %0, %0, %1;" : "+l"(d) : "l"(mm));
+        asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(d) : "l"(cc));
+        float d0, d1;
+        unpack2(d, d0, d1);
+        d0 = max_nan(d0, kMinExp2);
+        d1 = max_nan(d1, kMinExp2);
+        d = pack2(d0, d1);
+        const uint64_t e = pack2(ex2(d0), ex2(d1));
+        asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s2) : "l"(e));
+        asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a2) : "l"(e), "l"(d));
     }
-    st.acc.s += s;
-    st.acc.a += a;
+    float s0, s1, a0, a1;
+    unpack2(s2, s0, s1);
+    unpack2(a2, a0, a1);
+    st.acc.s += s0 + s1;
+    st.acc.a += a0 + a1;
     if (rank && mx >= xt) {
 #pragma unroll
         for (int j = 0; j < NE; ++j) {
-            const int64_t id = id0 + (j / kPer) * step + j % kPer;
+            const int32_t id = id0 + (j / kPer) * step + j % kPer;
             st.ahead += x[j] > xt || (x[j] == xt && id < t && id >= 0 && id < limit);
         }
     }
@@ -170,7 +205,7 @@ __device__ __forceinline__ void scan_elems(const LpDev& p, LpShared* sh, LpScan&
             uint32_t hits = 0;
 #pragma unroll
             for (int j = 0; j < NE; ++j) {
-                const int64_t id = id0 + (j / kPer) * step + j % kPer;
+                const int32_t id = id0 + (j / kPer) * step + j % kPer;
                 hits |= uint32_t(x[j] >= X && id >= 0 && id < limit) << j;
             }
             while (__any_sync(0xffffffffu, hits != 0)) {
@@ -181,7 +216,7 @@ __device__ __forceinline__ void scan_elems(const LpDev& p, LpShared* sh, LpScan&
                     float v = x[0];
 #pragma unroll
                     for (int j = 1; j < NE; ++j) v = j == at ? x[j] : v;
-                    cand = loom_rank_key(v, int32_t(id0 + (at / kPer) * step + at % kPer));
+                    cand = loom_rank_key(v, id0 + (at / kPer) * step + at % kPer);
                 }
                 uint64_t last = __shfl_sync(0xffffffffu, st.key, p.n_top - 1);
                 uint32_t b = __ballot_sync(0xffffffffu, cand > last);
@@ -214,93 +249,144 @@ __device__ __forceinline__ void seed_threshold(const LpDev& p, LpShared* sh, flo
     __syncthreads();
 }
 
+// A cluster of blocks per row: block b of C takes every C-th step of kU * kLpNT vectors. Each block
+// reduces its share; the cluster's first block reads the others' results from their shared memory.
+// No workspace, tickets or waits between clusters.
 template <int kDtype, bool kTop>
 __global__ void __launch_bounds__(kLpNT) token_logprobs_kernel(const LpDev p) {
     constexpr int kEsz = kDtype == LOOM_SELECT_BF16 ? 2 : 4;
     constexpr int kPer = 16 / kEsz;
     constexpr int kU = 16 / kPer;  // vectors per thread and step: 16 elements
     __shared__ LpShared sh;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int C = int(cluster.num_blocks()), rank_in = int(cluster.block_rank());
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t row = blockIdx.x;
+    const int64_t row = blockIdx.x / unsigned(C);
     const unsigned char* rowp = p.base + row * p.row_stride * kEsz;
     // the row as 16-byte aligned vectors: vector v holds ids [v kPer - shift, (v + 1) kPer - shift)
-    const int shift = int((reinterpret_cast<uintptr_t>(rowp) & 15) / kEsz);
-    const int64_t nv = (shift + p.width + kPer - 1) / kPer;
-    const int64_t v0 = shift ? 1 : 0;                            // first vector inside the row
-    const int64_t v1 = (shift + p.width) / kPer > v0 ? (shift + p.width) / kPer : v0;  // end of those inside it
+    const int32_t shift = int32_t((reinterpret_cast<uintptr_t>(rowp) & 15) / kEsz);
+    const int32_t nv = (shift + p.width + kPer - 1) / kPer;
+    const int32_t v0 = shift ? 1 : 0;                                                // first vector inside the row
+    const int32_t v1 = max((shift + p.width) / kPer, v0);                            // end of those inside it
+    const int32_t limit = v1 * kPer - shift;  // (an id past the whole vectors may be inside the row: an edge's)
+    const unsigned char* vec = rowp - shift * kEsz;
+    const int32_t stride = C * kU * kLpNT;
 
-    const int64_t t = p.ids ? p.ids[row] : -1;
+    uint4 raw[kU];
+    auto load = [&](int32_t v) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int32_t vu = v + lane + u * kLpNT;
+            if (vu < v1) {
+                raw[u] = ldg_stream_v4(vec + int64_t(vu) * 16);
+            } else {  // -inf throughout
+                const uint32_t w = kDtype == LOOM_SELECT_BF16 ? 0xff80ff80u : 0xff800000u;
+                raw[u] = make_uint4(w, w, w, w);
+            }
+        }
+    };
+    int32_t v = v0 + rank_in * kU * kLpNT + warp * 32;
+    load(v);
+    const int32_t t = p.ids ? p.ids[row] : -1;
     const bool has = t >= 0 && t < p.width;
     const float xt = has ? load_global_elem<kDtype>(rowp, t) : quiet_nan();
     const bool rank = p.out_rank != nullptr && has;
 
     LpScan st{soft_init(), 0, 0ull, neg_inf()};
     // vectors that the row only partly fills: the first (lowest ids, added first) and the last
-    auto edge = [&](int64_t v, bool there) {
+    auto edge = [&](int32_t v, bool there) {
         float x[kPer];
-        const int64_t id0 = v * kPer - shift;
+        const int32_t id0 = v * kPer - shift;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-            const int64_t id = id0 + j;
+            const int32_t id = id0 + j;
             x[j] = there && id >= 0 && id < p.width ? load_global_elem<kDtype>(rowp, id) : neg_inf();
         }
         scan_elems<kPer, kPer, kTop>(p, &sh, st, x, there ? id0 : -kPer, 0, p.width, xt, t, rank);
     };
-    const unsigned char* vec = rowp - shift * kEsz;
-    auto load = [&](int64_t v, float (&x)[16]) {
+    if constexpr (kTop) {
+        float mx = neg_inf();
+#pragma unroll
+        for (int u = 0; u < kU; ++u) mx = fmaxf(mx, vec_max<kDtype>(raw[u]));  // (NaN left out)
+        seed_threshold(p, &sh, mx);
+    }
+    if (warp == 0 && rank_in == 0 && v0 > 0) edge(0, lane == 0);
+    while (v < v1) {  // warp-uniform
+        float x[16];
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-            const int64_t vu = v + lane + u * kLpNT;
             Vec16<kDtype> e;
-            if (vu < v1) {
-                e.unpack(ldg_stream_v4(vec + vu * 16));
-            } else {
-#pragma unroll
-                for (int q = 0; q < kPer; ++q) e.x[q] = neg_inf();
-            }
+            e.unpack(raw[u]);
 #pragma unroll
             for (int q = 0; q < kPer; ++q) x[u * kPer + q] = e.x[q];
         }
-    };
-    const int64_t limit = v1 * kPer - shift;  // (an id past the whole vectors may be inside the row: an edge's)
-    int64_t v = v0 + warp * 32;
-    float x[16];
-    load(v, x);
-    if constexpr (kTop) {
-        float mx = x[0];
-#pragma unroll
-        for (int j = 1; j < 16; ++j) mx = fmaxf(mx, x[j]);
-        seed_threshold(p, &sh, fmaxf(mx, neg_inf()));
+        const int32_t id0 = (v + lane) * kPer - shift;
+        v += stride;
+        if (v < v1) load(v);  // the next step's loads are in flight while this one is added
+        scan_elems<16, kPer, kTop>(p, &sh, st, x, id0, kLpNT * kPer, limit, xt, t, rank);
     }
-    if (warp == 0 && v0 > 0) edge(0, lane == 0);
-    while (v < v1) {  // warp-uniform
-        scan_elems<16, kPer, kTop>(p, &sh, st, x, (v + lane) * kPer - shift, int64_t(kLpNT) * kPer, limit, xt, t, rank);
-        v += kU * kLpNT;
-        if (v < v1) load(v, x);
-    }
-    if (warp == 0 && v1 < nv && nv - 1 >= v0) edge(nv - 1, lane == 0);
+    // (the last vector's ids are above all others: after every step of its warp)
+    if (warp == 0 && rank_in == 0 && v1 < nv && nv - 1 >= v0) edge(nv - 1, lane == 0);
 
-    // warp, then block
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        SoftAcc q{__shfl_xor_sync(0xffffffffu, st.acc.m, o), __shfl_xor_sync(0xffffffffu, st.acc.s, o),
-                  __shfl_xor_sync(0xffffffffu, st.acc.a, o)};
-        st.acc = soft_merge(st.acc, q, p.c);
-        st.ahead += __shfl_xor_sync(0xffffffffu, st.ahead, o);
-    }
+    // warp, block, cluster
+    SoftAcc acc = soft_reduce(st.acc, 32, p.c);
+    int32_t ahead = __reduce_add_sync(0xffffffffu, st.ahead);
     if (lane == 0) {
-        sh.acc[warp] = st.acc;
-        sh.ahead[warp] = st.ahead;
+        sh.acc[warp] = acc;
+        sh.ahead[warp] = ahead;
     }
-    if constexpr (kTop) sh.list[warp][lane] = st.key;
-    __syncthreads();
-    if (warp != 0) return;
-    SoftAcc acc = sh.acc[0];
-    int32_t ahead = sh.ahead[0];
-    for (int w = 1; w < kLpWarps; ++w) {
-        acc = soft_merge(acc, sh.acc[w], p.c);
-        ahead += sh.ahead[w];
+    uint64_t key = st.key;
+    if constexpr (kTop) {
+        // lists by halves: warp w takes in warp w + n's
+#pragma unroll
+        for (int n = kLpWarps / 2; n > 0; n >>= 1) {
+            if (warp >= n && warp < 2 * n) sh.list[warp][lane] = key;
+            __syncthreads();
+            if (warp < n) key = merge_lists(key, sh.list[warp + n][lane]);
+        }
+    } else {
+        __syncthreads();
     }
+    if (warp == 0) {
+        acc = lane < kLpWarps ? sh.acc[lane] : soft_init();
+        acc = soft_reduce(acc, 32, p.c);
+        ahead = __reduce_add_sync(0xffffffffu, lane < kLpWarps ? sh.ahead[lane] : 0);
+    }
+    if (C > 1) {
+        if (warp == 0) {
+            if (lane == 0) {
+                sh.block_acc = acc;
+                sh.block_ahead = ahead;
+            }
+            if constexpr (kTop) sh.block_list[lane] = key;
+        }
+        cluster.sync();
+        if (rank_in == 0) {
+            if constexpr (kTop) {
+                // (C is at most kLpWarps: warp b takes block b's list)
+                if (warp < C) key = cluster.map_shared_rank(&sh, warp)->block_list[lane];
+                for (int n = C / 2; n > 0; n >>= 1) {
+                    if (warp >= n && warp < 2 * n) sh.list[warp][lane] = key;
+                    __syncthreads();
+                    if (warp < n) key = merge_lists(key, sh.list[warp + n][lane]);
+                }
+            }
+            if (warp == 0) {
+                acc = soft_init();
+                ahead = 0;
+                if (lane < C) {
+                    const LpShared* other = cluster.map_shared_rank(&sh, lane);
+                    acc = other->block_acc;
+                    ahead = other->block_ahead;
+                }
+                acc = soft_reduce(acc, 32, p.c);
+                ahead = __reduce_add_sync(0xffffffffu, ahead);
+            }
+        }
+        cluster.sync();  // no block's shared memory goes away before it has been read
+    }
+    if (warp != 0 || rank_in != 0) return;
+
     const float lns = logf(acc.s);  // -inf for an empty row, NaN where a logit was NaN or +inf
     const bool empty = acc.s == 0.0f;
     if (lane == 0) {
@@ -315,8 +401,6 @@ __global__ void __launch_bounds__(kLpNT) token_logprobs_kernel(const LpDev p) {
         if (p.out_rank) p.out_rank[row] = has && xt == xt ? ahead : -1;
     }
     if constexpr (kTop) {
-        uint64_t key = st.key;
-        for (int w = 1; w < kLpWarps; ++w) key = merge_lists(key, sh.list[w][lane]);
         if (lane < p.n_top) {
             const float v = rank_key_value(key);
             if (p.out_top_ids) p.out_top_ids[row * p.n_top + lane] = key ? rank_key_id(key) : -1;
@@ -325,6 +409,30 @@ __global__ void __launch_bounds__(kLpNT) token_logprobs_kernel(const LpDev p) {
                     empty || !key ? quiet_nan() : __fdiv_rn(__fsub_rn(v, acc.m), p.T) - lns;
         }
     }
+}
+
+// Blocks per row: as many as it takes to fill the GPU (kLpBlocksPerSm resident blocks each), at most 8 (a portable
+// cluster), and no more than there are steps of 16 elements a thread in a row.
+constexpr int kLpBlocksPerSm = 4;
+int lp_cluster(int64_t rows, int64_t n_vocab, int sms) {
+    int c = 1;
+    while (c < 8 && rows * c < int64_t(kLpBlocksPerSm) * sms && n_vocab > int64_t(c) * 16 * kLpNT) c *= 2;
+    return c;
+}
+
+template <int kDtype, bool kTop>
+cudaError_t launch_lp(const LpDev& p, int64_t rows, int C, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(rows * C));
+    cfg.blockDim = dim3(kLpNT);
+    cfg.stream = s;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = unsigned(C);
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<kDtype, kTop>, p);
 }
 
 // ---- the gradient ----
@@ -418,10 +526,10 @@ LOOM_SELECT_API int loom_token_logprobs(const void* logits, int dtype, int64_t r
     if (!temperature_ok(temperature)) return LOOM_SELECT_EPARAM;
     if (n_top < 0 || n_top > kMaxTop || n_top > n_vocab) return LOOM_SELECT_EPARAM;
     if ((n_top > 0) != (out_top_ids || out_top_logp)) return LOOM_SELECT_EINVAL;
-    if (n_vocab > INT32_MAX || rows > INT32_MAX / 16) return LOOM_SELECT_ESHAPE;
+    if (n_vocab > kMaxVocab || rows > INT32_MAX / 16) return LOOM_SELECT_ESHAPE;
     LpDev p;
     p.base = static_cast<const unsigned char*>(logits);
-    p.width = n_vocab;
+    p.width = int32_t(n_vocab);
     p.row_stride = row_stride;
     p.ids = ids;
     p.T = temperature;
@@ -433,16 +541,17 @@ LOOM_SELECT_API int loom_token_logprobs(const void* logits, int dtype, int64_t r
     p.out_rank = out_rank;
     p.out_top_ids = out_top_ids;
     p.out_top_logp = out_top_logp;
+    int st = LOOM_SELECT_OK;
+    const int sms = device_sm_count(&st);
+    if (st != LOOM_SELECT_OK) return st;
+    const int C = lp_cluster(rows, n_vocab, sms);
     const auto s = static_cast<cudaStream_t>(stream);
-    const unsigned grid = unsigned(rows);
-    if (dtype == LOOM_SELECT_BF16) {
-        if (n_top) token_logprobs_kernel<LOOM_SELECT_BF16, true><<<grid, kLpNT, 0, s>>>(p);
-        else token_logprobs_kernel<LOOM_SELECT_BF16, false><<<grid, kLpNT, 0, s>>>(p);
-    } else {
-        if (n_top) token_logprobs_kernel<LOOM_SELECT_F32, true><<<grid, kLpNT, 0, s>>>(p);
-        else token_logprobs_kernel<LOOM_SELECT_F32, false><<<grid, kLpNT, 0, s>>>(p);
-    }
-    return cudaGetLastError() == cudaSuccess ? LOOM_SELECT_OK : LOOM_SELECT_ECUDA;
+    cudaError_t e;
+    if (dtype == LOOM_SELECT_BF16)
+        e = n_top ? launch_lp<LOOM_SELECT_BF16, true>(p, rows, C, s) : launch_lp<LOOM_SELECT_BF16, false>(p, rows, C, s);
+    else
+        e = n_top ? launch_lp<LOOM_SELECT_F32, true>(p, rows, C, s) : launch_lp<LOOM_SELECT_F32, false>(p, rows, C, s);
+    return e == cudaSuccess ? LOOM_SELECT_OK : LOOM_SELECT_ECUDA;
 }
 
 LOOM_SELECT_API int loom_token_logprobs_grad(const void* logits, int dtype, int64_t rows, int64_t n_vocab,
@@ -458,7 +567,7 @@ LOOM_SELECT_API int loom_token_logprobs_grad(const void* logits, int dtype, int6
         misaligned(lse, 4) || misaligned(entropy, 4) || misaligned(grad_logp, 4) || misaligned(grad_entropy, 4))
         return LOOM_SELECT_EINVAL;
     if (!temperature_ok(temperature)) return LOOM_SELECT_EPARAM;
-    if (n_vocab > INT32_MAX || rows > INT32_MAX / 16) return LOOM_SELECT_ESHAPE;
+    if (n_vocab > kMaxVocab || rows > INT32_MAX / 16) return LOOM_SELECT_ESHAPE;
     // in place only element for element
     if (logits == out_grad && row_stride != grad_stride) return LOOM_SELECT_EINVAL;
     LpGradDev p;
