@@ -8,11 +8,6 @@
 // maximum rises (A moves with m: sum e^(y - M)(y - M) = f (A + (m - M) S), f = e^(m - M)). Everything is
 // held in f32: A <= 0 <= ln S, so H has no cancellation, and a thread adds at most a few thousand terms.
 // Bound: HBM (each logit read once).
-//
-// Alternatives: each warp keeps the best 32 of its elements as 64-bit rank keys (value, then lower id),
-// one per lane, sorted. Few elements get as far as the list: a lane compares the maximum of its elements
-// with a threshold that at least n_top elements of the row reach -- the smallest, over the block's
-// warps, of their lists' ceil(n_top / warps)-th values, seeded from the first elements' lane maxima.
 #include <cfloat>
 #include <cmath>
 #include <cooperative_groups.h>
@@ -29,8 +24,6 @@ namespace cg = cooperative_groups;
 namespace loom_select {
 namespace {
 
-constexpr int kLpWarps = 8;
-constexpr int kLpNT = kLpWarps * 32;
 constexpr int64_t kMaxVocab = int64_t(1) << 30;  // ids, and steps past the last one, in 32 bits
 constexpr int kMaxTop = LOOM_SELECT_MAX_TOP_LOGPROBS;
 static_assert(kMaxTop <= 32, "a warp's list is one key per lane");
@@ -86,26 +79,38 @@ struct LpDev {
     float* out_top_logp;
 };
 
+#ifndef LP_MINB
+#define LP_MINB 4
+#endif
+#ifndef LP_MINB1
+#define LP_MINB1 24
+#endif
+// A thread keeps the maxima of its elements in up to this many equal runs of steps.
+constexpr int kSlots = 32;
+
+template <int kW>
 struct LpShared {
-    SoftAcc acc[kLpWarps];
-    int32_t ahead[kLpWarps];
-    uint64_t list[kLpWarps][32];
-    uint32_t wq[kLpWarps];  // per warp: order key of a value that ceil(n_top / warps) of its elements reach
+    SoftAcc acc[kW];
+    int32_t ahead[kW];
+    uint64_t list[kW][32];
+    uint32_t wq[kW];           // per warp: order key of a value that ceil(n_top / kW) of its lanes' maxima reach
+    uint16_t queue[kW][64];    // per warp: (slot, lane) groups to look through
+    float slot_max[kW][kSlots][32];
     // the block's results, read by the cluster's first block
     SoftAcc block_acc;
     int32_t block_ahead;
     uint64_t block_list[32];
 };
 
-// Descending bitonic sort of one float per lane.
-__device__ __forceinline__ float sort_desc(float v) {
+// Descending bitonic sort of one key per lane.
+__device__ __forceinline__ uint64_t sort_desc(uint64_t v) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1) {
 #pragma unroll
         for (int stride = size >> 1; stride > 0; stride >>= 1) {
-            const float o = __shfl_xor_sync(0xffffffffu, v, stride);
-            v = (((lane & stride) == 0) == ((lane & size) == 0)) ? fmaxf(v, o) : fminf(v, o);
+            const uint64_t o = __shfl_xor_sync(0xffffffffu, v, stride);
+            v = ((((lane & stride) == 0) == ((lane & size) == 0)) == (v > o)) ? v : o;
         }
     }
     return v;
@@ -137,14 +142,6 @@ __device__ __forceinline__ SoftAcc soft_reduce(SoftAcc p, int n, float c) {
     return p;
 }
 
-// One thread's running state over its elements of a row.
-struct LpScan {
-    SoftAcc acc;
-    int32_t ahead;
-    uint64_t key;   // this lane's entry of the warp's list
-    float own;      // smallest float that an element must reach to enter the warp's own list
-};
-
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -155,128 +152,161 @@ __device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
 }
 
-// Adds NE elements: x[j] has id id0 + (j / kPer) * step + j % kPer; elements whose id is not in
-// [0, limit) hold -inf and are neither counted nor listed. All lanes of the warp call it together.
-template <int NE, int kPer, bool kTop>
-__device__ __forceinline__ void scan_elems(const LpDev& p, LpShared* sh, LpScan& st, const float (&x)[NE], int32_t id0,
-                                           int32_t step, int32_t limit, float xt, int32_t t, bool rank) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    float mx = x[0];
+// 1 where a > b, else 0 (NaN: 0).
+__device__ __forceinline__ float gt_one(float a, float b) {
+    float y;
+    asm("set.gt.f32.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// The largest float below x (x finite or +inf; one below either zero).
+__device__ __forceinline__ float float_below(float x) {
+    return order_key_to_float(loom_order_key(x) - (x == 0.0f ? 2u : 1u));
+}
+
+// One thread's running softmax sums and rank count over its elements of a row. Elements come NE at a time: x[j]
+// has id id0 + (j / kPer) * step + j % kPer; those whose id is not in [0, limit) hold -inf and are not counted.
+template <int kPer>
+struct LpScan {
+    SoftAcc acc;
+    float c;
+    // the rank: ids before t count when x > xt_below, i.e. x >= xt, ids after it when x > xt
+    float xt, xt_below;
+    int32_t t;
+    uint64_t ahead2;  // two f32 counts (exact: a thread has far fewer than 2^24 elements)
+
+    // Softmax terms, two elements per instruction (f32x2). They are summed apart first: a thread's chain is
+    // one addition per call, not one per element.
+    template <int NE>
+    __device__ __forceinline__ void add(const float (&x)[NE], float mx) {
+        if (mx > acc.m) acc = soft_move(acc, mx, c);
+        const uint64_t mm = pack2(acc.m, acc.m), cc = pack2(c, c);
+        uint64_t s2 = 0, a2 = 0;
 #pragma unroll
-    for (int j = 1; j < NE; ++j) mx = fmaxf(mx, x[j]);
-    if (mx > st.acc.m) st.acc = soft_move(st.acc, mx, p.c);
-    // Two elements per instruction (f32x2); summed apart first: a thread's chain is one addition per
-    // call, not one per element.
-    const uint64_t mm = pack2(st.acc.m, st.acc.m), cc = pack2(p.c, p.c);
-    uint64_t s2 = 0, a2 = 0;
-#pragma unroll
-    for (int j = 0; j < NE; j += 2) {
-        uint64_t d = pack2(x[j], x[j + 1]);
-        asm("sub.rn.f32x2 %0, %0, %1;" : "+l"(d) : "l"(mm));
-        asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(d) : "l"(cc));
-        float d0, d1;
-        unpack2(d, d0, d1);
-        d0 = max_nan(d0, kMinExp2);
-        d1 = max_nan(d1, kMinExp2);
-        d = pack2(d0, d1);
-        const uint64_t e = pack2(ex2(d0), ex2(d1));
-        asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s2) : "l"(e));
-        asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a2) : "l"(e), "l"(d));
-    }
-    float s0, s1, a0, a1;
-    unpack2(s2, s0, s1);
-    unpack2(a2, a0, a1);
-    st.acc.s += s0 + s1;
-    st.acc.a += a0 + a1;
-    if (rank && mx >= xt) {
-#pragma unroll
-        for (int j = 0; j < NE; ++j) {
-            const int32_t id = id0 + (j / kPer) * step + j % kPer;
-            st.ahead += x[j] > xt || (x[j] == xt && id < t && id >= 0 && id < limit);
+        for (int j = 0; j < NE; j += 2) {
+            uint64_t d = pack2(x[j], x[j + 1]);
+            asm("sub.rn.f32x2 %0, %0, %1;" : "+l"(d) : "l"(mm));
+            asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(d) : "l"(cc));
+            float d0, d1;
+            unpack2(d, d0, d1);
+            d0 = max_nan(d0, kMinExp2);
+            d1 = max_nan(d1, kMinExp2);
+            d = pack2(d0, d1);
+            const uint64_t e = pack2(ex2(d0), ex2(d1));
+            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s2) : "l"(e));
+            asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a2) : "l"(e), "l"(d));
         }
+        float s0, s1, a0, a1;
+        unpack2(s2, s0, s1);
+        unpack2(a2, a0, a1);
+        acc.s += s0 + s1;
+        acc.a += a0 + a1;
     }
-    if constexpr (kTop) {
-        // the row's threshold: what every warp's wq vouches for together
-        uint32_t q = 0xffffffffu;
-        if (lane < kLpWarps) q = *reinterpret_cast<volatile uint32_t*>(&sh->wq[lane]);
-        q = __reduce_min_sync(0xffffffffu, q);
-        const float X = fmaxf(order_key_to_float(q), st.own);
-        if (__any_sync(0xffffffffu, mx >= X)) {
-            uint32_t hits = 0;
+
+    // Ids ahead of t. lo and hi bound the warp's ids of this call (as warp-uniform values).
+    template <int NE>
+    __device__ __forceinline__ void count(const float (&x)[NE], float mx, int32_t id0, int32_t step, int32_t limit,
+                                          int32_t lo, int32_t hi) {
+        if (!__any_sync(0xffffffffu, mx >= xt)) return;
+        const bool before = hi <= t;
+        if ((before || lo > t) && xt > neg_inf()) {
+            const float g = before ? xt_below : xt;
+#pragma unroll
+            for (int j = 0; j < NE; j += 2) {
+                const uint64_t n = pack2(gt_one(x[j], g), gt_one(x[j + 1], g));
+                asm("add.rn.f32x2 %0, %0, %1;" : "+l"(ahead2) : "l"(n));
+            }
+        } else {
+            float n = 0.0f;
 #pragma unroll
             for (int j = 0; j < NE; ++j) {
                 const int32_t id = id0 + (j / kPer) * step + j % kPer;
-                hits |= uint32_t(x[j] >= X && id >= 0 && id < limit) << j;
+                n += x[j] > xt || (x[j] == xt && id < t && id >= 0 && id < limit) ? 1.0f : 0.0f;
             }
-            while (__any_sync(0xffffffffu, hits != 0)) {
-                uint64_t cand = 0;
-                if (hits) {
-                    const int at = __ffs(hits) - 1;
-                    hits &= hits - 1;
-                    float v = x[0];
+            const uint64_t n2 = pack2(n, 0.0f);
+            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(ahead2) : "l"(n2));
+        }
+    }
+
+};
+
+// One lane's share of the row in one slot: `n` steps from vector `v` on, kU vectors (kNT apart) to a step, `stride`
+// vectors between steps. Appends, for every lane at once, the elements >= X to the warp's list of the best 32 keys:
+// in each round every lane offers its best element not offered yet, and the offers, sorted, are merged in.
+template <int kDtype, int kU, int kNT>
+__device__ __forceinline__ void list_group(uint64_t& key, int n_top, const unsigned char* vec, int32_t shift, int32_t v,
+                                           int32_t v1, int32_t stride, int n, bool there, float X) {
+    constexpr int kPer = kDtype == LOOM_SELECT_BF16 ? 8 : 4;
+    for (int i = 0; i < n; ++i) {
+        uint4 raw[kU];
+        const int32_t at = v + i * stride;
 #pragma unroll
-                    for (int j = 1; j < NE; ++j) v = j == at ? x[j] : v;
-                    cand = loom_rank_key(v, id0 + (at / kPer) * step + at % kPer);
-                }
-                uint64_t last = __shfl_sync(0xffffffffu, st.key, p.n_top - 1);
-                uint32_t b = __ballot_sync(0xffffffffu, cand > last);
-                while (b) {
-                    const int src = __ffs(b) - 1;
-                    b &= b - 1;
-                    const uint64_t k = __shfl_sync(0xffffffffu, cand, src);
-                    const int pos = __popc(__ballot_sync(0xffffffffu, st.key > k));
-                    const uint64_t up = __shfl_up_sync(0xffffffffu, st.key, 1);
-                    if (lane == pos) st.key = k;
-                    else if (lane > pos) st.key = up;
+        for (int u = 0; u < kU; ++u) {
+            const uint32_t w = kDtype == LOOM_SELECT_BF16 ? 0xffffffffu : 0x7fffffffu;  // NaN: never an alternative
+            raw[u] = make_uint4(w, w, w, w);
+            if (there && at + u * kNT < v1) raw[u] = ldg_stream_v4(vec + int64_t(at + u * kNT) * 16);
+        }
+        uint64_t below = ~0ull;  // keys from here on have been offered
+        for (;;) {
+            uint64_t best = 0;
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                Vec16<kDtype> e;
+                e.unpack(raw[u]);
+#pragma unroll
+                for (int q = 0; q < kPer; ++q) {
+                    if (e.x[q] >= X) {
+                        const uint64_t k = loom_rank_key(e.x[q], (at + u * kNT) * kPer - shift + q);
+                        best = k < below && k > best ? k : best;
+                    }
                 }
             }
-            // later elements of this warp have higher ids: an equal value cannot displace the last entry
-            const uint64_t last = __shfl_sync(0xffffffffu, st.key, p.n_top - 1);
-            if (last) st.own = order_key_to_float(uint32_t(last >> 32) + 1);
-            const uint64_t qth = __shfl_sync(0xffffffffu, st.key, (p.n_top + kLpWarps - 1) / kLpWarps - 1);
-            if (lane == 0 && uint32_t(qth >> 32) > sh->wq[warp])
-                *reinterpret_cast<volatile uint32_t*>(&sh->wq[warp]) = uint32_t(qth >> 32);
+            const uint64_t last = __shfl_sync(0xffffffffu, key, n_top - 1);
+            if (best <= last) best = 0;
+            if (!__any_sync(0xffffffffu, best != 0)) break;
+            if (best) below = best;
+            key = merge_lists(key, sort_desc(best));
         }
     }
 }
 
-// The first threshold: each warp's ceil(n_top / warps)-th largest lane maximum is reached by that
-// many of its elements. Every thread of the block calls it with the maximum of its first elements.
-__device__ __forceinline__ void seed_threshold(const LpDev& p, LpShared* sh, float mx) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const float v = __shfl_sync(0xffffffffu, sort_desc(mx), (p.n_top + kLpWarps - 1) / kLpWarps - 1);
-    if (lane == 0) sh->wq[warp] = loom_order_key(v);
-    __syncthreads();
-}
-
-// A cluster of blocks per row: block b of C takes every C-th step of kU * kLpNT vectors. Each block
+// A cluster of C blocks of kW warps per row: block b takes every C-th step of kU vectors per thread. Each block
 // reduces its share; the cluster's first block reads the others' results from their shared memory.
 // No workspace, tickets or waits between clusters.
-template <int kDtype, bool kTop>
-__global__ void __launch_bounds__(kLpNT) token_logprobs_kernel(const LpDev p) {
+//
+// Alternatives: while streaming, a thread only notes the largest element of each slot (a run of steps). At the end
+// the ceil(n_top / kW)-th largest of each warp's 32 thread maxima, the smallest of the warps' values, is a threshold X
+// that at least n_top elements of the block reach, and few more do (n_top of 256 threads). The slots whose maximum
+// reaches X are read again, from L2, and their elements >= X sorted into the warps' lists.
+template <int kDtype, bool kTop, int kW>
+__global__ void __launch_bounds__(kW * 32, kW == 1 ? LP_MINB1 : LP_MINB) token_logprobs_kernel(const LpDev p) {
     constexpr int kEsz = kDtype == LOOM_SELECT_BF16 ? 2 : 4;
     constexpr int kPer = 16 / kEsz;
-    constexpr int kU = 16 / kPer;  // vectors per thread and step: 16 elements
-    __shared__ LpShared sh;
+    constexpr int kU = 4;                // vectors per thread and step
+    constexpr int kPart = 16 / kPer;     // vectors added at a time: 16 elements
+    constexpr int kNT = kW * 32;
+    __shared__ LpShared<kW> sh;
     const cg::cluster_group cluster = cg::this_cluster();
     const int C = int(cluster.num_blocks()), rank_in = int(cluster.block_rank());
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t row = blockIdx.x / unsigned(C);
     const unsigned char* rowp = p.base + row * p.row_stride * kEsz;
     // the row as 16-byte aligned vectors: vector v holds ids [v kPer - shift, (v + 1) kPer - shift)
     const int32_t shift = int32_t((reinterpret_cast<uintptr_t>(rowp) & 15) / kEsz);
     const int32_t nv = (shift + p.width + kPer - 1) / kPer;
-    const int32_t v0 = shift ? 1 : 0;                                                // first vector inside the row
-    const int32_t v1 = max((shift + p.width) / kPer, v0);                            // end of those inside it
+    const int32_t v0 = shift ? 1 : 0;                      // first vector inside the row
+    const int32_t v1 = max((shift + p.width) / kPer, v0);  // end of those inside it
     const int32_t limit = v1 * kPer - shift;  // (an id past the whole vectors may be inside the row: an edge's)
     const unsigned char* vec = rowp - shift * kEsz;
-    const int32_t stride = C * kU * kLpNT;
+    const int32_t stride = C * kU * kNT;
+    const int32_t steps = (v1 - v0 + stride - 1) / stride;
+    const int32_t per_slot = (steps + kSlots - 1) / kSlots;
 
     uint4 raw[kU];
     auto load = [&](int32_t v) {
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-            const int32_t vu = v + lane + u * kLpNT;
+            const int32_t vu = v + lane + u * kNT;
             if (vu < v1) {
                 raw[u] = ldg_stream_v4(vec + int64_t(vu) * 16);
             } else {  // -inf throughout
@@ -285,107 +315,180 @@ __global__ void __launch_bounds__(kLpNT) token_logprobs_kernel(const LpDev p) {
             }
         }
     };
-    int32_t v = v0 + rank_in * kU * kLpNT + warp * 32;
+    const int32_t v_start = v0 + rank_in * kU * kNT + warp * 32;
+    int32_t v = v_start;
     load(v);
+
+    LpScan<kPer> st;
+    st.acc = soft_init();
+    st.c = p.c;
+    st.ahead2 = 0;
     const int32_t t = p.ids ? p.ids[row] : -1;
     const bool has = t >= 0 && t < p.width;
-    const float xt = has ? load_global_elem<kDtype>(rowp, t) : quiet_nan();
+    st.t = t;
+    st.xt = has ? load_global_elem<kDtype>(rowp, t) : quiet_nan();
+    st.xt_below = float_below(st.xt);
     const bool rank = p.out_rank != nullptr && has;
+    const float xt = st.xt;
 
-    LpScan st{soft_init(), 0, 0ull, neg_inf()};
-    // vectors that the row only partly fills: the first (lowest ids, added first) and the last
-    auto edge = [&](int32_t v, bool there) {
-        float x[kPer];
-        const int32_t id0 = v * kPer - shift;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const int32_t id = id0 + j;
-            x[j] = there && id >= 0 && id < p.width ? load_global_elem<kDtype>(rowp, id) : neg_inf();
-        }
-        scan_elems<kPer, kPer, kTop>(p, &sh, st, x, there ? id0 : -kPer, 0, p.width, xt, t, rank);
-    };
-    if constexpr (kTop) {
-        float mx = neg_inf();
-#pragma unroll
-        for (int u = 0; u < kU; ++u) mx = fmaxf(mx, vec_max<kDtype>(raw[u]));  // (NaN left out)
-        seed_threshold(p, &sh, mx);
-    }
-    if (warp == 0 && rank_in == 0 && v0 > 0) edge(0, lane == 0);
+    float top = neg_inf(), slot_top = neg_inf();  // this thread's maximum, and its maximum in the current slot
+    int32_t slot = 0, in_slot = 0;
     while (v < v1) {  // warp-uniform
-        float x[16];
+        const int32_t at = v;
+        uint4 cur[kU];
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            Vec16<kDtype> e;
-            e.unpack(raw[u]);
-#pragma unroll
-            for (int q = 0; q < kPer; ++q) x[u * kPer + q] = e.x[q];
-        }
-        const int32_t id0 = (v + lane) * kPer - shift;
+        for (int u = 0; u < kU; ++u) cur[u] = raw[u];
         v += stride;
         if (v < v1) load(v);  // the next step's loads are in flight while this one is added
-        scan_elems<16, kPer, kTop>(p, &sh, st, x, id0, kLpNT * kPer, limit, xt, t, rank);
+#pragma unroll
+        for (int h = 0; h < kU / kPart; ++h) {
+            float x[16], mx = neg_inf();
+#pragma unroll
+            for (int u = 0; u < kPart; ++u) {
+                const uint4 w = cur[h * kPart + u];
+                mx = fmaxf(mx, vec_max<kDtype>(w));  // (NaN left out)
+                Vec16<kDtype> e;
+                e.unpack(w);
+#pragma unroll
+                for (int q = 0; q < kPer; ++q) x[u * kPer + q] = e.x[q];
+            }
+            st.add(x, mx);
+            if (rank) {
+                const int32_t va = at + h * kPart * kNT;
+                st.count(x, mx, (va + lane) * kPer - shift, kNT * kPer, limit, va * kPer - shift,
+                         (va + (kPart - 1) * kNT + 32) * kPer - shift);
+            }
+            slot_top = fmaxf(slot_top, mx);
+        }
+        if constexpr (kTop) {
+            if (++in_slot == per_slot || v >= v1) {
+                sh.slot_max[warp][slot][lane] = slot_top;
+                top = fmaxf(top, slot_top);
+                slot_top = neg_inf();
+                ++slot;
+                in_slot = 0;
+            }
+        }
     }
-    // (the last vector's ids are above all others: after every step of its warp)
-    if (warp == 0 && rank_in == 0 && v1 < nv && nv - 1 >= v0) edge(nv - 1, lane == 0);
+    // the elements of the vectors that the row only partly fills, at most one to a lane of the first warp: those
+    // of the first in lanes 0 .. kPer - 1, those of the last in kPer .. 2 kPer - 1
+    float ex = neg_inf();
+    int32_t eid = -1;
+    if (warp == 0 && rank_in == 0) {
+        if (lane < kPer && v0 > 0) eid = lane - shift;
+        if (lane >= kPer && lane < 2 * kPer && v1 < nv && nv - 1 >= v0) eid = (nv - 1) * kPer - shift + lane - kPer;
+        if (eid >= p.width) eid = -1;
+        if (eid >= 0) ex = load_global_elem<kDtype>(rowp, eid);
+        const float pair[2] = {ex, neg_inf()}, one[2] = {ex, quiet_nan()};
+        st.add(pair, fmaxf(ex, neg_inf()));
+        if (rank) st.count(one, ex, eid, 0, p.width, -1, p.width);
+        top = fmaxf(top, ex);
+    }
 
     // warp, block, cluster
     SoftAcc acc = soft_reduce(st.acc, 32, p.c);
-    int32_t ahead = __reduce_add_sync(0xffffffffu, st.ahead);
-    if (lane == 0) {
-        sh.acc[warp] = acc;
-        sh.ahead[warp] = ahead;
-    }
-    uint64_t key = st.key;
+    float n0, n1;
+    unpack2(st.ahead2, n0, n1);
+    int32_t ahead = __reduce_add_sync(0xffffffffu, int32_t(n0) + int32_t(n1));
+    uint64_t key = 0;
     if constexpr (kTop) {
-        // lists by halves: warp w takes in warp w + n's
-#pragma unroll
-        for (int n = kLpWarps / 2; n > 0; n >>= 1) {
-            if (warp >= n && warp < 2 * n) sh.list[warp][lane] = key;
+        const int qth = (p.n_top + kW - 1) / kW - 1;
+        const uint32_t wq = uint32_t(__shfl_sync(0xffffffffu, sort_desc(uint64_t(loom_order_key(top))), qth));
+        float X;
+        if constexpr (kW > 1) {
+            if (lane == 0) sh.wq[warp] = wq;
             __syncthreads();
-            if (warp < n) key = merge_lists(key, sh.list[warp + n][lane]);
+            X = order_key_to_float(__reduce_min_sync(0xffffffffu, lane < kW ? sh.wq[lane] : 0xffffffffu));
+        } else {
+            __syncwarp();
+            X = order_key_to_float(wq);
         }
-    } else {
-        __syncthreads();
+        // the groups of each slot, queued for 32 lanes at a time
+        int queued = 0;
+        auto flush = [&]() {
+            __syncwarp();
+            const int n = queued < 32 ? queued : 32;
+            const uint32_t g = lane < n ? sh.queue[warp][lane] : 0;
+            const uint16_t rest = sh.queue[warp][32 + lane];
+            const int32_t s = int32_t(g >> 5) * per_slot;
+            list_group<kDtype, kU, kNT>(key, p.n_top, vec, shift, v_start + s * stride + int32_t(g & 31), v1, stride,
+                                        per_slot, lane < n, X);
+            __syncwarp();
+            sh.queue[warp][lane] = rest;
+            queued -= n;
+            // a later slot's ids are above all earlier ones: only a larger value can displace the list's last
+            const uint64_t last = __shfl_sync(0xffffffffu, key, p.n_top - 1);
+            return last ? order_key_to_float(uint32_t(last >> 32) + 1) : neg_inf();
+        };
+        float own = neg_inf();
+        for (int s = 0; s < slot; ++s) {
+            const bool hit = sh.slot_max[warp][s][lane] >= fmaxf(X, own);
+            const uint32_t b = __ballot_sync(0xffffffffu, hit);
+            if (b == 0) continue;
+            if (hit) sh.queue[warp][queued + __popc(b & ((1u << lane) - 1u))] = uint16_t(s * 32 + lane);
+            queued += __popc(b);
+            if (queued >= 32) own = flush();
+        }
+        while (queued > 0) flush();
+        if (warp == 0 && rank_in == 0)
+            key = merge_lists(key, sort_desc(ex >= X && eid >= 0 ? loom_rank_key(ex, eid) : 0ull));
     }
-    if (warp == 0) {
-        acc = lane < kLpWarps ? sh.acc[lane] : soft_init();
-        acc = soft_reduce(acc, 32, p.c);
-        ahead = __reduce_add_sync(0xffffffffu, lane < kLpWarps ? sh.ahead[lane] : 0);
-    }
-    if (C > 1) {
+    if constexpr (kW > 1) {
+        if (lane == 0) {
+            sh.acc[warp] = acc;
+            sh.ahead[warp] = ahead;
+        }
+        if constexpr (kTop) {
+            // lists by halves: warp w takes in warp w + n's
+#pragma unroll
+            for (int n = kW / 2; n > 0; n >>= 1) {
+                if (warp >= n && warp < 2 * n) sh.list[warp][lane] = key;
+                __syncthreads();
+                if (warp < n) key = merge_lists(key, sh.list[warp + n][lane]);
+            }
+        } else {
+            __syncthreads();
+        }
         if (warp == 0) {
-            if (lane == 0) {
-                sh.block_acc = acc;
-                sh.block_ahead = ahead;
-            }
-            if constexpr (kTop) sh.block_list[lane] = key;
+            acc = lane < kW ? sh.acc[lane] : soft_init();
+            acc = soft_reduce(acc, 32, p.c);
+            ahead = __reduce_add_sync(0xffffffffu, lane < kW ? sh.ahead[lane] : 0);
         }
-        cluster.sync();
-        if (rank_in == 0) {
-            if constexpr (kTop) {
-                // (C is at most kLpWarps: warp b takes block b's list)
-                if (warp < C) key = cluster.map_shared_rank(&sh, warp)->block_list[lane];
-                for (int n = C / 2; n > 0; n >>= 1) {
-                    if (warp >= n && warp < 2 * n) sh.list[warp][lane] = key;
-                    __syncthreads();
-                    if (warp < n) key = merge_lists(key, sh.list[warp + n][lane]);
-                }
-            }
+        if (C > 1) {
             if (warp == 0) {
-                acc = soft_init();
-                ahead = 0;
-                if (lane < C) {
-                    const LpShared* other = cluster.map_shared_rank(&sh, lane);
-                    acc = other->block_acc;
-                    ahead = other->block_ahead;
+                if (lane == 0) {
+                    sh.block_acc = acc;
+                    sh.block_ahead = ahead;
                 }
-                acc = soft_reduce(acc, 32, p.c);
-                ahead = __reduce_add_sync(0xffffffffu, ahead);
+                if constexpr (kTop) sh.block_list[lane] = key;
             }
+            cluster.sync();
+            if (rank_in == 0) {
+                if constexpr (kTop) {
+                    // (C is at most kW: warp b takes block b's list)
+                    if (warp < C) key = cluster.map_shared_rank(&sh, warp)->block_list[lane];
+                    for (int n = C / 2; n > 0; n >>= 1) {
+                        if (warp >= n && warp < 2 * n) sh.list[warp][lane] = key;
+                        __syncthreads();
+                        if (warp < n) key = merge_lists(key, sh.list[warp + n][lane]);
+                    }
+                }
+                if (warp == 0) {
+                    acc = soft_init();
+                    ahead = 0;
+                    if (lane < C) {
+                        const LpShared<kW>* other = cluster.map_shared_rank(&sh, lane);
+                        acc = other->block_acc;
+                        ahead = other->block_ahead;
+                    }
+                    acc = soft_reduce(acc, 32, p.c);
+                    ahead = __reduce_add_sync(0xffffffffu, ahead);
+                }
+            }
+            cluster.sync();  // no block's shared memory goes away before it has been read
         }
-        cluster.sync();  // no block's shared memory goes away before it has been read
+        if (warp != 0 || rank_in != 0) return;
     }
-    if (warp != 0 || rank_in != 0) return;
 
     const float lns = logf(acc.s);  // -inf for an empty row, NaN where a logit was NaN or +inf
     const bool empty = acc.s == 0.0f;
@@ -412,19 +515,26 @@ __global__ void __launch_bounds__(kLpNT) token_logprobs_kernel(const LpDev p) {
 }
 
 // Blocks per row: as many as it takes to fill the GPU (kLpBlocksPerSm resident blocks each), at most 8 (a portable
-// cluster), and no more than there are steps of 16 elements a thread in a row.
-constexpr int kLpBlocksPerSm = 4;
+// cluster), and no more than there are steps in a row.
+#ifndef LP_BPS
+#define LP_BPS 4
+#endif
+#ifndef LP_NARROW
+#define LP_NARROW 2048
+#endif
+constexpr int kLpWarps = 8;
+constexpr int kLpBlocksPerSm = LP_BPS;
 int lp_cluster(int64_t rows, int64_t n_vocab, int sms) {
     int c = 1;
-    while (c < 8 && rows * c < int64_t(kLpBlocksPerSm) * sms && n_vocab > int64_t(c) * 16 * kLpNT) c *= 2;
+    while (c < 8 && rows * c < int64_t(kLpBlocksPerSm) * sms && n_vocab > int64_t(c) * 16 * kLpWarps * 32) c *= 2;
     return c;
 }
 
-template <int kDtype, bool kTop>
+template <int kDtype, bool kTop, int kW>
 cudaError_t launch_lp(const LpDev& p, int64_t rows, int C, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(rows * C));
-    cfg.blockDim = dim3(kLpNT);
+    cfg.blockDim = dim3(kW * 32);
     cfg.stream = s;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeClusterDimension;
@@ -432,7 +542,13 @@ cudaError_t launch_lp(const LpDev& p, int64_t rows, int C, cudaStream_t s) {
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<kDtype, kTop>, p);
+    return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<kDtype, kTop, kW>, p);
+}
+
+template <int kDtype, bool kTop>
+cudaError_t launch_lp_any(const LpDev& p, int64_t rows, int sms, cudaStream_t s) {
+    if (p.width <= LP_NARROW) return launch_lp<kDtype, kTop, 1>(p, rows, 1, s);
+    return launch_lp<kDtype, kTop, kLpWarps>(p, rows, lp_cluster(rows, p.width, sms), s);
 }
 
 // ---- the gradient ----
@@ -544,13 +660,14 @@ LOOM_SELECT_API int loom_token_logprobs(const void* logits, int dtype, int64_t r
     int st = LOOM_SELECT_OK;
     const int sms = device_sm_count(&st);
     if (st != LOOM_SELECT_OK) return st;
-    const int C = lp_cluster(rows, n_vocab, sms);
     const auto s = static_cast<cudaStream_t>(stream);
     cudaError_t e;
     if (dtype == LOOM_SELECT_BF16)
-        e = n_top ? launch_lp<LOOM_SELECT_BF16, true>(p, rows, C, s) : launch_lp<LOOM_SELECT_BF16, false>(p, rows, C, s);
+        e = n_top ? launch_lp_any<LOOM_SELECT_BF16, true>(p, rows, sms, s)
+                  : launch_lp_any<LOOM_SELECT_BF16, false>(p, rows, sms, s);
     else
-        e = n_top ? launch_lp<LOOM_SELECT_F32, true>(p, rows, C, s) : launch_lp<LOOM_SELECT_F32, false>(p, rows, C, s);
+        e = n_top ? launch_lp_any<LOOM_SELECT_F32, true>(p, rows, sms, s)
+                  : launch_lp_any<LOOM_SELECT_F32, false>(p, rows, sms, s);
     return e == cudaSuccess ? LOOM_SELECT_OK : LOOM_SELECT_ECUDA;
 }
 
