@@ -87,14 +87,18 @@ struct LpDev {
 #endif
 // A thread keeps the maxima of its elements in up to this many equal runs of steps.
 constexpr int kSlots = 32;
+constexpr int kMaxCand = 512;
 
 template <int kW>
 struct LpShared {
     SoftAcc acc[kW];
     int32_t ahead[kW];
     uint64_t list[kW][32];
-    uint32_t wq[kW];           // per warp: order key of a value that ceil(n_top / kW) of its lanes' maxima reach
-    uint16_t queue[kW][64];    // per warp: (slot, lane) groups to look through
+    uint32_t group[kW == 1 ? 32 : 8 * kW];  // order keys of the maxima of groups of threads
+    uint32_t x_key;                         // order key of the threshold
+    int32_t n_cand;
+    uint16_t queue[kW][64];    // per warp: (slot, lane) pairs to look through
+    uint64_t cand[kMaxCand];   // the elements that reach the threshold
     float slot_max[kW][kSlots][32];
     // the block's results, read by the cluster's first block
     SoftAcc block_acc;
@@ -230,44 +234,171 @@ struct LpScan {
 
 };
 
-// One lane's share of the row in one slot: `n` steps from vector `v` on, kU vectors (kNT apart) to a step, `stride`
-// vectors between steps. Appends, for every lane at once, the elements >= X to the warp's list of the best 32 keys:
-// in each round every lane offers its best element not offered yet, and the offers, sorted, are merged in.
-template <int kDtype, int kU, int kNT>
-__device__ __forceinline__ void list_group(uint64_t& key, int n_top, const unsigned char* vec, int32_t shift, int32_t v,
-                                           int32_t v1, int32_t stride, int n, bool there, float X) {
+// One block's view of its row, for looking through the slots again.
+struct LpShare {
+    const unsigned char* vec;
+    int32_t shift, v_start, v1, stride, per_slot, slots;  // v_start: the warp's first vector
+    int n_top;
+    float X;
+};
+
+// The slots whose maximum reaches X (and `own`, when the callback raises it), 32 (slot, lane) pairs at a time: each
+// lane gets a pair, and the callback the first vector of its run of steps.
+template <int kW, class F>
+__device__ __forceinline__ void for_slots(const LpShare& r, LpShared<kW>* sh, F&& look) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int queued = 0;
+    float own = neg_inf();
+    auto flush = [&]() {
+        __syncwarp();
+        const int n = queued < 32 ? queued : 32;
+        const uint32_t g = lane < n ? sh->queue[warp][lane] : 0;
+        const uint16_t rest = sh->queue[warp][32 + lane];
+        own = look(r.v_start + int32_t(g >> 5) * r.per_slot * r.stride + int32_t(g & 31), lane < n);
+        __syncwarp();
+        sh->queue[warp][lane] = rest;
+        queued -= n;
+    };
+    for (int s = 0; s < r.slots; ++s) {
+        const bool hit = sh->slot_max[warp][s][lane] >= fmaxf(r.X, own);
+        const uint32_t b = __ballot_sync(0xffffffffu, hit);
+        if (b == 0) continue;
+        if (hit) sh->queue[warp][queued + __popc(b & ((1u << lane) - 1u))] = uint16_t(s * 32 + lane);
+        queued += __popc(b);
+        if (queued >= 32) flush();
+    }
+    while (queued > 0) flush();
+}
+
+template <int kDtype>
+__device__ __forceinline__ uint4 load_or_nan(const unsigned char* vec, int32_t v, bool there) {
+    const uint32_t w = kDtype == LOOM_SELECT_BF16 ? 0xffffffffu : 0x7fffffffu;
+    return there ? ldg_stream_v4(vec + int64_t(v) * 16) : make_uint4(w, w, w, w);
+}
+
+// The warp's best 32 of its elements >= X, sorted, when too many of them reach X to be held (a row of few
+// values, or of almost nothing but -inf). In each round every lane offers its best element not offered yet, and
+// the offers, sorted, are merged into the list.
+template <int kDtype, int kU, int kW>
+__device__ __noinline__ uint64_t list_slots(const LpShare& r, LpShared<kW>* sh) {
     constexpr int kPer = kDtype == LOOM_SELECT_BF16 ? 8 : 4;
-    for (int i = 0; i < n; ++i) {
-        uint4 raw[kU];
-        const int32_t at = v + i * stride;
+    constexpr int kNT = kW * 32;
+    uint64_t key = 0;
+    for_slots<kW>(r, sh, [&](int32_t v, bool there) {
+        for (int i = 0; i < r.per_slot; ++i, v += r.stride) {
+            uint64_t below = ~0ull;  // keys from here on have been offered
+            for (;;) {
+                uint64_t best = 0;
+#pragma unroll 1
+                for (int u = 0; u < kU; ++u) {
+                    Vec16<kDtype> e;
+                    e.unpack(load_or_nan<kDtype>(r.vec, v + u * kNT, there && v + u * kNT < r.v1));
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            const uint32_t w = kDtype == LOOM_SELECT_BF16 ? 0xffffffffu : 0x7fffffffu;  // NaN: never an alternative
-            raw[u] = make_uint4(w, w, w, w);
-            if (there && at + u * kNT < v1) raw[u] = ldg_stream_v4(vec + int64_t(at + u * kNT) * 16);
+                    for (int q = 0; q < kPer; ++q) {
+                        if (e.x[q] >= r.X) {
+                            const uint64_t k = loom_rank_key(e.x[q], (v + u * kNT) * kPer - r.shift + q);
+                            best = k < below && k > best ? k : best;
+                        }
+                    }
+                }
+                const uint64_t last = __shfl_sync(0xffffffffu, key, r.n_top - 1);
+                if (best <= last) best = 0;
+                if (!__any_sync(0xffffffffu, best != 0)) break;
+                if (best) below = best;
+                key = merge_lists(key, sort_desc(best));
+            }
         }
-        uint64_t below = ~0ull;  // keys from here on have been offered
-        for (;;) {
-            uint64_t best = 0;
+        // a later slot's ids are above all earlier ones: only a larger value can displace the list's last
+        const uint64_t last = __shfl_sync(0xffffffffu, key, r.n_top - 1);
+        return last ? order_key_to_float(uint32_t(last >> 32) + 1) : neg_inf();
+    });
+    return key;
+}
+
+template <int kW>
+__device__ __forceinline__ void block_sync() {
+    if constexpr (kW == 1) __syncwarp();
+    else __syncthreads();
+}
+
+// The block's best n_top elements, sorted, in the first warp's lanes. `top` is the thread's largest element; (ex, eid)
+// an element outside the whole vectors, in the first warp's lanes (eid < 0: none).
+template <int kDtype, int kU, int kW>
+__device__ __forceinline__ uint64_t block_best(LpShare r, LpShared<kW>* sh, float top, float ex, int32_t eid) {
+    constexpr int kPer = kDtype == LOOM_SELECT_BF16 ? 8 : 4;
+    constexpr int kNT = kW * 32;
+    constexpr int kGroups = kW == 1 ? 32 : 8 * kW;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // the threshold: the n_top-th largest of the groups' maxima
+    if constexpr (kW > 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if ((lane & 3) == 0) sh->group[tid >> 2] = loom_order_key(top);
+    } else {
+        sh->group[lane] = loom_order_key(top);
+    }
+    if (tid == 0) sh->n_cand = 0;
+    if (warp == 0) sh->list[0][lane] = 0;
+    block_sync<kW>();
+    if (tid < kGroups) {
+        const uint32_t mine = sh->group[tid];
+        int ahead = 0;
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) {
+            const uint32_t o = sh->group[j];
+            ahead += o > mine || (o == mine && j < tid);
+        }
+        if (ahead == r.n_top - 1) sh->x_key = mine;
+    }
+    block_sync<kW>();
+    r.X = order_key_to_float(sh->x_key);
+    auto add = [&](float x, int32_t id) {
+        const int at = atomicAdd(&sh->n_cand, 1);
+        if (at < kMaxCand) sh->cand[at] = loom_rank_key(x, id);
+    };
+    for_slots<kW>(r, sh, [&](int32_t v, bool there) {
+        for (int i = 0; i < r.per_slot; ++i, v += r.stride) {
+            uint4 raw[kU];
+#pragma unroll
+            for (int u = 0; u < kU; ++u) raw[u] = load_or_nan<kDtype>(r.vec, v + u * kNT, there && v + u * kNT < r.v1);
 #pragma unroll
             for (int u = 0; u < kU; ++u) {
+                if (!(vec_max<kDtype>(raw[u]) >= r.X)) continue;
                 Vec16<kDtype> e;
                 e.unpack(raw[u]);
 #pragma unroll
-                for (int q = 0; q < kPer; ++q) {
-                    if (e.x[q] >= X) {
-                        const uint64_t k = loom_rank_key(e.x[q], (at + u * kNT) * kPer - shift + q);
-                        best = k < below && k > best ? k : best;
-                    }
-                }
+                for (int q = 0; q < kPer; ++q)
+                    if (e.x[q] >= r.X) add(e.x[q], (v + u * kNT) * kPer - r.shift + q);
             }
-            const uint64_t last = __shfl_sync(0xffffffffu, key, n_top - 1);
-            if (best <= last) best = 0;
-            if (!__any_sync(0xffffffffu, best != 0)) break;
-            if (best) below = best;
-            key = merge_lists(key, sort_desc(best));
+        }
+        return neg_inf();
+    });
+    if (eid >= 0 && ex >= r.X) add(ex, eid);
+    block_sync<kW>();
+    const int n = sh->n_cand;
+    uint64_t key = 0;
+    if (n <= kMaxCand) {
+        // each one's place is the number of larger ones
+        for (int i = tid; i < n; i += kNT) {
+            const uint64_t mine = sh->cand[i];
+            int ahead = 0;
+            for (int j = 0; j < n; ++j) ahead += sh->cand[j] > mine;
+            if (ahead < r.n_top) sh->list[0][ahead] = mine;
+        }
+        block_sync<kW>();
+        if (warp == 0) key = sh->list[0][lane];
+    } else {
+        key = list_slots<kDtype, kU, kW>(r, sh);
+        if (warp == 0) key = merge_lists(key, sort_desc(eid >= 0 && ex >= r.X ? loom_rank_key(ex, eid) : 0ull));
+        // by halves: warp w takes in warp w + n's list
+#pragma unroll
+        for (int h = kW / 2; h > 0; h >>= 1) {
+            if (warp >= h && warp < 2 * h) sh->list[warp][lane] = key;
+            __syncthreads();
+            if (warp < h) key = merge_lists(key, sh->list[warp + h][lane]);
         }
     }
+    return key;
 }
 
 // A cluster of C blocks of kW warps per row: block b takes every C-th step of kU vectors per thread. Each block
@@ -275,9 +406,9 @@ __device__ __forceinline__ void list_group(uint64_t& key, int n_top, const unsig
 // No workspace, tickets or waits between clusters.
 //
 // Alternatives: while streaming, a thread only notes the largest element of each slot (a run of steps). At the end
-// the ceil(n_top / kW)-th largest of each warp's 32 thread maxima, the smallest of the warps' values, is a threshold X
-// that at least n_top elements of the block reach, and few more do (n_top of 256 threads). The slots whose maximum
-// reaches X are read again, from L2, and their elements >= X sorted into the warps' lists.
+// the n_top-th largest of 64 maxima (of groups of four threads) is a threshold that at least n_top elements of the
+// block reach, and few more do (64 -ln(1 - n / 64): 24 for 20). The slots whose maximum reaches it are read
+// again, from L2, and those elements sorted by counting.
 template <int kDtype, bool kTop, int kW>
 __global__ void __launch_bounds__(kW * 32, kW == 1 ? LP_MINB1 : LP_MINB) token_logprobs_kernel(const LpDev p) {
     constexpr int kEsz = kDtype == LOOM_SELECT_BF16 ? 2 : 4;
@@ -392,63 +523,15 @@ __global__ void __launch_bounds__(kW * 32, kW == 1 ? LP_MINB1 : LP_MINB) token_l
     int32_t ahead = __reduce_add_sync(0xffffffffu, int32_t(n0) + int32_t(n1));
     uint64_t key = 0;
     if constexpr (kTop) {
-        const int qth = (p.n_top + kW - 1) / kW - 1;
-        const uint32_t wq = uint32_t(__shfl_sync(0xffffffffu, sort_desc(uint64_t(loom_order_key(top))), qth));
-        float X;
-        if constexpr (kW > 1) {
-            if (lane == 0) sh.wq[warp] = wq;
-            __syncthreads();
-            X = order_key_to_float(__reduce_min_sync(0xffffffffu, lane < kW ? sh.wq[lane] : 0xffffffffu));
-        } else {
-            __syncwarp();
-            X = order_key_to_float(wq);
-        }
-        // the groups of each slot, queued for 32 lanes at a time
-        int queued = 0;
-        auto flush = [&]() {
-            __syncwarp();
-            const int n = queued < 32 ? queued : 32;
-            const uint32_t g = lane < n ? sh.queue[warp][lane] : 0;
-            const uint16_t rest = sh.queue[warp][32 + lane];
-            const int32_t s = int32_t(g >> 5) * per_slot;
-            list_group<kDtype, kU, kNT>(key, p.n_top, vec, shift, v_start + s * stride + int32_t(g & 31), v1, stride,
-                                        per_slot, lane < n, X);
-            __syncwarp();
-            sh.queue[warp][lane] = rest;
-            queued -= n;
-            // a later slot's ids are above all earlier ones: only a larger value can displace the list's last
-            const uint64_t last = __shfl_sync(0xffffffffu, key, p.n_top - 1);
-            return last ? order_key_to_float(uint32_t(last >> 32) + 1) : neg_inf();
-        };
-        float own = neg_inf();
-        for (int s = 0; s < slot; ++s) {
-            const bool hit = sh.slot_max[warp][s][lane] >= fmaxf(X, own);
-            const uint32_t b = __ballot_sync(0xffffffffu, hit);
-            if (b == 0) continue;
-            if (hit) sh.queue[warp][queued + __popc(b & ((1u << lane) - 1u))] = uint16_t(s * 32 + lane);
-            queued += __popc(b);
-            if (queued >= 32) own = flush();
-        }
-        while (queued > 0) flush();
-        if (warp == 0 && rank_in == 0)
-            key = merge_lists(key, sort_desc(ex >= X && eid >= 0 ? loom_rank_key(ex, eid) : 0ull));
+        const LpShare r{vec, shift, v_start, v1, stride, per_slot, slot, p.n_top, 0.0f};
+        key = block_best<kDtype, kU, kW>(r, &sh, top, ex, eid);
     }
     if constexpr (kW > 1) {
         if (lane == 0) {
             sh.acc[warp] = acc;
             sh.ahead[warp] = ahead;
         }
-        if constexpr (kTop) {
-            // lists by halves: warp w takes in warp w + n's
-#pragma unroll
-            for (int n = kW / 2; n > 0; n >>= 1) {
-                if (warp >= n && warp < 2 * n) sh.list[warp][lane] = key;
-                __syncthreads();
-                if (warp < n) key = merge_lists(key, sh.list[warp + n][lane]);
-            }
-        } else {
-            __syncthreads();
-        }
+        __syncthreads();
         if (warp == 0) {
             acc = lane < kW ? sh.acc[lane] : soft_init();
             acc = soft_reduce(acc, 32, p.c);
