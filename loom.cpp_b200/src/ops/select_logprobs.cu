@@ -88,22 +88,27 @@ struct LpDev {
 // A thread keeps the maxima of its elements in up to this many equal runs of steps.
 constexpr int kSlots = 32;
 constexpr int kMaxCand = 512;
+constexpr int kMaxCluster = 8;
+constexpr int kGroups = 64;  // (32 in a block of one warp)
 
 template <int kW>
 struct LpShared {
     SoftAcc acc[kW];
     int32_t ahead[kW];
     uint64_t list[kW][32];
-    uint32_t group[kW == 1 ? 32 : 8 * kW];  // order keys of the maxima of groups of threads
-    uint32_t x_key;                         // order key of the threshold
-    int32_t n_cand;
+    uint32_t group[kGroups];   // order keys of the maxima of the cluster's groups of threads
+    uint32_t x_key;            // order key of the threshold
+    int32_t n_cand;            // elements of this block that reach it
+    int32_t overflow;          // some block of the cluster has more of them than it may hand on
     uint16_t queue[kW][64];    // per warp: (slot, lane) pairs to look through
-    uint64_t cand[kMaxCand];   // the elements that reach the threshold
     float slot_max[kW][kSlots][32];
-    // the block's results, read by the cluster's first block
-    SoftAcc block_acc;
-    int32_t block_ahead;
-    uint64_t block_list[32];
+    // of the cluster's first block: what the blocks hand on
+    SoftAcc part[kMaxCluster];
+    int32_t part_ahead[kMaxCluster];
+    int32_t part_cand[kMaxCluster];
+    uint64_t cand[kMaxCand];   // kMaxCand / C from each block
+    uint64_t sorting[kMaxCand + 8];
+    uint64_t part_list[kMaxCluster][32];
 };
 
 // Descending bitonic sort of one key per lane.
@@ -156,82 +161,177 @@ __device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
 }
 
-// 1 where a > b, else 0 (NaN: 0).
-__device__ __forceinline__ float gt_one(float a, float b) {
+// 1 where a > b (kGe: a >= b), else 0 (NaN: 0).
+template <bool kGe>
+__device__ __forceinline__ float ahead_one(float a, float b) {
     float y;
-    asm("set.gt.f32.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    if constexpr (kGe) asm("set.ge.f32.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    else asm("set.gt.f32.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
 
-// The largest float below x (x finite or +inf; one below either zero).
-__device__ __forceinline__ float float_below(float x) {
-    return order_key_to_float(loom_order_key(x) - (x == 0.0f ? 2u : 1u));
+// One 16-byte vector as pairs of floats.
+template <int kDtype>
+struct Pairs {
+    static constexpr int kPairs = kDtype == LOOM_SELECT_BF16 ? 4 : 2;
+    uint64_t v[kPairs];
+    __device__ __forceinline__ explicit Pairs(uint4 raw) {
+        if constexpr (kDtype == LOOM_SELECT_BF16) {
+            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = pack2(__uint_as_float(w[q] << 16), __uint_as_float(w[q] & 0xffff0000u));
+        } else {
+            v[0] = pack2(__uint_as_float(raw.x), __uint_as_float(raw.y));
+            v[1] = pack2(__uint_as_float(raw.z), __uint_as_float(raw.w));
+        }
+    }
+};
+
+__device__ __forceinline__ void add2(uint64_t& a, uint64_t b) { asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a) : "l"(b)); }
+__device__ __forceinline__ void fma2(uint64_t& d, uint64_t a, uint64_t b) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b));
 }
 
-// One thread's running softmax sums and rank count over its elements of a row. Elements come NE at a time: x[j]
-// has id id0 + (j / kPer) * step + j % kPer; those whose id is not in [0, limit) hold -inf and are not counted.
-template <int kPer>
+// One thread's running softmax sums and rank count over its elements of a row, which come as kU vectors of kPer
+// elements each: element q of vector u has id id0 + u * step + q; those whose id is not in [0, limit) hold -inf and
+// are not counted.
+template <int kDtype, int kU>
 struct LpScan {
+    static constexpr int kPer = kDtype == LOOM_SELECT_BF16 ? 8 : 4;
     SoftAcc acc;
-    float c;
-    // the rank: ids before t count when x > xt_below, i.e. x >= xt, ids after it when x > xt
-    float xt, xt_below;
-    int32_t t;
-    uint64_t ahead2;  // two f32 counts (exact: a thread has far fewer than 2^24 elements)
+    float c;         // log2(e) / T
+    float mc, r, g;  // rn(m c), what its rounding lost, 2^-r
+    bool slow;
+    int32_t ahead;
 
-    // Softmax terms, two elements per instruction (f32x2). They are summed apart first: a thread's chain is
-    // one addition per call, not one per element.
-    template <int NE>
-    __device__ __forceinline__ void add(const float (&x)[NE], float mx) {
-        if (mx > acc.m) acc = soft_move(acc, mx, c);
-        const uint64_t mm = pack2(acc.m, acc.m), cc = pack2(c, c);
-        uint64_t s2 = 0, a2 = 0;
-#pragma unroll
-        for (int j = 0; j < NE; j += 2) {
-            uint64_t d = pack2(x[j], x[j + 1]);
-            asm("sub.rn.f32x2 %0, %0, %1;" : "+l"(d) : "l"(mm));
-            asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(d) : "l"(cc));
-            float d0, d1;
-            unpack2(d, d0, d1);
-            d0 = max_nan(d0, kMinExp2);
-            d1 = max_nan(d1, kMinExp2);
-            d = pack2(d0, d1);
-            const uint64_t e = pack2(ex2(d0), ex2(d1));
-            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s2) : "l"(e));
-            asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a2) : "l"(e), "l"(d));
-        }
-        float s0, s1, a0, a1;
-        unpack2(s2, s0, s1);
-        unpack2(a2, a0, a1);
-        acc.s += s0 + s1;
-        acc.a += a0 + a1;
+    __device__ __forceinline__ void start(float c_) {
+        acc = soft_init();
+        c = c_;
+        mc = -neg_inf();  // (until there is a maximum, the common path gives NaN)
+        r = 0.0f;
+        g = 1.0f;
+        slow = false;
+        ahead = 0;
     }
 
-    // Ids ahead of t. lo and hi bound the warp's ids of this call (as warp-uniform values).
-    template <int NE>
-    __device__ __forceinline__ void count(const float (&x)[NE], float mx, int32_t id0, int32_t step, int32_t limit,
-                                          int32_t lo, int32_t hi) {
-        if (!__any_sync(0xffffffffu, mx >= xt)) return;
-        const bool before = hi <= t;
-        if ((before || lo > t) && xt > neg_inf()) {
-            const float g = before ? xt_below : xt;
+    // Two elements per instruction (f32x2). The common path takes 2^(x c - rn(m c)), one fused operation, one ex2 and
+    // two additions an element, and moves the vectors' sums to the exact reference m c afterwards. A -inf (its
+    // product with the exponent is NaN), a NaN, or a maximum so large that rounding m c loses much send the thread
+    // to the other path from then on: (x - m) c, clamped. `partial`: some elements are not there.
+    __device__ __forceinline__ void add(const uint4 (&raw)[kU], float mx, bool partial) {
+        if (mx > acc.m) {
+            acc = soft_move(acc, mx, c);
+            mc = __fmul_rn(mx, c);
+            r = __fmaf_rn(mx, c, -mc);
+            g = exp2f(-r);
+            slow = slow || !(fabsf(mc) <= 65536.0f);
+        }
+        float s, a;
+        bool clamped = slow || partial;
+        if (!clamped) {
+            const uint64_t cc = pack2(c, c), mm = pack2(-mc, -mc);
+            uint64_t s2 = 0, a2 = 0;
 #pragma unroll
-            for (int j = 0; j < NE; j += 2) {
-                const uint64_t n = pack2(gt_one(x[j], g), gt_one(x[j + 1], g));
-                asm("add.rn.f32x2 %0, %0, %1;" : "+l"(ahead2) : "l"(n));
+            for (int u = 0; u < kU; ++u) {
+                const Pairs<kDtype> x(raw[u]);
+#pragma unroll
+                for (int q = 0; q < Pairs<kDtype>::kPairs; ++q) {
+                    uint64_t d = mm;
+                    fma2(d, x.v[q], cc);
+                    float d0, d1;
+                    unpack2(d, d0, d1);
+                    const uint64_t e = pack2(ex2(d0), ex2(d1));
+                    add2(s2, e);
+                    fma2(a2, e, d);
+                }
             }
+            float s0, s1, a0, a1;
+            unpack2(s2, s0, s1);
+            unpack2(a2, a0, a1);
+            s = s0 + s1;
+            a = __fmaf_rn(-r, s, a0 + a1) * g;
+            s *= g;
+            clamped = slow = a != a;
+        }
+        if (clamped) {
+            s = a = 0.0f;
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const Pairs<kDtype> x(raw[u]);
+#pragma unroll
+                for (int q = 0; q < Pairs<kDtype>::kPairs; ++q) {
+                    float x0, x1;
+                    unpack2(x.v[q], x0, x1);
+                    add_one(x0, s, a);
+                    add_one(x1, s, a);
+                }
+            }
+        }
+        acc.s += s;
+        acc.a += a;
+    }
+
+    __device__ __forceinline__ void add_one(float x, float& s, float& a) const {
+        const float d = max_nan(__fmul_rn(__fsub_rn(x, acc.m), c), kMinExp2);
+        const float e = ex2(d);
+        s += e;
+        a = __fmaf_rn(e, d, a);
+    }
+
+    // Elements above xt, or (kGe) not below it.
+    template <bool kGe>
+    __device__ __forceinline__ void count_all(const uint4 (&raw)[kU], float xt) {
+        if constexpr (kDtype == LOOM_SELECT_BF16) {
+            // packed: at most kU * 4 to a half, exact in bf16
+            const __nv_bfloat162 t2 = __float2bfloat162_rn(xt);
+            __nv_bfloat162 n = __float2bfloat162_rn(0.0f);
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&w[q]);
+                    n = __hadd2(n, kGe ? __hge2(x, t2) : __hgt2(x, t2));
+                }
+            }
+            ahead += int32_t(__low2float(n) + __high2float(n));
         } else {
-            float n = 0.0f;
+            uint64_t n2 = 0;
 #pragma unroll
-            for (int j = 0; j < NE; ++j) {
-                const int32_t id = id0 + (j / kPer) * step + j % kPer;
-                n += x[j] > xt || (x[j] == xt && id < t && id >= 0 && id < limit) ? 1.0f : 0.0f;
+            for (int u = 0; u < kU; ++u) {
+                const float x[4] = {__uint_as_float(raw[u].x), __uint_as_float(raw[u].y), __uint_as_float(raw[u].z),
+                                    __uint_as_float(raw[u].w)};
+                add2(n2, pack2(ahead_one<kGe>(x[0], xt), ahead_one<kGe>(x[1], xt)));
+                add2(n2, pack2(ahead_one<kGe>(x[2], xt), ahead_one<kGe>(x[3], xt)));
             }
-            const uint64_t n2 = pack2(n, 0.0f);
-            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(ahead2) : "l"(n2));
+            float n0, n1;
+            unpack2(n2, n0, n1);
+            ahead += int32_t(n0 + n1);
         }
     }
 
+    // Ids ahead of t, whose logit is xt: x > xt, or x == xt and a lower id. The warp's ids of this call are in
+    // [lo, hi): all before t or all after it, usually.
+    __device__ __forceinline__ void count(const uint4 (&raw)[kU], float mx, int32_t id0, int32_t step, int32_t limit,
+                                          int32_t lo, int32_t hi, float xt, int32_t t) {
+        if (!__any_sync(0xffffffffu, mx >= xt)) return;
+        if (lo > t) {
+            count_all<false>(raw, xt);
+        } else if (hi <= t && xt > neg_inf()) {  // (the -inf of elements that are not there must not count)
+            count_all<true>(raw, xt);
+        } else {
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                Vec16<kDtype> e;
+                e.unpack(raw[u]);
+#pragma unroll
+                for (int q = 0; q < kPer; ++q) {
+                    const int32_t id = id0 + u * step + q;
+                    ahead += e.x[q] > xt || (e.x[q] == xt && id < t && id >= 0 && id < limit);
+                }
+            }
+        }
+    }
 };
 
 // One block's view of its row, for looking through the slots again.
@@ -321,106 +421,26 @@ __device__ __forceinline__ void block_sync() {
     else __syncthreads();
 }
 
-// The block's best n_top elements, sorted, in the first warp's lanes. `top` is the thread's largest element; (ex, eid)
-// an element outside the whole vectors, in the first warp's lanes (eid < 0: none).
-template <int kDtype, int kU, int kW>
-__device__ __forceinline__ uint64_t block_best(LpShare r, LpShared<kW>* sh, float top, float ex, int32_t eid) {
-    constexpr int kPer = kDtype == LOOM_SELECT_BF16 ? 8 : 4;
-    constexpr int kNT = kW * 32;
-    constexpr int kGroups = kW == 1 ? 32 : 8 * kW;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // the threshold: the n_top-th largest of the groups' maxima
-    if constexpr (kW > 1) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        if ((lane & 3) == 0) sh->group[tid >> 2] = loom_order_key(top);
-    } else {
-        sh->group[lane] = loom_order_key(top);
-    }
-    if (tid == 0) sh->n_cand = 0;
-    if (warp == 0) sh->list[0][lane] = 0;
-    block_sync<kW>();
-    if (tid < kGroups) {
-        const uint32_t mine = sh->group[tid];
-        int ahead = 0;
-#pragma unroll
-        for (int j = 0; j < kGroups; ++j) {
-            const uint32_t o = sh->group[j];
-            ahead += o > mine || (o == mine && j < tid);
-        }
-        if (ahead == r.n_top - 1) sh->x_key = mine;
-    }
-    block_sync<kW>();
-    r.X = order_key_to_float(sh->x_key);
-    auto add = [&](float x, int32_t id) {
-        const int at = atomicAdd(&sh->n_cand, 1);
-        if (at < kMaxCand) sh->cand[at] = loom_rank_key(x, id);
-    };
-    for_slots<kW>(r, sh, [&](int32_t v, bool there) {
-        for (int i = 0; i < r.per_slot; ++i, v += r.stride) {
-            uint4 raw[kU];
-#pragma unroll
-            for (int u = 0; u < kU; ++u) raw[u] = load_or_nan<kDtype>(r.vec, v + u * kNT, there && v + u * kNT < r.v1);
-#pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                if (!(vec_max<kDtype>(raw[u]) >= r.X)) continue;
-                Vec16<kDtype> e;
-                e.unpack(raw[u]);
-#pragma unroll
-                for (int q = 0; q < kPer; ++q)
-                    if (e.x[q] >= r.X) add(e.x[q], (v + u * kNT) * kPer - r.shift + q);
-            }
-        }
-        return neg_inf();
-    });
-    if (eid >= 0 && ex >= r.X) add(ex, eid);
-    block_sync<kW>();
-    const int n = sh->n_cand;
-    uint64_t key = 0;
-    if (n <= kMaxCand) {
-        // each one's place is the number of larger ones
-        for (int i = tid; i < n; i += kNT) {
-            const uint64_t mine = sh->cand[i];
-            int ahead = 0;
-            for (int j = 0; j < n; ++j) ahead += sh->cand[j] > mine;
-            if (ahead < r.n_top) sh->list[0][ahead] = mine;
-        }
-        block_sync<kW>();
-        if (warp == 0) key = sh->list[0][lane];
-    } else {
-        key = list_slots<kDtype, kU, kW>(r, sh);
-        if (warp == 0) key = merge_lists(key, sort_desc(eid >= 0 && ex >= r.X ? loom_rank_key(ex, eid) : 0ull));
-        // by halves: warp w takes in warp w + n's list
-#pragma unroll
-        for (int h = kW / 2; h > 0; h >>= 1) {
-            if (warp >= h && warp < 2 * h) sh->list[warp][lane] = key;
-            __syncthreads();
-            if (warp < h) key = merge_lists(key, sh->list[warp + h][lane]);
-        }
-    }
-    return key;
-}
-
-// A cluster of C blocks of kW warps per row: block b takes every C-th step of kU vectors per thread. Each block
-// reduces its share; the cluster's first block reads the others' results from their shared memory.
-// No workspace, tickets or waits between clusters.
+// A cluster of C blocks of kW warps per row: block b takes every C-th step of kU vectors per thread, and hands its
+// share's results to the cluster's first block through distributed shared memory. No workspace, tickets or waits
+// between clusters.
 //
 // Alternatives: while streaming, a thread only notes the largest element of each slot (a run of steps). At the end
-// the n_top-th largest of 64 maxima (of groups of four threads) is a threshold that at least n_top elements of the
-// block reach, and few more do (64 -ln(1 - n / 64): 24 for 20). The slots whose maximum reaches it are read
-// again, from L2, and those elements sorted by counting.
+// the n_top-th largest of 64 maxima, of equal groups of the cluster's threads, is a threshold that at least n_top
+// elements of the row reach, and few more do (64 -ln(1 - n / 64): 24 for 20). The slots whose maximum reaches it are
+// read again, from L2, and those elements sorted by counting the larger ones.
 template <int kDtype, bool kTop, int kW>
 __global__ void __launch_bounds__(kW * 32, kW == 1 ? LP_MINB1 : LP_MINB) token_logprobs_kernel(const LpDev p) {
     constexpr int kEsz = kDtype == LOOM_SELECT_BF16 ? 2 : 4;
     constexpr int kPer = 16 / kEsz;
     constexpr int kU = 4;                // vectors per thread and step
-    constexpr int kPart = 16 / kPer;     // vectors added at a time: 16 elements
     constexpr int kNT = kW * 32;
     __shared__ LpShared<kW> sh;
     const cg::cluster_group cluster = cg::this_cluster();
-    const int C = int(cluster.num_blocks()), rank_in = int(cluster.block_rank());
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int C = kW == 1 ? 1 : int(cluster.num_blocks()), rank_in = kW == 1 ? 0 : int(cluster.block_rank());
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t row = blockIdx.x / unsigned(C);
+    const int32_t t = p.ids ? p.ids[row] : -1;
     const unsigned char* rowp = p.base + row * p.row_stride * kEsz;
     // the row as 16-byte aligned vectors: vector v holds ids [v kPer - shift, (v + 1) kPer - shift)
     const int32_t shift = int32_t((reinterpret_cast<uintptr_t>(rowp) & 15) / kEsz);
@@ -449,18 +469,24 @@ __global__ void __launch_bounds__(kW * 32, kW == 1 ? LP_MINB1 : LP_MINB) token_l
     const int32_t v_start = v0 + rank_in * kU * kNT + warp * 32;
     int32_t v = v_start;
     load(v);
+    // the elements of the vectors that the row only partly fills, at most one to a lane of the first warp: those
+    // of the first in lanes 0 .. kPer - 1, those of the last in kPer .. 2 kPer - 1
+    float ex = neg_inf();
+    int32_t eid = -1;
+    if (warp == 0 && rank_in == 0) {
+        if (lane < kPer && v0 > 0) eid = lane - shift;
+        if (lane >= kPer && lane < 2 * kPer && v1 < nv && nv - 1 >= v0) eid = (nv - 1) * kPer - shift + lane - kPer;
+        if (eid >= p.width) eid = -1;
+        if (eid >= 0) ex = load_global_elem<kDtype>(rowp, eid);
+    }
+    if (tid == 0) sh.n_cand = sh.overflow = 0;
+    if (C > 1) cluster.barrier_arrive();  // (waited for before the first remote store: all blocks have begun)
 
-    LpScan<kPer> st;
-    st.acc = soft_init();
-    st.c = p.c;
-    st.ahead2 = 0;
-    const int32_t t = p.ids ? p.ids[row] : -1;
+    LpScan<kDtype, kU> st;
+    st.start(p.c);
     const bool has = t >= 0 && t < p.width;
-    st.t = t;
-    st.xt = has ? load_global_elem<kDtype>(rowp, t) : quiet_nan();
-    st.xt_below = float_below(st.xt);
+    const float xt = has ? load_global_elem<kDtype>(rowp, t) : quiet_nan();
     const bool rank = p.out_rank != nullptr && has;
-    const float xt = st.xt;
 
     float top = neg_inf(), slot_top = neg_inf();  // this thread's maximum, and its maximum in the current slot
     int32_t slot = 0, in_slot = 0;
@@ -471,26 +497,14 @@ __global__ void __launch_bounds__(kW * 32, kW == 1 ? LP_MINB1 : LP_MINB) token_l
         for (int u = 0; u < kU; ++u) cur[u] = raw[u];
         v += stride;
         if (v < v1) load(v);  // the next step's loads are in flight while this one is added
+        float mx = neg_inf();
 #pragma unroll
-        for (int h = 0; h < kU / kPart; ++h) {
-            float x[16], mx = neg_inf();
-#pragma unroll
-            for (int u = 0; u < kPart; ++u) {
-                const uint4 w = cur[h * kPart + u];
-                mx = fmaxf(mx, vec_max<kDtype>(w));  // (NaN left out)
-                Vec16<kDtype> e;
-                e.unpack(w);
-#pragma unroll
-                for (int q = 0; q < kPer; ++q) x[u * kPer + q] = e.x[q];
-            }
-            st.add(x, mx);
-            if (rank) {
-                const int32_t va = at + h * kPart * kNT;
-                st.count(x, mx, (va + lane) * kPer - shift, kNT * kPer, limit, va * kPer - shift,
-                         (va + (kPart - 1) * kNT + 32) * kPer - shift);
-            }
-            slot_top = fmaxf(slot_top, mx);
-        }
+        for (int u = 0; u < kU; ++u) mx = fmaxf(mx, vec_max<kDtype>(cur[u]));  // (NaN left out)
+        st.add(cur, mx, at + (kU - 1) * kNT + 32 > v1);
+        if (rank)
+            st.count(cur, mx, (at + lane) * kPer - shift, kNT * kPer, limit, at * kPer - shift,
+                     (at + (kU - 1) * kNT + 32) * kPer - shift, xt, t);
+        slot_top = fmaxf(slot_top, mx);
         if constexpr (kTop) {
             if (++in_slot == per_slot || v >= v1) {
                 sh.slot_max[warp][slot][lane] = slot_top;
@@ -501,31 +515,76 @@ __global__ void __launch_bounds__(kW * 32, kW == 1 ? LP_MINB1 : LP_MINB) token_l
             }
         }
     }
-    // the elements of the vectors that the row only partly fills, at most one to a lane of the first warp: those
-    // of the first in lanes 0 .. kPer - 1, those of the last in kPer .. 2 kPer - 1
-    float ex = neg_inf();
-    int32_t eid = -1;
     if (warp == 0 && rank_in == 0) {
-        if (lane < kPer && v0 > 0) eid = lane - shift;
-        if (lane >= kPer && lane < 2 * kPer && v1 < nv && nv - 1 >= v0) eid = (nv - 1) * kPer - shift + lane - kPer;
-        if (eid >= p.width) eid = -1;
-        if (eid >= 0) ex = load_global_elem<kDtype>(rowp, eid);
-        const float pair[2] = {ex, neg_inf()}, one[2] = {ex, quiet_nan()};
-        st.add(pair, fmaxf(ex, neg_inf()));
-        if (rank) st.count(one, ex, eid, 0, p.width, -1, p.width);
+        if (ex > st.acc.m) st.acc = soft_move(st.acc, ex, p.c);
+        st.add_one(ex, st.acc.s, st.acc.a);
+        st.ahead += rank && eid >= 0 && (ex > xt || (ex == xt && eid < t));
         top = fmaxf(top, ex);
     }
+    LpShared<kW>* first = C > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
 
-    // warp, block, cluster
-    SoftAcc acc = soft_reduce(st.acc, 32, p.c);
-    float n0, n1;
-    unpack2(st.ahead2, n0, n1);
-    int32_t ahead = __reduce_add_sync(0xffffffffu, int32_t(n0) + int32_t(n1));
-    uint64_t key = 0;
+    LpShare r{vec, shift, v_start, v1, stride, per_slot, slot, p.n_top, 0.0f};
     if constexpr (kTop) {
-        const LpShare r{vec, shift, v_start, v1, stride, per_slot, slot, p.n_top, 0.0f};
-        key = block_best<kDtype, kU, kW>(r, &sh, top, ex, eid);
+        // the threshold: the n_top-th largest of the groups' maxima
+        constexpr int kG = kW == 1 ? 32 : kGroups;
+        const int threads = C * kNT / kG;  // of one group: 1 to 32 neighbours
+        for (int o = 1; o < threads; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (C > 1) cluster.barrier_wait();
+        if ((lane & (threads - 1)) == 0) {
+            const uint32_t k = loom_order_key(top);
+            const int at = (rank_in * kNT + tid) / threads;
+            if (C > 1)
+                for (int b = 0; b < C; ++b) cluster.map_shared_rank(&sh, b)->group[at] = k;
+            else
+                sh.group[at] = k;
+        }
+        if (C > 1) cluster.sync();
+        else block_sync<kW>();
+        if (tid < kG) {
+            const uint32_t mine = sh.group[tid];
+            int ahead = 0;
+#pragma unroll
+            for (int j = 0; j < kG; ++j) {
+                const uint32_t o = sh.group[j];
+                ahead += o > mine || (o == mine && j < tid);
+            }
+            if (ahead == p.n_top - 1) sh.x_key = mine;
+        }
+        if (warp == 0) sh.list[0][lane] = 0;
+        block_sync<kW>();
+        r.X = order_key_to_float(sh.x_key);
+        // the elements that reach it, to the first block
+        const int most = kMaxCand / C;
+        uint64_t* to = first->cand + rank_in * most;
+        auto add = [&](float x, int32_t id) {
+            const int at = atomicAdd(&sh.n_cand, 1);
+            if (at < most) to[at] = loom_rank_key(x, id);
+        };
+        for_slots<kW>(r, &sh, [&](int32_t v, bool there) {
+            for (int i = 0; i < r.per_slot; ++i, v += r.stride) {
+                uint4 w[kU];
+#pragma unroll
+                for (int u = 0; u < kU; ++u) w[u] = load_or_nan<kDtype>(r.vec, v + u * kNT, there && v + u * kNT < r.v1);
+#pragma unroll
+                for (int u = 0; u < kU; ++u) {
+                    if (!(vec_max<kDtype>(w[u]) >= r.X)) continue;
+                    Vec16<kDtype> e;
+                    e.unpack(w[u]);
+#pragma unroll
+                    for (int q = 0; q < kPer; ++q)
+                        if (e.x[q] >= r.X) add(e.x[q], (v + u * kNT) * kPer - r.shift + q);
+                }
+            }
+            return neg_inf();
+        });
+        if (eid >= 0 && ex >= r.X) add(ex, eid);
+    } else if (C > 1) {
+        cluster.barrier_wait();
     }
+
+    // softmax state and rank: warp, block, cluster
+    SoftAcc acc = soft_reduce(st.acc, 32, p.c);
+    int32_t ahead = __reduce_add_sync(0xffffffffu, st.ahead);
     if constexpr (kW > 1) {
         if (lane == 0) {
             sh.acc[warp] = acc;
@@ -537,40 +596,72 @@ __global__ void __launch_bounds__(kW * 32, kW == 1 ? LP_MINB1 : LP_MINB) token_l
             acc = soft_reduce(acc, 32, p.c);
             ahead = __reduce_add_sync(0xffffffffu, lane < kW ? sh.ahead[lane] : 0);
         }
-        if (C > 1) {
-            if (warp == 0) {
-                if (lane == 0) {
-                    sh.block_acc = acc;
-                    sh.block_ahead = ahead;
-                }
-                if constexpr (kTop) sh.block_list[lane] = key;
-            }
-            cluster.sync();
-            if (rank_in == 0) {
-                if constexpr (kTop) {
-                    // (C is at most kW: warp b takes block b's list)
-                    if (warp < C) key = cluster.map_shared_rank(&sh, warp)->block_list[lane];
-                    for (int n = C / 2; n > 0; n >>= 1) {
-                        if (warp >= n && warp < 2 * n) sh.list[warp][lane] = key;
-                        __syncthreads();
-                        if (warp < n) key = merge_lists(key, sh.list[warp + n][lane]);
-                    }
-                }
-                if (warp == 0) {
-                    acc = soft_init();
-                    ahead = 0;
-                    if (lane < C) {
-                        const LpShared<kW>* other = cluster.map_shared_rank(&sh, lane);
-                        acc = other->block_acc;
-                        ahead = other->block_ahead;
-                    }
-                    acc = soft_reduce(acc, 32, p.c);
-                    ahead = __reduce_add_sync(0xffffffffu, ahead);
-                }
-            }
-            cluster.sync();  // no block's shared memory goes away before it has been read
+    } else {
+        __syncwarp();
+    }
+    if (tid == 0) {
+        first->part[rank_in] = acc;
+        first->part_ahead[rank_in] = ahead;
+        if constexpr (kTop) {
+            const int n = sh.n_cand, most = kMaxCand / C;
+            first->part_cand[rank_in] = n < most ? n : most;
+            if (n > most)
+                for (int b = 0; b < C; ++b) (C > 1 ? cluster.map_shared_rank(&sh, b) : &sh)->overflow = 1;
         }
-        if (warp != 0 || rank_in != 0) return;
+    }
+    if (C > 1) cluster.sync();
+    else block_sync<kW>();
+
+    uint64_t key = 0;
+    bool listed = false;
+    if constexpr (kTop) {
+        listed = sh.overflow != 0;
+        if (listed) {  // too many to hand on: each warp sorts its own, then lists by halves, warps and blocks
+            key = list_slots<kDtype, kU, kW>(r, &sh);
+            if (warp == 0) key = merge_lists(key, sort_desc(eid >= 0 && ex >= r.X ? loom_rank_key(ex, eid) : 0ull));
+            for (int h = kW / 2; h > 0; h >>= 1) {
+                if (warp >= h && warp < 2 * h) sh.list[warp][lane] = key;
+                block_sync<kW>();
+                if (warp < h) key = merge_lists(key, sh.list[warp + h][lane]);
+            }
+            if (C > 1) {
+                if (warp == 0) first->part_list[rank_in][lane] = key;
+                cluster.sync();
+                if (warp == 0 && rank_in == 0)
+                    for (int b = 1; b < C; ++b) key = merge_lists(key, sh.part_list[b][lane]);
+            }
+        }
+    }
+    if (rank_in != 0) return;  // (nothing of this block's shared memory is read from here on)
+    if constexpr (kTop) {
+        if (!listed) {
+            int n = 0;
+            const int most = kMaxCand / C;
+            for (int b = 0; b < C; ++b) {
+                const int m = sh.part_cand[b];
+                for (int i = tid; i < m; i += kNT) sh.sorting[n + i] = sh.cand[b * most + i];
+                n += m;
+            }
+            if (tid < 8) sh.sorting[n + tid] = 0;  // (below every key)
+            block_sync<kW>();
+            for (int i = tid; i < n; i += kNT) {
+                const uint64_t mine = sh.sorting[i];
+                int larger = 0;
+                for (int j = 0; j < n; j += 8) {
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) larger += sh.sorting[j + q] > mine;
+                }
+                if (larger < p.n_top) sh.list[0][larger] = mine;
+            }
+            block_sync<kW>();
+            if (warp == 0) key = sh.list[0][lane];
+        }
+    }
+    if (warp != 0) return;
+    if (C > 1) {
+        acc = lane < C ? sh.part[lane] : soft_init();
+        acc = soft_reduce(acc, 32, p.c);
+        ahead = __reduce_add_sync(0xffffffffu, lane < C ? sh.part_ahead[lane] : 0);
     }
 
     const float lns = logf(acc.s);  // -inf for an empty row, NaN where a logit was NaN or +inf
