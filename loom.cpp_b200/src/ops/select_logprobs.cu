@@ -27,7 +27,6 @@ namespace {
 constexpr int64_t kMaxVocab = int64_t(1) << 30;  // ids, and steps past the last one, in 32 bits
 constexpr int kMaxTop = LOOM_SELECT_MAX_TOP_LOGPROBS;
 static_assert(kMaxTop <= 32, "a warp's list is one key per lane");
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // Exponents are clamped here: 2^-200 is zero in f32, and zero times this is zero (a -inf logit would
 // otherwise add 0 * -inf to A).
@@ -453,22 +452,26 @@ __global__ void __launch_bounds__(kW * 32, kW == 1 ? LP_MINB1 : LP_MINB) token_l
     const int32_t steps = (v1 - v0 + stride - 1) / stride;
     const int32_t per_slot = (steps + kSlots - 1) / kSlots;
 
-    uint4 raw[kU];
-    auto load = [&](int32_t v) {
+    // A step's vectors for this lane; in a step that the row's end cuts, those past it are -inf throughout.
+    const int32_t v_start = v0 + rank_in * kU * kNT + warp * 32;
+    const int32_t whole = v1 - (kU - 1) * kNT - 32;  // a warp's step at v is whole when v <= this
+    auto load = [&](uint4(&raw)[kU], int32_t v) {
+        const unsigned char* at = vec + int64_t(v + lane) * 16;
+        if (v <= whole) {
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            const int32_t vu = v + lane + u * kNT;
-            if (vu < v1) {
-                raw[u] = ldg_stream_v4(vec + int64_t(vu) * 16);
-            } else {  // -inf throughout
-                const uint32_t w = kDtype == LOOM_SELECT_BF16 ? 0xff80ff80u : 0xff800000u;
+            for (int u = 0; u < kU; ++u) raw[u] = ldg_stream_v4(at + u * kNT * 16);
+        } else {
+            const uint32_t w = kDtype == LOOM_SELECT_BF16 ? 0xff80ff80u : 0xff800000u;
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
                 raw[u] = make_uint4(w, w, w, w);
+                if (v + lane + u * kNT < v1) raw[u] = ldg_stream_v4(at + u * kNT * 16);
             }
         }
     };
-    const int32_t v_start = v0 + rank_in * kU * kNT + warp * 32;
     int32_t v = v_start;
-    load(v);
+    uint4 raw_a[kU], raw_b[kU];  // the step being added and the next one, whose loads are in flight
+    if (v < v1) load(raw_a, v);
     // the elements of the vectors that the row only partly fills, at most one to a lane of the first warp: those
     // of the first in lanes 0 .. kPer - 1, those of the last in kPer .. 2 kPer - 1
     float ex = neg_inf();
@@ -490,23 +493,17 @@ __global__ void __launch_bounds__(kW * 32, kW == 1 ? LP_MINB1 : LP_MINB) token_l
 
     float top = neg_inf(), slot_top = neg_inf();  // this thread's maximum, and its maximum in the current slot
     int32_t slot = 0, in_slot = 0;
-    while (v < v1) {  // warp-uniform
-        const int32_t at = v;
-        uint4 cur[kU];
+    auto step = [&](const uint4(&raw)[kU], int32_t at) {
+        float mx = vec_max<kDtype>(raw[0]);  // (NaN left out)
 #pragma unroll
-        for (int u = 0; u < kU; ++u) cur[u] = raw[u];
-        v += stride;
-        if (v < v1) load(v);  // the next step's loads are in flight while this one is added
-        float mx = neg_inf();
-#pragma unroll
-        for (int u = 0; u < kU; ++u) mx = fmaxf(mx, vec_max<kDtype>(cur[u]));  // (NaN left out)
-        st.add(cur, mx, at + (kU - 1) * kNT + 32 > v1);
+        for (int u = 1; u < kU; ++u) mx = fmaxf(mx, vec_max<kDtype>(raw[u]));
+        st.add(raw, mx, at > whole);
         if (rank)
-            st.count(cur, mx, (at + lane) * kPer - shift, kNT * kPer, limit, at * kPer - shift,
+            st.count(raw, mx, (at + lane) * kPer - shift, kNT * kPer, limit, at * kPer - shift,
                      (at + (kU - 1) * kNT + 32) * kPer - shift, xt, t);
-        slot_top = fmaxf(slot_top, mx);
         if constexpr (kTop) {
-            if (++in_slot == per_slot || v >= v1) {
+            slot_top = fmaxf(slot_top, mx);
+            if (++in_slot == per_slot || at + stride >= v1) {
                 sh.slot_max[warp][slot][lane] = slot_top;
                 top = fmaxf(top, slot_top);
                 slot_top = neg_inf();
@@ -514,6 +511,15 @@ __global__ void __launch_bounds__(kW * 32, kW == 1 ? LP_MINB1 : LP_MINB) token_l
                 in_slot = 0;
             }
         }
+    };
+    while (v < v1) {  // warp-uniform
+        if (v + stride < v1) load(raw_b, v + stride);
+        step(raw_a, v);
+        v += stride;
+        if (v >= v1) break;
+        if (v + stride < v1) load(raw_a, v + stride);
+        step(raw_b, v);
+        v += stride;
     }
     if (warp == 0 && rank_in == 0) {
         if (ex > st.acc.m) st.acc = soft_move(st.acc, ex, p.c);
@@ -733,9 +739,10 @@ cudaError_t launch_lp_any(const LpDev& p, int64_t rows, int sms, cudaStream_t s)
 // the gradient, nothing else. Bound: HBM.
 struct LpGradDev {
     const unsigned char* base;
-    int64_t width, row_stride;
+    int64_t rows, width, row_stride;
     const int32_t* ids;
-    float inv_t, inv_t_lo;  // 1 / T and what rounding it lost
+    double T;
+    float inv_t, c;  // 1 / T, log2(e) / T
     const float* lse;
     const float* entropy;
     const float* g_logp;
@@ -750,41 +757,148 @@ __device__ __forceinline__ void store_elem(void* base, int64_t i, float v) {
     else reinterpret_cast<float*>(base)[i] = v;
 }
 
+// (plain loads: the gradient may be written over the logits)
+template <int kDtype>
+__device__ __forceinline__ float plain_elem(const void* base, int64_t i) {
+    if constexpr (kDtype == LOOM_SELECT_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base)[i]);
+    else return reinterpret_cast<const float*>(base)[i];
+}
+
+__device__ __forceinline__ uint4 plain_v4(const void* p) {
+    uint4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                 : "l"(p)
+                 : "memory");
+    return r;
+}
+
+// What a row's elements share. l / ln 2 = ((x - lse T) log2(e) / T), with lse T in two f32 parts: near the row's
+// likely elements the first difference is exact, so l is off by a few units of its own size and not of lse's.
 struct LpGradRow {
-    float g, h, lse, ent, inv_t, inv_t_lo;
-    // x / T - lse with 1 / T in two parts: the rounding of 1 / T alone would be off by |y| 2^-24.
-    __device__ __forceinline__ float grad(float x, bool at) const {
-        // (-inf logits as -FLT_MAX: their p is 0 all the same, and -inf * 0 would be NaN)
-        x = max_nan(x, -FLT_MAX);
-        const float l = __fmaf_rn(x, inv_t, __fmaf_rn(x, inv_t_lo, -lse));
-        const float e = ex2(__fmul_rn(l, kLog2e));
-        float d = e == 0.0f ? 0.0f : -e * (g + (h == 0.0f ? 0.0f : h * (l + ent)));
-        if (at) d += g;
-        return d * inv_t;
+    float hi, lo;   // lse T
+    float g, h;     // the gradient is -p (g + h l / ln 2), plus `at` at t
+    float c;        // log2(e) / T
+    float at;
+
+    __device__ __forceinline__ float grad(float x, bool is_t) const {
+        // (clamped: p is 0 there, and stays finite times l)
+        const float l = max_nan(__fmul_rn(__fsub_rn(__fsub_rn(x, hi), lo), c), kMinExp2);
+        const float d = __fmul_rn(ex2(l), __fmaf_rn(h, l, g));
+        return is_t ? at - d : -d;
+    }
+
+    // Two at a time; the signs of g and h are turned, so that no negation is left.
+    __device__ __forceinline__ uint64_t grad2(uint64_t x, uint64_t hi2, uint64_t lo2, uint64_t c2, uint64_t h2,
+                                              uint64_t g2) const {
+        asm("sub.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(hi2));
+        asm("sub.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(lo2));
+        asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(c2));
+        float l0, l1;
+        unpack2(x, l0, l1);
+        l0 = max_nan(l0, kMinExp2);
+        l1 = max_nan(l1, kMinExp2);
+        fma2(g2, h2, pack2(l0, l1));
+        const uint64_t e = pack2(ex2(l0), ex2(l1));
+        asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(g2) : "l"(e));
+        return g2;
     }
 };
 
 constexpr int kGradNT = 256;
+// Four vectors a thread keep the reads and the writes both going: [1024, 151936] f32 193.7 us (2 vectors: 202.6, 8: 188.3)
+// and bf16 96.6 us (114.6, 108.7), where a copy of the same bytes takes 190 and 95 us.
+constexpr int kGradU = 4;
+// Rows up to this wide go a warp to a row: [16384, 1025] f32 32.7 us (a block to a row: 110).
+constexpr int64_t kGradNarrow = 4096;
 
-template <int kDtype>
-__global__ void __launch_bounds__(kGradNT) token_logprobs_grad_kernel(const LpGradDev p) {
+// kTPR threads per piece of a row (kGradU vectors a thread), 256 / kTPR pieces to a block. Rows of logits and of the gradient that start at the same
+// place within 16 bytes go by vectors, but for the ones the row only partly fills; others element by element.
+template <int kDtype, int kTPR>
+__global__ void __launch_bounds__(kGradNT) token_logprobs_grad_kernel(const LpGradDev p, int32_t pieces) {
     constexpr int kEsz = kDtype == LOOM_SELECT_BF16 ? 2 : 4;
-    const int64_t row = blockIdx.x;
+    constexpr int kPer = 16 / kEsz;
+    const uint32_t unit = blockIdx.x * (kGradNT / kTPR) + threadIdx.x / kTPR;
+    const int64_t row = unit / unsigned(pieces);
+    const int32_t piece = int32_t(unit % unsigned(pieces));
+    const int32_t thread = threadIdx.x % kTPR;
+    if (row >= p.rows) return;
     const unsigned char* in = p.base + row * p.row_stride * kEsz;
     unsigned char* out = p.out + row * p.out_stride * kEsz;
-    const int64_t t = p.ids ? p.ids[row] : -1;
+    const int32_t shift = int32_t((reinterpret_cast<uintptr_t>(in) & 15) / kEsz);
+    const bool vectors = shift == int32_t((reinterpret_cast<uintptr_t>(out) & 15) / kEsz);
+    const int32_t v = piece * kGradU * kTPR + thread;  // this thread's first vector, the others kTPR apart
+
+    const int32_t t = p.ids ? p.ids[row] : -1;
+    const float g = p.g_logp && t >= 0 ? p.g_logp[row] : 0.0f;
+    const float h = p.g_entropy ? p.g_entropy[row] : 0.0f;
+    const float lse = p.lse[row];
+    const float ent = h != 0.0f ? p.entropy[row] : 0.0f;
+    const bool zero = g == 0.0f && h == 0.0f;
+    uint4 raw[kGradU];
+#pragma unroll
+    for (int u = 0; u < kGradU; ++u) {
+        const int32_t first = (v + u * kTPR) * kPer - shift;
+        if (vectors && !zero && first >= 0 && first + kPer <= p.width)
+            raw[u] = plain_v4(in + int64_t(first) * kEsz);
+    }
     LpGradRow r;
-    r.g = p.g_logp && t >= 0 ? p.g_logp[row] : 0.0f;
-    r.h = p.g_entropy ? p.g_entropy[row] : 0.0f;
-    const bool zero = r.g == 0.0f && r.h == 0.0f;
-    r.lse = p.lse[row];
-    r.ent = r.h != 0.0f ? p.entropy[row] : 0.0f;
+    const double lt = double(lse) * p.T;
+    r.hi = __double2float_rn(lt);
+    r.lo = __double2float_rn(lt - double(r.hi));
+    r.c = p.c;
+    r.at = __fmul_rn(g, p.inv_t);
+    const float hs = __fmul_rn(h, p.inv_t);
+    r.g = h != 0.0f ? __fmaf_rn(hs, ent, r.at) : r.at;
+    r.h = __fmul_rn(hs, kLn2);
     // an id past the vocabulary, an empty row, a row with NaN or +inf: NaN throughout
-    const bool bad = (t >= p.width && r.g != 0.0f) || !(fabsf(r.lse) <= FLT_MAX);
-    r.inv_t = bad ? quiet_nan() : p.inv_t;
-    r.inv_t_lo = p.inv_t_lo;
-    for (int64_t j = threadIdx.x; j < p.width; j += kGradNT)
-        store_elem<kDtype>(out, j, zero ? 0.0f : r.grad(load_global_elem<kDtype>(in, j), j == t));
+    if (!(fabsf(lse) <= FLT_MAX) || (t >= p.width && g != 0.0f)) r.g = quiet_nan();
+    const uint64_t hi2 = pack2(r.hi, r.hi), lo2 = pack2(r.lo, r.lo), c2 = pack2(r.c, r.c), h2 = pack2(-r.h, -r.h),
+                   g2 = pack2(-r.g, -r.g);
+#pragma unroll
+    for (int u = 0; u < kGradU; ++u) {
+        const int32_t first = (v + u * kTPR) * kPer - shift;
+        if (vectors && first >= 0 && first + kPer <= p.width) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (!zero) {
+                const Pairs<kDtype> x(raw[u]);
+                float d[kPer];
+#pragma unroll
+                for (int q = 0; q < kPer / 2; ++q) unpack2(r.grad2(x.v[q], hi2, lo2, c2, h2, g2), d[2 * q], d[2 * q + 1]);
+                if (t >= first && t < first + kPer) {
+#pragma unroll
+                    for (int q = 0; q < kPer; ++q) d[q] += first + q == t ? r.at : 0.0f;
+                }
+                if constexpr (kDtype == LOOM_SELECT_BF16) {
+                    uint32_t b[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const __nv_bfloat162 pr = __floats2bfloat162_rn(d[2 * q], d[2 * q + 1]);
+                        b[q] = *reinterpret_cast<const uint32_t*>(&pr);
+                    }
+                    w = make_uint4(b[0], b[1], b[2], b[3]);
+                } else {
+                    w = make_uint4(__float_as_uint(d[0]), __float_as_uint(d[1]), __float_as_uint(d[2]),
+                                   __float_as_uint(d[3]));
+                }
+            }
+            *reinterpret_cast<uint4*>(out + int64_t(first) * kEsz) = w;
+        } else if (vectors) {
+            for (int q = 0; q < kPer; ++q) {
+                const int32_t id = first + q;
+                if (id >= 0 && id < p.width)
+                    store_elem<kDtype>(out, id, zero ? 0.0f : r.grad(plain_elem<kDtype>(in, id), id == t));
+            }
+        }
+    }
+    if (!vectors) {
+        const int32_t begin = piece * kGradU * kTPR * kPer;
+        for (int j = 0; j < kGradU * kPer; ++j) {
+            const int32_t id = begin + j * kTPR + thread;
+            if (id < p.width)
+                store_elem<kDtype>(out, id, zero ? 0.0f : r.grad(plain_elem<kDtype>(in, id), id == t));
+        }
+    }
 }
 
 bool dtype_ok(int dtype) { return dtype == LOOM_SELECT_F32 || dtype == LOOM_SELECT_BF16; }
@@ -863,12 +977,13 @@ LOOM_SELECT_API int loom_token_logprobs_grad(const void* logits, int dtype, int6
     if (logits == out_grad && row_stride != grad_stride) return LOOM_SELECT_EINVAL;
     LpGradDev p;
     p.base = static_cast<const unsigned char*>(logits);
+    p.rows = rows;
     p.width = n_vocab;
     p.row_stride = row_stride;
     p.ids = ids;
-    const double inv = 1.0 / double(temperature);
-    p.inv_t = float(inv);
-    p.inv_t_lo = float(inv - double(p.inv_t));
+    p.T = double(temperature);
+    p.inv_t = float(1.0 / double(temperature));
+    p.c = float(1.4426950408889634 / double(temperature));
     p.lse = lse;
     p.entropy = entropy;
     p.g_logp = grad_logp;
@@ -876,8 +991,20 @@ LOOM_SELECT_API int loom_token_logprobs_grad(const void* logits, int dtype, int6
     p.out = static_cast<unsigned char*>(out_grad);
     p.out_stride = grad_stride;
     const auto s = static_cast<cudaStream_t>(stream);
-    if (dtype == LOOM_SELECT_BF16) token_logprobs_grad_kernel<LOOM_SELECT_BF16><<<unsigned(rows), kGradNT, 0, s>>>(p);
-    else token_logprobs_grad_kernel<LOOM_SELECT_F32><<<unsigned(rows), kGradNT, 0, s>>>(p);
+    const bool narrow = n_vocab <= kGradNarrow;
+    const int64_t per_piece = int64_t(kGradU) * (narrow ? 32 : kGradNT) * (dtype == LOOM_SELECT_BF16 ? 8 : 4);
+    const int64_t pieces = (n_vocab + 7 + per_piece - 1) / per_piece;  // (a row may start inside a vector)
+    const int64_t per_block = narrow ? kGradNT / 32 : 1, blocks = (rows * pieces + per_block - 1) / per_block;
+    if (rows * pieces > INT32_MAX) return LOOM_SELECT_ESHAPE;
+    const unsigned grid = unsigned(blocks);
+    const int32_t n = int32_t(pieces);
+    if (dtype == LOOM_SELECT_BF16) {
+        if (narrow) token_logprobs_grad_kernel<LOOM_SELECT_BF16, 32><<<grid, kGradNT, 0, s>>>(p, n);
+        else token_logprobs_grad_kernel<LOOM_SELECT_BF16, kGradNT><<<grid, kGradNT, 0, s>>>(p, n);
+    } else {
+        if (narrow) token_logprobs_grad_kernel<LOOM_SELECT_F32, 32><<<grid, kGradNT, 0, s>>>(p, n);
+        else token_logprobs_grad_kernel<LOOM_SELECT_F32, kGradNT><<<grid, kGradNT, 0, s>>>(p, n);
+    }
     return cudaGetLastError() == cudaSuccess ? LOOM_SELECT_OK : LOOM_SELECT_ECUDA;
 }
 
