@@ -46,98 +46,371 @@ __device__ __forceinline__ float nan_max(float a, float b) {
     return y;
 }
 
-template <int kDtype>
-__device__ __forceinline__ float round_to(float v) {
-    if constexpr (kDtype == LOOM_SELECT_BF16) return __bfloat162float(__float2bfloat16_rn(v));
-    else return v;
-}
-
-template <int kDtype>
-__device__ __forceinline__ float plain_load(const void* base, int64_t i) {
-    if constexpr (kDtype == LOOM_SELECT_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base)[i]);
-    else return reinterpret_cast<const float*>(base)[i];
-}
-
-template <int kDtype>
-__device__ __forceinline__ void plain_store(void* base, int64_t i, float v) {
-    if constexpr (kDtype == LOOM_SELECT_BF16) reinterpret_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(v);
-    else reinterpret_cast<float*>(base)[i] = v;
-}
-
-// kNT threads hold one row, kPer elements each: thread t the elements t, t + kNT, ...
-template <int kDtype, int kWDtype, bool kNorm, int kNT, int kPer>
-__global__ void __launch_bounds__(kNT) quant_rows_kernel(const QuantDev p) {
-    constexpr int kEsz = kDtype == LOOM_SELECT_BF16 ? 2 : 4;
-    constexpr int kWarps = kNT / 32;
-    __shared__ double part_ss[kWarps];
-    __shared__ float part_max[kWarps];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t row = blockIdx.x;
-    const unsigned char* x = p.x + row * p.x_stride * kEsz;
-    float h[kPer];
+// The 16-byte vectors around kWords 32-bit words that begin at a multiple of 2.
+template <int kWords>
+struct Around {
+    static constexpr int kVecs = (kWords + 3) / 4 + 1;
+    uint32_t w[4 * kVecs];
+    // Those of the vectors that hold something before `end` (the others are not touched).
+    __device__ __forceinline__ void load(const unsigned char* at, const unsigned char* end, bool there) {
+        const unsigned char* v = at - (reinterpret_cast<uintptr_t>(at) & 15);
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const int i = j * kNT + tid;
-        h[j] = i < p.dim ? plain_load<kDtype>(x, i) : 0.0f;
+        for (int i = 0; i < kVecs; ++i) {
+            uint4 r = make_uint4(0, 0, 0, 0);
+            if (there && v + 16 * i < end) r = reinterpret_cast<const uint4*>(v)[i];
+            w[4 * i] = r.x, w[4 * i + 1] = r.y, w[4 * i + 2] = r.z, w[4 * i + 3] = r.w;
+        }
     }
-    if constexpr (kNorm) {
-        if (p.residual) {
-            const unsigned char* r = p.residual + row * p.residual_stride * kEsz;
-            unsigned char* s = p.sum ? p.sum + row * p.sum_stride * kEsz : nullptr;
+    // The words themselves. The shift is the same for a whole row's runs, so the branches are uniform.
+    __device__ __forceinline__ void get(const unsigned char* at, uint32_t (&out)[kWords]) const {
+        const uint32_t s = uint32_t(reinterpret_cast<uintptr_t>(at) & 15), bits = (s & 2) * 8;
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                const int i = j * kNT + tid;
-                if (i < p.dim) {
-                    h[j] = round_to<kDtype>(__fadd_rn(h[j], plain_load<kDtype>(r, i)));
-                    if (s) plain_store<kDtype>(s, i, h[j]);
+        for (int skip = 0; skip < 4; ++skip) {
+            if (s >> 2 == skip) {
+#pragma unroll
+                for (int q = 0; q < kWords; ++q) out[q] = __funnelshift_r(w[q + skip], w[q + skip + 1], bits);
+            }
+        }
+    }
+};
+
+// Elements [id, id + kN) of a row of dim elements, zeros outside it. kAligned: the row begins at a vector and the run is
+// either whole or outside.
+template <int kDtype, int kN, bool kAligned>
+__device__ __forceinline__ void load_run(const unsigned char* base, int32_t id, int32_t dim, float (&x)[kN]) {
+    constexpr int kEsz = kDtype == LOOM_SELECT_BF16 ? 2 : 4;
+    constexpr int kWords = kN * kEsz / 4;
+    const unsigned char* at = base + int64_t(id) * kEsz;
+    uint32_t w[kWords];
+#pragma unroll
+    for (int q = 0; q < kWords; ++q) w[q] = 0;
+    if constexpr (kAligned) {
+        if (id + kN <= dim) {
+            if constexpr (kWords == 2) {
+                const uint2 r = *reinterpret_cast<const uint2*>(at);
+                w[0] = r.x, w[1] = r.y;
+            } else {
+#pragma unroll
+                for (int q = 0; q < kWords; q += 4) {
+                    const uint4 r = *reinterpret_cast<const uint4*>(at + 4 * q);
+                    w[q] = r.x, w[q + 1] = r.y, w[q + 2] = r.z, w[q + 3] = r.w;
                 }
             }
         }
-        double ss = 0.0;
+    } else {
+        // f32 word by word, which is quicker for four of them ([30000, 1037] 108 us; by vectors 142); others by the vectors
+        // around the run where those lie in the row
+        constexpr bool kByWord = kDtype == LOOM_SELECT_F32 && kN == 4;
+        const unsigned char* lo = kByWord ? at : at - (reinterpret_cast<uintptr_t>(at) & 15);
+        const unsigned char* hi = kByWord ? at + 16 : lo + 16 * ((kWords + 3) / 4 + 1);
+        if (id < dim && lo >= base && hi <= base + int64_t(dim) * kEsz) {
+            if constexpr (kByWord) {
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) ss = __fma_rn(double(h[j]), double(h[j]), ss);
+                for (int q = 0; q < kWords; ++q) w[q] = reinterpret_cast<const uint32_t*>(at)[q];
+            } else {
+                Around<kWords> around;
+                around.load(at, hi, true);
+                around.get(at, w);
+            }
+        } else {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (lane == 0) part_ss[warp] = ss;
-        __syncthreads();
-        ss = part_ss[0];
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) ss += part_ss[w];
-        const float inv = __double2float_rn(__drcp_rn(__dsqrt_rn(__ddiv_rn(ss, double(p.dim)) + p.eps)));
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const int i = j * kNT + tid;
-            if (i < p.dim) h[j] = __fmul_rn(__fmul_rn(h[j], inv), plain_load<kWDtype>(p.weight, i));
+            for (int q = 0; q < kN; ++q) {
+                if (id + q >= 0 && id + q < dim) {
+                    if constexpr (kDtype == LOOM_SELECT_BF16)
+                        w[q / 2] |= uint32_t(reinterpret_cast<const unsigned short*>(base)[id + q]) << (16 * (q % 2));
+                    else
+                        w[q] = reinterpret_cast<const uint32_t*>(base)[id + q];
+                }
+            }
         }
     }
-    float a = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) a = nan_max(a, fabsf(h[j]));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) a = nan_max(a, __shfl_xor_sync(0xffffffffu, a, o));
-    if (lane == 0) part_max[warp] = a;
-    __syncthreads();
-    a = part_max[0];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) a = nan_max(a, part_max[w]);
-    // a NaN or an infinity anywhere: q 0 and a NaN scale, so that what is made of them is NaN
-    const bool fine = a <= FLT_MAX, some = fine && a >= kTinyRow;
-    const float inv_scale = some ? __fmul_rn(__frcp_rn(a), 127.0f) : 0.0f;
-    if (tid == 0) p.scale[row] = !fine ? __int_as_float(0x7fc00000) : some ? __fdiv_rn(a, 127.0f) : 0.0f;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const int i = j * kNT + tid;
-        if (i < p.dim)
-            p.q[row * p.dim + i] = some ? static_cast<int8_t>(__float2int_rn(__fmul_rn(h[j], inv_scale))) : int8_t(0);
+    for (int q = 0; q < kWords; ++q) {
+        if constexpr (kDtype == LOOM_SELECT_BF16) {
+            x[2 * q] = __uint_as_float(w[q] << 16);
+            x[2 * q + 1] = __uint_as_float(w[q] & 0xffff0000u);
+        } else {
+            x[q] = __uint_as_float(w[q]);
+        }
     }
 }
 
+// The four words of a run to elements [id, id + 16 / element size) of a row of dim elements, those outside it left out.
+template <int kDtype, bool kAligned>
+__device__ __forceinline__ void store_run(unsigned char* base, int32_t id, int32_t dim, const uint32_t (&w)[4]) {
+    constexpr int kEsz = kDtype == LOOM_SELECT_BF16 ? 2 : 4;
+    constexpr int kPer = 16 / kEsz;
+    unsigned char* at = base + int64_t(id) * kEsz;
+    const bool whole = id >= 0 && id + kPer <= dim;
+    if constexpr (kAligned) {
+        if (whole) *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else if (whole && (reinterpret_cast<uintptr_t>(at) & 3) == 0) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) reinterpret_cast<uint32_t*>(at)[q] = w[q];
+    } else if (whole) {  // bf16 between words
+        *reinterpret_cast<unsigned short*>(at) = (unsigned short)w[0];
+#pragma unroll
+        for (int q = 0; q < 3; ++q) *reinterpret_cast<uint32_t*>(at + 2 + 4 * q) = __funnelshift_r(w[q], w[q + 1], 16);
+        *reinterpret_cast<unsigned short*>(at + 14) = (unsigned short)(w[3] >> 16);
+    } else {
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) {
+            if (id + q >= 0 && id + q < dim) {
+                if constexpr (kDtype == LOOM_SELECT_BF16)
+                    reinterpret_cast<unsigned short*>(base)[id + q] = (unsigned short)(w[q / 2] >> (16 * (q % 2)));
+                else
+                    reinterpret_cast<uint32_t*>(base)[id + q] = w[q];
+            }
+        }
+    }
+}
+
+// A thread's kPer elements in the rows' own type, four registers: f32 x 4 or bf16 x 8.
+template <int kDtype>
+struct Held {
+    static constexpr int kPer = kDtype == LOOM_SELECT_BF16 ? 8 : 4;
+    uint32_t w[4];
+    __device__ __forceinline__ void get(float (&x)[kPer]) const {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if constexpr (kDtype == LOOM_SELECT_BF16) {
+                x[2 * q] = __uint_as_float(w[q] << 16);
+                x[2 * q + 1] = __uint_as_float(w[q] & 0xffff0000u);
+            } else {
+                x[q] = __uint_as_float(w[q]);
+            }
+        }
+    }
+    __device__ __forceinline__ void set(const float (&x)[kPer]) {  // rounds to the type
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if constexpr (kDtype == LOOM_SELECT_BF16) {
+                const __nv_bfloat162 t = __floats2bfloat162_rn(x[2 * q], x[2 * q + 1]);
+                w[q] = *reinterpret_cast<const uint32_t*>(&t);
+            } else {
+                w[q] = __float_as_uint(x[q]);
+            }
+        }
+    }
+};
+
+// kTPR threads hold one row, kVPT runs of kPer neighbouring elements each, kTPR runs apart; a block holds one row, or
+// several of those a warp or less holds. All of a thread's loads are in flight together, and its elements stay in
+// registers. Runs are laid out by the output: run k covers ids [k kPer - lead, (k + 1) kPer - lead), where out_q's row
+// begins `lead` bytes after a multiple of kPer, so that a whole run is one store. kAligned: every row of every tensor
+// begins at a vector (lead is 0).
+//
+// Resident threads per SM asked of the compiler: 1024 (64 registers) where it takes registers to keep the loads in flight,
+// 1536 (40) for the plain aligned quantiser, whose [151936, 2048] bf16 takes 132.5 us then (1024: 134.7; the bytes at
+// the copy rate 142.8); two blocks of 1024 threads where that is the block ([8192, 16384] f32 96.9 us; one: 128).
+constexpr int min_blocks(bool norm, bool aligned, int threads) {
+    return norm || !aligned ? 1024 / threads : threads == 1024 ? 2 : 1536 / threads;
+}
+
+template <int kDtype, int kWDtype, bool kNorm, int kTPR, int kVPT, bool kAligned>
+__global__ void __launch_bounds__(kTPR < 64 ? 128 : kTPR, min_blocks(kNorm, kAligned, kTPR < 64 ? 128 : kTPR))
+    quant_rows_kernel(const QuantDev p) {
+    constexpr int kEsz = kDtype == LOOM_SELECT_BF16 ? 2 : 4;
+    constexpr int kPer = 16 / kEsz;
+    constexpr int kWarps = kTPR / 32;  // 0: several rows to a warp
+    constexpr int kRows = kTPR < 64 ? 128 / kTPR : 1;
+    // y in f32 where a thread has few elements; with many, bf16 rows make it again for the output (from the row and
+    // the weight in L1)
+    constexpr bool kHoldY = kNorm && (kDtype == LOOM_SELECT_F32 || kVPT <= 4);
+    __shared__ double part_ss[kWarps > 1 ? kWarps : 1];
+    __shared__ float part_max[kWarps > 1 ? kWarps : 1];
+    __shared__ float row_inv;
+    const int tid = threadIdx.x % kTPR, lane = tid & 31, warp = tid >> 5;
+    const int64_t row_or_past = int64_t(blockIdx.x) * kRows + threadIdx.x / kTPR;
+    const bool there = kRows == 1 || row_or_past < p.rows;  // (warps stay whole: rows past the last do nothing)
+    const int64_t row = there ? row_or_past : 0;
+    const int32_t dim = there ? p.dim : 0;
+    unsigned char* out = reinterpret_cast<unsigned char*>(p.q + row * p.dim);
+    const int32_t lead = kAligned ? 0 : int32_t(reinterpret_cast<uintptr_t>(out) % kPer);
+    auto first = [&](int j) { return (j * kTPR + tid) * kPer - lead; };
+
+    // The runs of one tensor's row. Unaligned bf16 rows but for the tensor's first and last: all the vectors around the
+    // runs are requested before any is shifted (what they hold of the neighbouring rows is masked off).
+    const bool inner = !kAligned && kDtype == LOOM_SELECT_BF16 && row > 0 && row + 1 < p.rows;
+    auto load_row = [&](const unsigned char* base, Held<kDtype>(&to)[kVPT]) {
+        if (inner) {
+            Around<4> around[kVPT];
+#pragma unroll
+            for (int j = 0; j < kVPT; ++j)
+                around[j].load(base + int64_t(first(j)) * kEsz, base + int64_t(dim) * kEsz, first(j) < dim);
+#pragma unroll
+            for (int j = 0; j < kVPT; ++j) {
+                const int32_t id = first(j);
+                around[j].get(base + int64_t(id) * kEsz, to[j].w);
+                if (id < 0 || id + kPer > dim) {
+                    float v[kPer];
+                    to[j].get(v);
+#pragma unroll
+                    for (int q = 0; q < kPer; ++q) v[q] = id + q >= 0 && id + q < dim ? v[q] : 0.0f;
+                    to[j].set(v);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kVPT; ++j) {
+                float v[kPer];
+                load_run<kDtype, kPer, kAligned>(base, first(j), dim, v);
+                to[j].set(v);
+            }
+        }
+    };
+    Held<kDtype> h[kVPT];
+    load_row(p.x + row * p.x_stride * kEsz, h);
+    if (kNorm && p.residual) {
+        const unsigned char* r = p.residual + row * p.residual_stride * kEsz;
+        unsigned char* s = p.sum ? p.sum + row * p.sum_stride * kEsz : nullptr;
+        Held<kDtype> add[kVPT];
+        load_row(r, add);
+#pragma unroll
+        for (int j = 0; j < kVPT; ++j) {
+            float v[kPer], u[kPer];
+            h[j].get(v);
+            add[j].get(u);
+#pragma unroll
+            for (int q = 0; q < kPer; ++q) v[q] = __fadd_rn(v[q], u[q]);
+            h[j].set(v);
+            if (s) store_run<kDtype, kAligned>(s, first(j), dim, h[j].w);
+        }
+    }
+    float inv = 0.0f;
+    if constexpr (kNorm) {
+        double ss = 0.0;
+#pragma unroll
+        for (int j = 0; j < kVPT; ++j) {
+            float v[kPer];
+            h[j].get(v);
+#pragma unroll
+            for (int q = 0; q < kPer; ++q) ss = __fma_rn(double(v[q]), double(v[q]), ss);
+        }
+#pragma unroll
+        for (int o = (kTPR < 32 ? kTPR : 32) / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        // (64-bit division and square root by one warp: every warp's would take turns at the unit)
+        auto inverse = [&](double sum) {
+            return __double2float_rn(__drcp_rn(__dsqrt_rn(__ddiv_rn(sum, double(p.dim)) + p.eps)));
+        };
+        if constexpr (kWarps > 1) {
+            if (lane == 0) part_ss[warp] = ss;
+            __syncthreads();
+            if (warp == 0) {
+                ss = part_ss[0];
+#pragma unroll
+                for (int w = 1; w < kWarps; ++w) ss += part_ss[w];
+                inv = inverse(ss);
+                if (lane == 0) row_inv = inv;
+            }
+            __syncthreads();
+            inv = row_inv;
+        } else {
+            inv = inverse(ss);
+        }
+    }
+    auto make = [&](int j, float (&v)[kPer]) {
+        h[j].get(v);
+        if constexpr (kNorm) {
+            float w[kPer];
+            load_run<kWDtype, kPer, kAligned>(p.weight, first(j), dim, w);
+#pragma unroll
+            for (int q = 0; q < kPer; ++q) v[q] = __fmul_rn(__fmul_rn(v[q], inv), w[q]);
+        }
+    };
+    float y[kHoldY ? kVPT : 1][kPer];
+    float a = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kVPT; ++j) {
+        float v[kPer];
+        make(j, v);
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) {
+            a = nan_max(a, fabsf(v[q]));
+            if constexpr (kHoldY) y[j][q] = v[q];
+        }
+    }
+#pragma unroll
+    for (int o = (kTPR < 32 ? kTPR : 32) / 2; o > 0; o >>= 1) a = nan_max(a, __shfl_xor_sync(0xffffffffu, a, o));
+    if constexpr (kWarps > 1) {
+        if (lane == 0) part_max[warp] = a;
+        __syncthreads();
+        a = part_max[0];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) a = nan_max(a, part_max[w]);
+    }
+    // a NaN or an infinity anywhere: q 0 and a NaN scale, so that what is made of them is NaN
+    const bool fine = a <= FLT_MAX, some = fine && a >= kTinyRow;
+    const float inv_scale = some ? __fmul_rn(__frcp_rn(a), 127.0f) : 0.0f;
+    if (tid == 0 && there) p.scale[row] = !fine ? __int_as_float(0x7fc00000) : some ? __fdiv_rn(a, 127.0f) : 0.0f;
+    // rint by adding 1.5 * 2^23 (to nearest even): the sum's low byte is the two's complement 8-bit integer
+    constexpr float kMagic = 12582912.0f;
+#pragma unroll
+    for (int j = 0; j < kVPT; ++j) {
+        float v[kPer];
+        if constexpr (kHoldY) {
+#pragma unroll
+            for (int q = 0; q < kPer; ++q) v[q] = y[j][q];
+        } else {
+            make(j, v);
+        }
+        uint32_t w[kPer / 4];
+#pragma unroll
+        for (int k = 0; k < kPer / 4; ++k) {
+            uint32_t b[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) b[q] = __float_as_uint(__fadd_rn(__fmul_rn(v[4 * k + q], inv_scale), kMagic));
+            w[k] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+            if (!some) w[k] = 0;  // (a NaN row's products are not numbers)
+        }
+        const int32_t id = first(j);
+        if ((kAligned || id >= 0) && id + kPer <= dim) {
+            if constexpr (kPer == 8) *reinterpret_cast<uint2*>(out + id) = make_uint2(w[0], w[1]);
+            else *reinterpret_cast<uint32_t*>(out + id) = w[0];
+        } else if (!kAligned) {
+#pragma unroll
+            for (int q = 0; q < kPer; ++q)
+                if (id + q >= 0 && id + q < dim) out[id + q] = (unsigned char)(w[q / 4] >> (8 * (q % 4)));
+        }
+    }
+}
+
+bool multiple_of(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+template <int kDtype, int kWDtype, bool kNorm, int kTPR, int kVPT, bool kAligned>
+void launch_rows(const QuantDev& p, cudaStream_t s) {
+    constexpr int kRows = kTPR < 64 ? 128 / kTPR : 1;
+    quant_rows_kernel<kDtype, kWDtype, kNorm, kTPR, kVPT, kAligned>
+        <<<unsigned((p.rows + kRows - 1) / kRows), kTPR * kRows, 0, s>>>(p);
+}
+
+// Threads for a row: as few as hold it at four runs each, since they have many loads in flight and little to join;
+// more, up to a run each, when the rows do not give every SM 256 threads ([1024, 1025] f32 3.0 us; with 1024 threads
+// asked for 4.6).
+template <int kDtype, int kWDtype, bool kNorm, bool kAligned>
+void launch_any(const QuantDev& p, int sms, cudaStream_t s) {
+    constexpr int kPer = kDtype == LOOM_SELECT_BF16 ? 8 : 4;
+    const int nv = (p.dim + (kAligned ? 0 : kPer - 1) + kPer - 1) / kPer;
+    int tpr = 8;
+    while (tpr < 1024 && (nv > tpr * 4 || (tpr < nv && p.rows * tpr < int64_t(sms) * 256))) tpr *= tpr == 8 ? 4 : 2;
+    if (tpr == 8) launch_rows<kDtype, kWDtype, kNorm, 8, 4, kAligned>(p, s);
+    else if (tpr == 32) launch_rows<kDtype, kWDtype, kNorm, 32, 4, kAligned>(p, s);
+    else if (tpr == 64) launch_rows<kDtype, kWDtype, kNorm, 64, 4, kAligned>(p, s);
+    else if (tpr == 128) launch_rows<kDtype, kWDtype, kNorm, 128, 4, kAligned>(p, s);
+    else if (tpr == 256) launch_rows<kDtype, kWDtype, kNorm, 256, 4, kAligned>(p, s);
+    else if (tpr == 512) launch_rows<kDtype, kWDtype, kNorm, 512, 4, kAligned>(p, s);
+    else if (nv <= 1024 * 4) launch_rows<kDtype, kWDtype, kNorm, 1024, 4, kAligned>(p, s);
+    else launch_rows<kDtype, kWDtype, kNorm, 1024, kAligned ? 8 : 9, kAligned>(p, s);
+}
+
 template <int kDtype, int kWDtype, bool kNorm>
-cudaError_t launch_quant_t(const QuantDev& p, cudaStream_t s) {
-    const unsigned grid = unsigned(p.rows);
-    if (p.dim <= 1024) quant_rows_kernel<kDtype, kWDtype, kNorm, 128, 8><<<grid, 128, 0, s>>>(p);
-    else if (p.dim <= 8192) quant_rows_kernel<kDtype, kWDtype, kNorm, 512, 16><<<grid, 512, 0, s>>>(p);
-    else quant_rows_kernel<kDtype, kWDtype, kNorm, 1024, 32><<<grid, 1024, 0, s>>>(p);
+cudaError_t launch_quant_t(const QuantDev& p, int sms, cudaStream_t s) {
+    constexpr int kPer = kDtype == LOOM_SELECT_BF16 ? 8 : 4;
+    const bool aligned = p.dim % kPer == 0 && p.x_stride % kPer == 0 && p.residual_stride % kPer == 0 &&
+                         p.sum_stride % kPer == 0 && multiple_of(p.x, 16) && multiple_of(p.residual, 16) &&
+                         multiple_of(p.sum, 16) && multiple_of(p.weight, 16) && multiple_of(p.q, kPer);
+    if (aligned) launch_any<kDtype, kWDtype, kNorm, true>(p, sms, s);
+    else launch_any<kDtype, kWDtype, kNorm, false>(p, sms, s);
     return cudaGetLastError();
 }
 
@@ -181,14 +454,17 @@ LOOM_SELECT_API int loom_rms_norm_i8(const void* x, int dtype, int64_t rows, int
     p.sum_stride = sum_stride;
     p.dim = int32_t(dim);
     p.eps = eps;
+    int st = LOOM_SELECT_OK;
+    const int sms = device_sm_count(&st);
+    if (st != LOOM_SELECT_OK) return st;
     const auto s = static_cast<cudaStream_t>(stream);
     cudaError_t e;
     if (dtype == LOOM_SELECT_BF16)
-        e = weight_dtype == LOOM_SELECT_BF16 ? launch_quant_t<LOOM_SELECT_BF16, LOOM_SELECT_BF16, true>(p, s)
-                                             : launch_quant_t<LOOM_SELECT_BF16, LOOM_SELECT_F32, true>(p, s);
+        e = weight_dtype == LOOM_SELECT_BF16 ? launch_quant_t<LOOM_SELECT_BF16, LOOM_SELECT_BF16, true>(p, sms, s)
+                                             : launch_quant_t<LOOM_SELECT_BF16, LOOM_SELECT_F32, true>(p, sms, s);
     else
-        e = weight_dtype == LOOM_SELECT_BF16 ? launch_quant_t<LOOM_SELECT_F32, LOOM_SELECT_BF16, true>(p, s)
-                                             : launch_quant_t<LOOM_SELECT_F32, LOOM_SELECT_F32, true>(p, s);
+        e = weight_dtype == LOOM_SELECT_BF16 ? launch_quant_t<LOOM_SELECT_F32, LOOM_SELECT_BF16, true>(p, sms, s)
+                                             : launch_quant_t<LOOM_SELECT_F32, LOOM_SELECT_F32, true>(p, sms, s);
     return e == cudaSuccess ? LOOM_SELECT_OK : LOOM_SELECT_ECUDA;
 }
 
@@ -205,9 +481,12 @@ LOOM_SELECT_API int loom_quantize_rows_i8(const void* x, int dtype, int64_t rows
     p.rows = rows;
     p.x_stride = x_stride;
     p.dim = int32_t(dim);
+    int st = LOOM_SELECT_OK;
+    const int sms = device_sm_count(&st);
+    if (st != LOOM_SELECT_OK) return st;
     const auto s = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = dtype == LOOM_SELECT_BF16 ? launch_quant_t<LOOM_SELECT_BF16, LOOM_SELECT_F32, false>(p, s)
-                                                    : launch_quant_t<LOOM_SELECT_F32, LOOM_SELECT_F32, false>(p, s);
+    const cudaError_t e = dtype == LOOM_SELECT_BF16 ? launch_quant_t<LOOM_SELECT_BF16, LOOM_SELECT_F32, false>(p, sms, s)
+                                                    : launch_quant_t<LOOM_SELECT_F32, LOOM_SELECT_F32, false>(p, sms, s);
     return e == cudaSuccess ? LOOM_SELECT_OK : LOOM_SELECT_ECUDA;
 }
 
