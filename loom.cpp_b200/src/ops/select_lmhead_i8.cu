@@ -4,12 +4,17 @@
 //
 // with int8 operands, a scale per hidden row (token) and per weight row (vocabulary id). The integer sum is
 // exact (32 bits: 128 * 128 * 65536 < 2^31), so a logit has three f32 roundings whatever the order of the
-// sum, and a fourth where bf16 logits are asked for. Same plan as the bf16 head (select_lmhead.cu): one persistent
-// CTA per SM walks 128-row x BN-id tiles, row tile fastest; warp 0 streams 128-byte K slices of both tiles into a
-// shared-memory ring with TMA (128-byte swizzle, a K tail filled with zeros), warp 1 issues tcgen05.mma kind::i8
-// (M 128, N BN, K 32) into one of two TMEM accumulators, warps 2-5 drain the other one, scale it and write
-// the logits. A warp's 32 x 32 block goes through shared memory so that each store instruction covers 32
-// neighbouring ids of one row, whatever the alignment of the output rows.
+// sum, and a fourth where bf16 logits are asked for.
+//
+// The weight is the MMA's A operand, 128 ids to a tile, and the hidden rows its B operand, NR rows to a tile: an
+// accumulator lane is an id and its columns are rows, so that a warp's store of one column covers 32 neighbouring ids of
+// one row whatever the alignment of the output, and a call of few rows has a narrow MMA and few columns to drain. One
+// persistent CTA per SM. Warp 0 streams 128-byte K slices of both tiles into a shared-memory ring with TMA (128-byte
+// swizzle, a K tail filled with zeros), warp 1 issues tcgen05.mma kind::i8 (M 128, N NR, K 32) into one of two TMEM
+// accumulators, warps 2-5 drain the other one, scale it and write the logits.
+// With one tile of rows, each CTA takes an equal share of the ids, to 16 (a TMA box): 151936 ids are 1187.0 tiles, whose
+// whole ones would leave 3 of 148 SMs a ninth. With several, CTAs take whole tiles, rows fastest, so that those running
+// together share a weight tile through L2.
 // Bound: few rows, HBM (the weight, read once); many rows, the tensor cores and the logits' write.
 //
 // Waits are bounded and wind down as in select_lmhead.cu.
@@ -25,43 +30,76 @@
 namespace loom_select {
 namespace {
 
-constexpr int kBM = 128;       // rows per tile (MMA M)
+constexpr int kIds = 128;      // ids per tile (MMA M)
 constexpr int kBK = 128;       // K slice per stage: 128 int8, one swizzle span
 constexpr int kUK = 32;        // K per tcgen05.mma (kind::i8)
 constexpr int kThreads = 192;  // warp 0 TMA, warp 1 MMA + TMEM owner, warps 2-5 epilogue
-constexpr uint32_t kTmemCols = 512;
-constexpr int kAccStride = 256;
 constexpr int kMaxHidden = 65536;
-constexpr int kBufStride = 33;  // floats between rows of a warp's transposing block: no bank conflicts
-constexpr uint32_t kEpiBytes = 4 * 32 * kBufStride * 4;
+constexpr int kUnit = 16;      // ids per TMA box where CTAs share the ids out
 
-// kFewRows (calls of at most 16 rows): a 16-row hidden tile, as in select_lmhead.cu: the MMA reads 128
-// rows of A, and the TMEM lanes of the rows that do not exist are never read.
-template <int BN, bool kFewRows>
+// NR: hidden rows per tile (MMA N).
+template <int NR>
 struct I8Tile {
-    static constexpr int kARows = kFewRows ? 16 : kBM;
-    static constexpr uint32_t kTileABytes = uint32_t(kARows) * kBK;
-    static constexpr uint32_t kTileBBytes = uint32_t(BN) * kBK;
+    static_assert(NR % 16 == 0 && NR <= 256, "an MMA N for M = 128");
+    static constexpr uint32_t kTileABytes = uint32_t(kIds) * kBK;
+    static constexpr uint32_t kTileBBytes = uint32_t(NR) * kBK;
     static constexpr uint32_t kStageBytes = kTileABytes + kTileBBytes;
     static_assert(kStageBytes % 1024 == 0, "stage alignment");
-    static constexpr int kFit = int((227u * 1024u - 2048u - kEpiBytes) / kStageBytes);
-    static constexpr int kStages = kFit < 8 ? kFit : 8;
-    static_assert(kStages >= 2 && kStageBytes >= kBM * kBK, "the MMA's 128-row A read stays inside its stage");
-    static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kEpiBytes + 256 + 1024;
+    static constexpr uint32_t kScaleBytes = 4 * NR * 4;  // a copy of the tile's row scales for each epilogue warp
+    static constexpr int kFit = int((227u * 1024u - 2048u - kScaleBytes) / kStageBytes);
+    static constexpr int kStages = kFit < 12 ? kFit : 12;
+    static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kScaleBytes + 512 + 1024;
+    static constexpr uint32_t kTmemCols = 2 * NR < 32 ? 32 : 2 * NR;  // two accumulators
     // Instruction descriptor, kind::i8: s32 accumulator (2), signed A and B (1), K-major, N >> 3, M >> 4.
     static constexpr uint32_t kIdesc =
-        (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(BN >> 3) << 17) | (uint32_t(kBM >> 4) << 24);
+        (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(NR >> 3) << 17) | (uint32_t(kIds >> 4) << 24);
 };
 
 struct I8Args {
     int64_t rows, n_vocab;
     int k_blocks;
-    int m_tiles, v_tiles;
+    int r_tiles;       // tiles along the rows
+    int64_t v_tiles;   // tiles along the ids (r_tiles > 1)
+    int64_t units;     // ids / kUnit, rounded up (r_tiles == 1)
     const float* row_scale;
     const float* col_scale;
     void* out;
     int64_t out_stride;
     int* status;
+};
+
+// The tiles of one CTA, in order: ids [id, id_end), rows from `row` on.
+struct I8Walk {
+    int64_t id, id_end;
+    int64_t row;
+    int64_t next, end;  // one tile of rows: units of ids; several: tiles
+    __device__ __forceinline__ explicit I8Walk(const I8Args& a) {
+        if (a.r_tiles == 1) {
+            next = a.units * blockIdx.x / gridDim.x;
+            end = a.units * (blockIdx.x + 1) / gridDim.x;
+        } else {
+            next = blockIdx.x;
+            end = a.v_tiles * a.r_tiles;
+        }
+    }
+    template <int NR>
+    __device__ __forceinline__ bool step(const I8Args& a) {
+        if (next >= end) return false;
+        int64_t past;
+        if (a.r_tiles == 1) {
+            id = next * kUnit;
+            next = next + kIds / kUnit < end ? next + kIds / kUnit : end;
+            past = next * kUnit;
+            row = 0;
+        } else {
+            id = next / a.r_tiles * kIds;
+            past = id + kIds;
+            row = next % a.r_tiles * NR;
+            next += gridDim.x;
+        }
+        id_end = past < a.n_vocab ? past : a.n_vocab;
+        return true;
+    }
 };
 
 template <int kOut>
@@ -70,42 +108,48 @@ __device__ __forceinline__ void store_logit(void* out, int64_t i, float v) {
     else reinterpret_cast<float*>(out)[i] = v;
 }
 
-// W accumulator columns of the warp's 32 rows, scaled and written: col is the first one's id, n of them
-// exist; row0 is lane 0's row, n_rows of the warp's rows exist.
+// W rows of one id: accumulator bits, the rows' scales (shared memory, 16-byte aligned) and the id's scale; n rows
+// exist, at is the first one's place in the output.
 template <int kOut, int W>
-__device__ __forceinline__ void write_block(const I8Args& a, float* buf, const float (&acc)[W], float row_scale,
-                                            int64_t row0, int n_rows, int64_t col, int n) {
-    const int lane = threadIdx.x & 31;
+__device__ __forceinline__ void write_rows(const I8Args& a, const float (&acc)[W], const float* scale, float col_scale,
+                                           int64_t at, int n, bool there) {
+    float v[W];
 #pragma unroll
-    for (int j = 0; j < W; ++j) buf[lane * kBufStride + j] = __fmul_rn(__int2float_rn(__float_as_int(acc[j])), row_scale);
-    __syncwarp();
-    if (lane < n && lane < W) {
-        const float cs = __ldg(a.col_scale + col + lane);
-        int64_t at = row0 * a.out_stride + col + lane;
-        for (int r = 0; r < n_rows; ++r, at += a.out_stride)
-            store_logit<kOut>(a.out, at, __fmul_rn(buf[r * kBufStride + lane], cs));
+    for (int j = 0; j < W; j += 4) {
+        const float4 s = *reinterpret_cast<const float4*>(scale + j);
+        v[j] = __fmul_rn(__fmul_rn(__int2float_rn(__float_as_int(acc[j])), s.x), col_scale);
+        v[j + 1] = __fmul_rn(__fmul_rn(__int2float_rn(__float_as_int(acc[j + 1])), s.y), col_scale);
+        v[j + 2] = __fmul_rn(__fmul_rn(__int2float_rn(__float_as_int(acc[j + 2])), s.z), col_scale);
+        v[j + 3] = __fmul_rn(__fmul_rn(__int2float_rn(__float_as_int(acc[j + 3])), s.w), col_scale);
     }
-    __syncwarp();
+    if (!there) return;
+    if (n >= W) {
+#pragma unroll
+        for (int j = 0; j < W; ++j, at += a.out_stride) store_logit<kOut>(a.out, at, v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < W; ++j, at += a.out_stride)
+            if (j < n) store_logit<kOut>(a.out, at, v[j]);
+    }
 }
 
-template <int BN, bool kFewRows, int kOut>
+template <int NR, int kOut>
 __global__ void __launch_bounds__(kThreads, 1)
     lm_head_logits_i8_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w,
-                             const I8Args a) {
+                             const __grid_constant__ CUtensorMap map_unit, const I8Args a) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    using T = I8Tile<BN, kFewRows>;
-    constexpr uint32_t kTileABytes = T::kTileABytes;
+    using T = I8Tile<NR>;
     constexpr int kStages = T::kStages;
     constexpr uint32_t kStageBytes = T::kStageBytes;
-    float* epi = reinterpret_cast<float*>(smem + size_t(kStages) * kStageBytes);
-    LmBars<kStages>* bars = reinterpret_cast<LmBars<kStages>*>(smem + size_t(kStages) * kStageBytes + kEpiBytes);
+    float* scales = reinterpret_cast<float*>(smem + size_t(kStages) * kStageBytes);
+    LmBars<kStages>* bars = reinterpret_cast<LmBars<kStages>*>(smem + size_t(kStages) * kStageBytes + T::kScaleBytes);
+    static_assert(sizeof(LmBars<kStages>) <= 512, "barriers");
     volatile int* abort_flag = &bars->abort;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const WaitFault wf = read_wait_fault(a.status);  // the workspace header's test hook: zero for normal callers
     const uint64_t lim = wf.limit_ns;
-    const int n_tiles = a.m_tiles * a.v_tiles;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -122,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&bars->tmem_base)),
-                     "r"(kTmemCols)
+                     "r"(T::kTmemCols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -130,6 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = bars->tmem_base;
+    I8Walk walk(a);
 
     if (warp == 0) {
         if (lane == 0) {
@@ -137,8 +182,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             int64_t kc = 0;
             const int64_t withheld = (blockIdx.x == 0 && wf.withhold > 0) ? int64_t(wf.withhold) - 1 : -1;
             bool ok = true;
-            for (int t = blockIdx.x; t < n_tiles && ok; t += gridDim.x) {
-                const int mt = t % a.m_tiles, vt = t / a.m_tiles;
+            while (ok && walk.step<NR>(a)) {
+                // one box for a whole tile (sixteen 2 KiB boxes for each: 96 us for one row, where this takes 61),
+                // small ones for what is left of a CTA's share
+                const int left = int((walk.id_end - walk.id + kUnit - 1) / kUnit);
+                const bool cut = a.r_tiles == 1 && left < kIds / kUnit;
+                const uint32_t bytes = T::kTileBBytes + (cut ? uint32_t(left) * kUnit * kBK : T::kTileABytes);
                 for (int kb = 0; kb < a.k_blocks; ++kb, ++kc) {
                     const int s = int(kc % kStages);
                     const int64_t n = kc / kStages;
@@ -148,9 +197,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     if (kc == withheld) continue;  // test hook only: this slice never arrives
                     unsigned char* st = smem + size_t(s) * kStageBytes;
-                    mbar_arrive_expect_tx(&bars->full[s], kStageBytes);
-                    tma_load_2d(st, &map_h, kb * kBK, mt * kBM, &bars->full[s]);
-                    tma_load_2d(st + kTileABytes, &map_w, kb * kBK, vt * BN, &bars->full[s]);
+                    mbar_arrive_expect_tx(&bars->full[s], bytes);
+                    if (!cut) tma_load_2d(st, &map_w, kb * kBK, int(walk.id), &bars->full[s]);
+                    else
+                        for (int u = 0; u < left; ++u)
+                            tma_load_2d(st + u * kUnit * kBK, &map_unit, kb * kBK, int(walk.id) + u * kUnit, &bars->full[s]);
+                    tma_load_2d(st + T::kTileABytes, &map_h, kb * kBK, int(walk.row), &bars->full[s]);
                 }
             }
             // every copy issued lands before the CTA may exit (a withheld slice was never issued)
@@ -169,11 +221,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             int64_t kc = 0;
             int i = 0;
             bool ok = true;
-            for (int t = blockIdx.x; t < n_tiles && ok; t += gridDim.x, ++i) {
+            for (; ok && walk.step<NR>(a); ++i) {
                 const int b = i & 1, u = i >> 1;
                 if (u >= 1 && !lm_wait(&bars->tempty[b], uint32_t((u - 1) & 1), a.status, abort_flag, lim)) break;
                 tc_fence_after();
-                const uint32_t d_tmem = tmem_base + uint32_t(b * kAccStride);
+                const uint32_t d_tmem = tmem_base + uint32_t(b * NR);
                 for (int kb = 0; kb < a.k_blocks; ++kb, ++kc) {
                     const int s = int(kc % kStages);
                     const int64_t n = kc / kStages;
@@ -183,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     tc_fence_after();
                     const uint32_t sa = smem_addr(smem + size_t(s) * kStageBytes);
-                    const uint32_t sb = sa + kTileABytes;
+                    const uint32_t sb = sa + T::kTileABytes;
 #pragma unroll
                     for (int kk = 0; kk < kBK / kUK; ++kk) {
                         tc_mma_i8(d_tmem, smem_desc_sw128(sa + kk * kUK), smem_desc_sw128(sb + kk * kUK), T::kIdesc,
@@ -199,34 +251,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
     } else {
-        // ---- epilogue: warps 2-5 read TMEM lanes 32 * (warp % 4) .. + 31, one row per thread ----
+        // ---- epilogue: warps 2-5 read TMEM lanes 32 * (warp % 4) .. + 31, one id per thread ----
         const int q = warp & 3;
-        float* buf = epi + q * 32 * kBufStride;
-        int i = 0;
-        for (int t = blockIdx.x; t < n_tiles; t += gridDim.x, ++i) {
-            const int mt = t % a.m_tiles, vt = t / a.m_tiles;
+        float* scale = scales + q * NR;
+        int64_t scale_row = -1;  // the first row whose scales are in `scale`
+        for (int i = 0; walk.step<NR>(a); ++i) {
             const int b = i & 1, u = i >> 1;
-            const int64_t row0 = int64_t(mt) * kBM + q * 32;
-            const int n_rows = a.rows - row0 < 32 ? (a.rows > row0 ? int(a.rows - row0) : 0) : 32;
-            const float row_scale = lane < n_rows ? __ldg(a.row_scale + row0 + lane) : 0.0f;
+            if (walk.row != scale_row) {
+                scale_row = walk.row;
+                __syncwarp();
+                for (int j = lane; j < NR; j += 32)
+                    scale[j] = scale_row + j < a.rows ? __ldg(a.row_scale + scale_row + j) : 0.0f;
+                __syncwarp();
+            }
+            const int64_t id = walk.id + q * 32 + lane;
+            const bool there = id < walk.id_end;
+            const float col_scale = there ? __ldg(a.col_scale + id) : 0.0f;
+            const int n_rows = a.rows - walk.row < NR ? int(a.rows - walk.row) : NR;
             const bool ok = lm_wait(&bars->tfull[b], uint32_t(u & 1), a.status, abort_flag, lim);
             if (!__all_sync(0xffffffffu, ok)) break;
             tc_fence_after();
-            if (n_rows > 0) {
-                const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(b * kAccStride);
-                const int64_t col0 = int64_t(vt) * BN;
-                const int valid = a.n_vocab - col0 < BN ? int(a.n_vocab - col0) : BN;
-                constexpr int kFull = BN / 32 * 32;
+            const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(b * NR);
+            if (__any_sync(0xffffffffu, there)) {
+                int64_t at = walk.row * a.out_stride + id;
+                if constexpr (NR < 32) {
+                    float v[16];
+                    tc_ld16(taddr, v);
+                    write_rows<kOut, 16>(a, v, scale, col_scale, at, n_rows, there);
+                } else {
 #pragma unroll 1
-                for (int c = 0; c < kFull; c += 32) {
-                    float v[32];
-                    tc_ld32(taddr + uint32_t(c), v);
-                    write_block<kOut, 32>(a, buf, v, row_scale, row0, n_rows, col0 + c, valid - c);
-                }
-                if constexpr (BN % 32 != 0) {
-                    float w[16];
-                    tc_ld16(taddr + uint32_t(kFull), w);
-                    write_block<kOut, 16>(a, buf, w, row_scale, row0, n_rows, col0 + kFull, valid - kFull);
+                    for (int c = 0; c < NR && c < n_rows; c += 32, at += 32 * a.out_stride) {
+                        float v[32];
+                        tc_ld32(taddr + uint32_t(c), v);
+                        write_rows<kOut, 32>(a, v, scale + c, col_scale, at, n_rows - c, there);
+                    }
                 }
             }
             tc_fence_before();
@@ -239,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     if (warp == 1) {
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(T::kTmemCols) : "memory");
     }
 }
 
@@ -255,50 +313,39 @@ bool make_map_i8(CUtensorMap* m, const void* base, uint64_t inner, uint64_t oute
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Tile widths, chosen as in the bf16 head: 208 ids where that spreads the tiles over the SMs clearly more
-// evenly (151936 ids on one row tile: 594 tiles of 256 leave two SMs a fifth tile).
-constexpr int kWideBN = 256, kNarrowBN = 208;
-
-int pick_bn(int64_t m_tiles, int64_t n_vocab, int sms) {
-    auto cost = [&](int bn) {
-        const int64_t tiles = m_tiles * ((n_vocab + bn - 1) / bn);
-        return double((tiles + sms - 1) / sms) * bn;
-    };
-    return cost(kNarrowBN) < 0.97 * cost(kWideBN) ? kNarrowBN : kWideBN;
-}
-
-template <int BN, bool kFewRows, int kOut>
+template <int NR, int kOut>
 int launch_i8(const void* hidden, const void* weight, I8Args a, int64_t hidden_dim, int sms, cudaStream_t stream) {
-    using T = I8Tile<BN, kFewRows>;
-    a.v_tiles = int((a.n_vocab + BN - 1) / BN);
-    CUtensorMap map_h, map_w;
-    if (!make_map_i8(&map_h, hidden, uint64_t(hidden_dim), uint64_t(a.rows), uint32_t(T::kARows)) ||
-        !make_map_i8(&map_w, weight, uint64_t(hidden_dim), uint64_t(a.n_vocab), BN))
+    using T = I8Tile<NR>;
+    a.r_tiles = int((a.rows + NR - 1) / NR);
+    a.v_tiles = (a.n_vocab + kIds - 1) / kIds;
+    a.units = (a.n_vocab + kUnit - 1) / kUnit;
+    const int64_t work = a.r_tiles == 1 ? a.units : a.v_tiles * a.r_tiles;
+    CUtensorMap map_h, map_w, map_unit;
+    if (!make_map_i8(&map_h, hidden, uint64_t(hidden_dim), uint64_t(a.rows), NR) ||
+        !make_map_i8(&map_w, weight, uint64_t(hidden_dim), uint64_t(a.n_vocab), kIds) ||
+        !make_map_i8(&map_unit, weight, uint64_t(hidden_dim), uint64_t(a.n_vocab), kUnit))
         return LOOM_SELECT_ECUDA;
     static std::atomic<bool> configured[64] = {};  // set once per device, from any host thread
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return LOOM_SELECT_ECUDA;
     if (!configured[dev]) {
-        if (cudaFuncSetAttribute(lm_head_logits_i8_kernel<BN, kFewRows, kOut>,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize, int(T::kSmemBytes)) != cudaSuccess)
+        if (cudaFuncSetAttribute(lm_head_logits_i8_kernel<NR, kOut>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 int(T::kSmemBytes)) != cudaSuccess)
             return LOOM_SELECT_ECUDA;
         configured[dev] = true;
     }
-    const int64_t tiles = int64_t(a.m_tiles) * a.v_tiles;
-    const int grid = int(tiles < sms ? tiles : sms);
-    lm_head_logits_i8_kernel<BN, kFewRows, kOut><<<grid, kThreads, T::kSmemBytes, stream>>>(map_h, map_w, a);
+    const int grid = int(work < sms ? work : sms);
+    lm_head_logits_i8_kernel<NR, kOut><<<grid, kThreads, T::kSmemBytes, stream>>>(map_h, map_w, map_unit, a);
     return cudaGetLastError() == cudaSuccess ? LOOM_SELECT_OK : LOOM_SELECT_ECUDA;
 }
 
 template <int kOut>
 int launch_i8_any(const void* hidden, const void* weight, const I8Args& a, int64_t hidden_dim, int sms,
                   cudaStream_t stream) {
-    const bool few = a.rows <= 16;
-    if (pick_bn(a.m_tiles, a.n_vocab, sms) == kNarrowBN)
-        return few ? launch_i8<kNarrowBN, true, kOut>(hidden, weight, a, hidden_dim, sms, stream)
-                   : launch_i8<kNarrowBN, false, kOut>(hidden, weight, a, hidden_dim, sms, stream);
-    return few ? launch_i8<kWideBN, true, kOut>(hidden, weight, a, hidden_dim, sms, stream)
-               : launch_i8<kWideBN, false, kOut>(hidden, weight, a, hidden_dim, sms, stream);
+    if (a.rows <= 16) return launch_i8<16, kOut>(hidden, weight, a, hidden_dim, sms, stream);
+    if (a.rows <= 64) return launch_i8<64, kOut>(hidden, weight, a, hidden_dim, sms, stream);
+    if (a.rows <= 128) return launch_i8<128, kOut>(hidden, weight, a, hidden_dim, sms, stream);
+    return launch_i8<256, kOut>(hidden, weight, a, hidden_dim, sms, stream);
 }
 
 }  // namespace
@@ -327,19 +374,16 @@ LOOM_SELECT_API int loom_lm_head_logits_i8(const int8_t* hidden, const float* hi
         reinterpret_cast<uintptr_t>(hidden_scale) % 4 != 0 || reinterpret_cast<uintptr_t>(weight_scale) % 4 != 0 ||
         reinterpret_cast<uintptr_t>(out_logits) % osz != 0)
         return LOOM_SELECT_EINVAL;
-    const int64_t mt = (rows + kBM - 1) / kBM;
-    if (mt * ((n_vocab + kNarrowBN - 1) / kNarrowBN) > INT32_MAX) return LOOM_SELECT_ESHAPE;
+    if ((rows + 255) / 256 * ((n_vocab + kIds - 1) / kIds) > INT32_MAX) return LOOM_SELECT_ESHAPE;
     if (!workspace || workspace_bytes < kWsAlign || reinterpret_cast<uintptr_t>(workspace) % kWsAlign != 0)
         return LOOM_SELECT_EWORKSPACE;
     int st = LOOM_SELECT_OK;
     const int sms = device_sm_count(&st);
     if (st != LOOM_SELECT_OK) return st;
-    I8Args a;
+    I8Args a{};
     a.rows = rows;
     a.n_vocab = n_vocab;
     a.k_blocks = int((hidden_dim + kBK - 1) / kBK);
-    a.m_tiles = int(mt);
-    a.v_tiles = 0;
     a.row_scale = hidden_scale;
     a.col_scale = weight_scale;
     a.out = out_logits;
