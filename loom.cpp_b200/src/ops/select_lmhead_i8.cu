@@ -6,18 +6,22 @@
 // exact (32 bits: 128 * 128 * 65536 < 2^31), so a logit has three f32 roundings whatever the order of the
 // sum, and a fourth where bf16 logits are asked for.
 //
-// The weight is the MMA's A operand, 128 ids to a tile, and the hidden rows its B operand, NR rows to a tile: an
+// The weight is the MMA's A operand, 128 ids to a CTA's tile, and the hidden rows its B operand, NR rows to a tile: an
 // accumulator lane is an id and its columns are rows, so that a warp's store of one column covers 32 neighbouring ids of
 // one row whatever the alignment of the output, and a call of few rows has a narrow MMA and few columns to drain. One
 // persistent CTA per SM. Warp 0 streams 128-byte K slices of both tiles into a shared-memory ring with TMA (128-byte
 // swizzle, a K tail filled with zeros), warp 1 issues tcgen05.mma kind::i8 (M 128, N NR, K 32) into one of two TMEM
-// accumulators, warps 2-5 drain the other one, scale it and write the logits.
-// With one tile of rows, each CTA takes an equal share of the ids, to 16 (a TMA box): 151936 ids are 1187.0 tiles, whose
-// whole ones would leave 3 of 148 SMs a ninth. With several, CTAs take whole tiles, rows fastest, so that those running
-// together share a weight tile through L2.
+// accumulators, the other warps drain the other one, scale it and write the logits.
+// Calls of more than 128 rows work in pairs of CTAs (cta_group::2, M 256, N 256): each loads its own ids and half of the
+// rows, so a stage brings 32 KiB into an SM for the work that a CTA by itself would fetch 48 KiB for -- at 64 bytes a
+// cycle from L2 that fetch, 768 cycles, and not the MMA's 512, is what bound it.
+// With one tile of rows, each CTA (or pair) takes an equal share of the ids, to 16 (a TMA box): 151936 ids are 1187.0
+// tiles, whose whole ones would leave 3 of 148 SMs a ninth. With several, they take whole tiles, rows fastest, so that
+// those running together share a weight tile through L2.
 // Bound: few rows, HBM (the weight, read once); many rows, the tensor cores and the logits' write.
 //
-// Waits are bounded and wind down as in select_lmhead.cu.
+// Waits are bounded and wind down as in select_lmhead.cu; a CTA of a pair whose wait runs out leaves the other's to run
+// out by themselves, and both meet at the cluster barrier before TMEM is freed.
 #include <atomic>
 #include <cstdint>
 #include <cuda_runtime.h>
@@ -33,26 +37,44 @@ namespace {
 constexpr int kIds = 128;      // ids per tile (MMA M)
 constexpr int kBK = 128;       // K slice per stage: 128 int8, one swizzle span
 constexpr int kUK = 32;        // K per tcgen05.mma (kind::i8)
-constexpr int kThreads = 192;  // warp 0 TMA, warp 1 MMA + TMEM owner, warps 2-5 epilogue
 constexpr int kMaxHidden = 65536;
 constexpr int kUnit = 16;      // ids per TMA box where CTAs share the ids out
 
-// NR: hidden rows per tile (MMA N).
-template <int NR>
+// NR: hidden rows per tile (MMA N). kPair: two CTAs to a tile.
+template <int NR, bool kPair>
 struct I8Tile {
-    static_assert(NR % 16 == 0 && NR <= 256, "an MMA N for M = 128");
+    static_assert(NR % 16 == 0 && NR <= 256, "an MMA N for M = 128 or 256");
+    static constexpr int kCtas = kPair ? 2 : 1;
+    static constexpr int kBRows = NR / kCtas;  // rows a CTA loads
     static constexpr uint32_t kTileABytes = uint32_t(kIds) * kBK;
-    static constexpr uint32_t kTileBBytes = uint32_t(NR) * kBK;
+    static constexpr uint32_t kTileBBytes = uint32_t(kBRows) * kBK;
     static constexpr uint32_t kStageBytes = kTileABytes + kTileBBytes;
     static_assert(kStageBytes % 1024 == 0, "stage alignment");
-    static constexpr uint32_t kScaleBytes = 4 * NR * 4;  // a copy of the tile's row scales for each epilogue warp
+    // Warp 0 TMA, warp 1 MMA and TMEM, then the epilogue: four warps cover the accumulator's lanes, eight its columns by
+    // halves too (four drain a 256-row tile too slowly: 256 us for [1024, 2048] x [151936, 2048], bf16 logits).
+    static constexpr int kEpiWarps = NR >= 64 ? 8 : 4;
+    static constexpr int kThreads = 64 + 32 * kEpiWarps;
+    static constexpr int kEpiCols = NR / (kEpiWarps / 4);  // rows a warp drains of a tile
+    static constexpr uint32_t kScaleBytes = kEpiWarps * kEpiCols * 4;  // their scales, a copy for each warp
     static constexpr int kFit = int((227u * 1024u - 2048u - kScaleBytes) / kStageBytes);
     static constexpr int kStages = kFit < 12 ? kFit : 12;
     static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kScaleBytes + 512 + 1024;
     static constexpr uint32_t kTmemCols = 2 * NR < 32 ? 32 : 2 * NR;  // two accumulators
     // Instruction descriptor, kind::i8: s32 accumulator (2), signed A and B (1), K-major, N >> 3, M >> 4.
     static constexpr uint32_t kIdesc =
-        (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(NR >> 3) << 17) | (uint32_t(kIds >> 4) << 24);
+        (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(NR >> 3) << 17) | (uint32_t(kCtas * kIds >> 4) << 24);
+};
+
+template <int kStages>
+struct I8Bars {
+    uint64_t full[kStages];       // this CTA's TMA -> the MMA (or, in a pair's odd CTA, the warp that passes it on)
+    uint64_t peer_full[kStages];  // pair, even CTA: the odd one's slice is there
+    uint64_t empty[kStages];      // MMA -> TMA, in both CTAs of a pair
+    uint64_t tfull[2];            // MMA -> epilogue, in both
+    uint64_t tempty[2];           // epilogue warps (of both) -> MMA
+    uint64_t drain;               // the MMA warp's final commit
+    uint32_t tmem_base;
+    int abort;
 };
 
 struct I8Args {
@@ -68,35 +90,40 @@ struct I8Args {
     int* status;
 };
 
-// The tiles of one CTA, in order: ids [id, id_end), rows from `row` on.
+// The tiles of one CTA (or pair), in order: this CTA's ids [id, id_end), perhaps none, and rows from `row` on.
+template <int NR, bool kPair>
 struct I8Walk {
+    static constexpr int kCtas = kPair ? 2 : 1;
     int64_t id, id_end;
     int64_t row;
     int64_t next, end;  // one tile of rows: units of ids; several: tiles
     __device__ __forceinline__ explicit I8Walk(const I8Args& a) {
+        const int64_t worker = blockIdx.x / kCtas, workers = gridDim.x / kCtas;
         if (a.r_tiles == 1) {
-            next = a.units * blockIdx.x / gridDim.x;
-            end = a.units * (blockIdx.x + 1) / gridDim.x;
+            next = a.units * worker / workers;
+            end = a.units * (worker + 1) / workers;
         } else {
-            next = blockIdx.x;
+            next = worker;
             end = a.v_tiles * a.r_tiles;
         }
     }
-    template <int NR>
     __device__ __forceinline__ bool step(const I8Args& a) {
         if (next >= end) return false;
         int64_t past;
         if (a.r_tiles == 1) {
+            constexpr int kUnits = kCtas * kIds / kUnit;
             id = next * kUnit;
-            next = next + kIds / kUnit < end ? next + kIds / kUnit : end;
+            next = next + kUnits < end ? next + kUnits : end;
             past = next * kUnit;
             row = 0;
         } else {
-            id = next / a.r_tiles * kIds;
-            past = id + kIds;
+            id = next / a.r_tiles * (kCtas * kIds);
+            past = id + kCtas * kIds;
             row = next % a.r_tiles * NR;
-            next += gridDim.x;
+            next += gridDim.x / kCtas;
         }
+        if (kPair && blockIdx.x % 2) id += kIds;
+        if (past > id + kIds) past = id + kIds;
         id_end = past < a.n_vocab ? past : a.n_vocab;
         return true;
     }
@@ -133,19 +160,20 @@ __device__ __forceinline__ void write_rows(const I8Args& a, const float (&acc)[W
     }
 }
 
-template <int NR, int kOut>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int NR, bool kPair, int kOut>
+__global__ void __launch_bounds__(I8Tile<NR, kPair>::kThreads, 1)
     lm_head_logits_i8_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w,
                              const __grid_constant__ CUtensorMap map_unit, const I8Args a) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    using T = I8Tile<NR>;
+    using T = I8Tile<NR, kPair>;
     constexpr int kStages = T::kStages;
     constexpr uint32_t kStageBytes = T::kStageBytes;
     float* scales = reinterpret_cast<float*>(smem + size_t(kStages) * kStageBytes);
-    LmBars<kStages>* bars = reinterpret_cast<LmBars<kStages>*>(smem + size_t(kStages) * kStageBytes + T::kScaleBytes);
-    static_assert(sizeof(LmBars<kStages>) <= 512, "barriers");
+    I8Bars<kStages>* bars = reinterpret_cast<I8Bars<kStages>*>(smem + size_t(kStages) * kStageBytes + T::kScaleBytes);
+    static_assert(sizeof(I8Bars<kStages>) <= 512, "barriers");
     volatile int* abort_flag = &bars->abort;
+    const uint32_t rank = kPair ? blockIdx.x % 2 : 0;  // (clusters are neighbouring blocks)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const WaitFault wf = read_wait_fault(a.status);  // the workspace header's test hook: zero for normal callers
@@ -154,27 +182,38 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&bars->full[s], 1);
+            mbar_init(&bars->peer_full[s], 1);
             mbar_init(&bars->empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&bars->tfull[b], 1);
-            mbar_init(&bars->tempty[b], 4);
+            mbar_init(&bars->tempty[b], T::kCtas * T::kEpiWarps);
         }
         mbar_init(&bars->drain, 1);
         bars->abort = 0;
         mbar_fence_init();
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&bars->tmem_base)),
-                     "r"(T::kTmemCols)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (kPair) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                             smem_addr(&bars->tmem_base)),
+                         "r"(T::kTmemCols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                             smem_addr(&bars->tmem_base)),
+                         "r"(T::kTmemCols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (kPair) cluster_sync_all();  // the other CTA's barriers are there too
     tc_fence_after();
     const uint32_t tmem_base = bars->tmem_base;
-    I8Walk walk(a);
+    I8Walk<NR, kPair> walk(a);
 
     if (warp == 0) {
         if (lane == 0) {
@@ -182,11 +221,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             int64_t kc = 0;
             const int64_t withheld = (blockIdx.x == 0 && wf.withhold > 0) ? int64_t(wf.withhold) - 1 : -1;
             bool ok = true;
-            while (ok && walk.step<NR>(a)) {
+            while (ok && walk.step(a)) {
                 // one box for a whole tile (sixteen 2 KiB boxes for each: 96 us for one row, where this takes 61),
                 // small ones for what is left of a CTA's share
-                const int left = int((walk.id_end - walk.id + kUnit - 1) / kUnit);
-                const bool cut = a.r_tiles == 1 && left < kIds / kUnit;
+                const int left = walk.id_end > walk.id ? int((walk.id_end - walk.id + kUnit - 1) / kUnit) : 0;
+                const bool cut = left == 0 || (a.r_tiles == 1 && left < kIds / kUnit);
                 const uint32_t bytes = T::kTileBBytes + (cut ? uint32_t(left) * kUnit * kBK : T::kTileABytes);
                 for (int kb = 0; kb < a.k_blocks; ++kb, ++kc) {
                     const int s = int(kc % kStages);
@@ -202,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     else
                         for (int u = 0; u < left; ++u)
                             tma_load_2d(st + u * kUnit * kBK, &map_unit, kb * kBK, int(walk.id) + u * kUnit, &bars->full[s]);
-                    tma_load_2d(st + T::kTileABytes, &map_h, kb * kBK, int(walk.row), &bars->full[s]);
+                    tma_load_2d(st + T::kTileABytes, &map_h, kb * kBK, int(walk.row) + int(rank) * T::kBRows, &bars->full[s]);
                 }
             }
             // every copy issued lands before the CTA may exit (a withheld slice was never issued)
@@ -216,12 +255,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (lane == 0 && rank != 0) {
+            // ---- a pair's odd CTA: passes on that its slices are there ----
+            int64_t kc = 0;
+            bool ok = true;
+            while (ok && walk.step(a)) {
+                for (int kb = 0; ok && kb < a.k_blocks; ++kb, ++kc) {
+                    const int s = int(kc % kStages);
+                    ok = lm_wait(&bars->full[s], uint32_t((kc / kStages) & 1), a.status, abort_flag, lim);
+                    if (ok) mbar_arrive_remote(&bars->peer_full[s], 0);
+                }
+            }
+        } else if (lane == 0) {
             // ---- MMA issuer ----
             int64_t kc = 0;
             int i = 0;
             bool ok = true;
-            for (; ok && walk.step<NR>(a); ++i) {
+            for (; ok && walk.step(a); ++i) {
                 const int b = i & 1, u = i >> 1;
                 if (u >= 1 && !lm_wait(&bars->tempty[b], uint32_t((u - 1) & 1), a.status, abort_flag, lim)) break;
                 tc_fence_after();
@@ -229,7 +279,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int kb = 0; kb < a.k_blocks; ++kb, ++kc) {
                     const int s = int(kc % kStages);
                     const int64_t n = kc / kStages;
-                    if (!lm_wait(&bars->full[s], uint32_t(n & 1), a.status, abort_flag, lim)) {
+                    if (!lm_wait(&bars->full[s], uint32_t(n & 1), a.status, abort_flag, lim) ||
+                        (kPair && !lm_wait(&bars->peer_full[s], uint32_t(n & 1), a.status, abort_flag, lim))) {
                         ok = false;
                         break;
                     }
@@ -238,49 +289,55 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t sb = sa + T::kTileABytes;
 #pragma unroll
                     for (int kk = 0; kk < kBK / kUK; ++kk) {
-                        tc_mma_i8(d_tmem, smem_desc_sw128(sa + kk * kUK), smem_desc_sw128(sb + kk * kUK), T::kIdesc,
-                                  (kb | kk) != 0 ? 1u : 0u);
+                        const uint64_t da = smem_desc_sw128(sa + kk * kUK), db = smem_desc_sw128(sb + kk * kUK);
+                        if constexpr (kPair) tc_mma_i8_pair(d_tmem, da, db, T::kIdesc, (kb | kk) != 0 ? 1u : 0u);
+                        else tc_mma_i8(d_tmem, da, db, T::kIdesc, (kb | kk) != 0 ? 1u : 0u);
                     }
-                    tc_commit(&bars->empty[s]);
+                    if constexpr (kPair) tc_commit_both(&bars->empty[s]);
+                    else tc_commit(&bars->empty[s]);
                 }
-                if (ok) tc_commit(&bars->tfull[b]);
+                if (ok) {
+                    if constexpr (kPair) tc_commit_both(&bars->tfull[b]);
+                    else tc_commit(&bars->tfull[b]);
+                }
             }
             // all MMAs issued have completed before TMEM is freed
-            tc_commit(&bars->drain);
+            if constexpr (kPair) tc_commit_pair_own(&bars->drain);
+            else tc_commit(&bars->drain);
             mbar_wait_bounded(&bars->drain, 0, a.status, lim);
         }
         __syncwarp();
     } else {
-        // ---- epilogue: warps 2-5 read TMEM lanes 32 * (warp % 4) .. + 31, one id per thread ----
-        const int q = warp & 3;
-        float* scale = scales + q * NR;
-        int64_t scale_row = -1;  // the first row whose scales are in `scale`
-        for (int i = 0; walk.step<NR>(a); ++i) {
+        // ---- epilogue: a warp reads TMEM lanes 32 * (warp % 4) .. + 31, one id per thread ----
+        const int q = warp & 3, col0 = (warp - 2) / 4 * T::kEpiCols;
+        float* scale = scales + (warp - 2) * T::kEpiCols;
+        int64_t scale_row = -1;  // the tile whose scales are in `scale`
+        for (int i = 0; walk.step(a); ++i) {
             const int b = i & 1, u = i >> 1;
+            const int64_t row = walk.row + col0;  // this warp's first
             if (walk.row != scale_row) {
                 scale_row = walk.row;
                 __syncwarp();
-                for (int j = lane; j < NR; j += 32)
-                    scale[j] = scale_row + j < a.rows ? __ldg(a.row_scale + scale_row + j) : 0.0f;
+                for (int j = lane; j < T::kEpiCols; j += 32) scale[j] = row + j < a.rows ? __ldg(a.row_scale + row + j) : 0.0f;
                 __syncwarp();
             }
             const int64_t id = walk.id + q * 32 + lane;
             const bool there = id < walk.id_end;
             const float col_scale = there ? __ldg(a.col_scale + id) : 0.0f;
-            const int n_rows = a.rows - walk.row < NR ? int(a.rows - walk.row) : NR;
+            const int n_rows = a.rows - row < T::kEpiCols ? int(a.rows - row) : T::kEpiCols;  // (none: not positive)
             const bool ok = lm_wait(&bars->tfull[b], uint32_t(u & 1), a.status, abort_flag, lim);
             if (!__all_sync(0xffffffffu, ok)) break;
             tc_fence_after();
-            const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(b * NR);
+            const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(b * NR + col0);
             if (__any_sync(0xffffffffu, there)) {
-                int64_t at = walk.row * a.out_stride + id;
+                int64_t at = row * a.out_stride + id;
                 if constexpr (NR < 32) {
                     float v[16];
                     tc_ld16(taddr, v);
                     write_rows<kOut, 16>(a, v, scale, col_scale, at, n_rows, there);
                 } else {
 #pragma unroll 1
-                    for (int c = 0; c < NR && c < n_rows; c += 32, at += 32 * a.out_stride) {
+                    for (int c = 0; c < T::kEpiCols && c < n_rows; c += 32, at += 32 * a.out_stride) {
                         float v[32];
                         tc_ld32(taddr + uint32_t(c), v);
                         write_rows<kOut, 32>(a, v, scale + c, col_scale, at, n_rows - c, there);
@@ -289,15 +346,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->tempty[b]);
+            if (lane == 0) {
+                if (kPair && rank != 0) mbar_arrive_remote(&bars->tempty[b], 0);
+                else mbar_arrive(&bars->tempty[b]);
+            }
         }
     }
 
     tc_fence_before();
     __syncthreads();
+    // (neither CTA of a pair leaves, or frees TMEM, while the other may still write to it)
+    if constexpr (kPair) cluster_sync_all();
     tc_fence_after();
     if (warp == 1) {
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(T::kTmemCols) : "memory");
+        if constexpr (kPair)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(T::kTmemCols) : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(T::kTmemCols) : "memory");
     }
 }
 
@@ -313,39 +378,49 @@ bool make_map_i8(CUtensorMap* m, const void* base, uint64_t inner, uint64_t oute
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int NR, int kOut>
+template <int NR, bool kPair, int kOut>
 int launch_i8(const void* hidden, const void* weight, I8Args a, int64_t hidden_dim, int sms, cudaStream_t stream) {
-    using T = I8Tile<NR>;
+    using T = I8Tile<NR, kPair>;
     a.r_tiles = int((a.rows + NR - 1) / NR);
-    a.v_tiles = (a.n_vocab + kIds - 1) / kIds;
+    a.v_tiles = (a.n_vocab + T::kCtas * kIds - 1) / (T::kCtas * kIds);
     a.units = (a.n_vocab + kUnit - 1) / kUnit;
     const int64_t work = a.r_tiles == 1 ? a.units : a.v_tiles * a.r_tiles;
     CUtensorMap map_h, map_w, map_unit;
-    if (!make_map_i8(&map_h, hidden, uint64_t(hidden_dim), uint64_t(a.rows), NR) ||
+    if (!make_map_i8(&map_h, hidden, uint64_t(hidden_dim), uint64_t(a.rows), T::kBRows) ||
         !make_map_i8(&map_w, weight, uint64_t(hidden_dim), uint64_t(a.n_vocab), kIds) ||
         !make_map_i8(&map_unit, weight, uint64_t(hidden_dim), uint64_t(a.n_vocab), kUnit))
         return LOOM_SELECT_ECUDA;
     static std::atomic<bool> configured[64] = {};  // set once per device, from any host thread
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return LOOM_SELECT_ECUDA;
+    auto kernel = lm_head_logits_i8_kernel<NR, kPair, kOut>;
     if (!configured[dev]) {
-        if (cudaFuncSetAttribute(lm_head_logits_i8_kernel<NR, kOut>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 int(T::kSmemBytes)) != cudaSuccess)
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(T::kSmemBytes)) != cudaSuccess)
             return LOOM_SELECT_ECUDA;
         configured[dev] = true;
     }
-    const int grid = int(work < sms ? work : sms);
-    lm_head_logits_i8_kernel<NR, kOut><<<grid, kThreads, T::kSmemBytes, stream>>>(map_h, map_w, map_unit, a);
-    return cudaGetLastError() == cudaSuccess ? LOOM_SELECT_OK : LOOM_SELECT_ECUDA;
+    const int64_t most = sms / T::kCtas;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned((work < most ? work : most) * T::kCtas));
+    cfg.blockDim = dim3(T::kThreads);
+    cfg.dynamicSmemBytes = T::kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = unsigned(T::kCtas);
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, map_h, map_w, map_unit, a) == cudaSuccess ? LOOM_SELECT_OK : LOOM_SELECT_ECUDA;
 }
 
 template <int kOut>
 int launch_i8_any(const void* hidden, const void* weight, const I8Args& a, int64_t hidden_dim, int sms,
                   cudaStream_t stream) {
-    if (a.rows <= 16) return launch_i8<16, kOut>(hidden, weight, a, hidden_dim, sms, stream);
-    if (a.rows <= 64) return launch_i8<64, kOut>(hidden, weight, a, hidden_dim, sms, stream);
-    if (a.rows <= 128) return launch_i8<128, kOut>(hidden, weight, a, hidden_dim, sms, stream);
-    return launch_i8<256, kOut>(hidden, weight, a, hidden_dim, sms, stream);
+    if (a.rows <= 16) return launch_i8<16, false, kOut>(hidden, weight, a, hidden_dim, sms, stream);
+    if (a.rows <= 64) return launch_i8<64, false, kOut>(hidden, weight, a, hidden_dim, sms, stream);
+    if (a.rows <= 128) return launch_i8<128, false, kOut>(hidden, weight, a, hidden_dim, sms, stream);
+    return launch_i8<256, true, kOut>(hidden, weight, a, hidden_dim, sms, stream);
 }
 
 }  // namespace

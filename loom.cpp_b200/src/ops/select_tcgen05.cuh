@@ -72,6 +72,45 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
                  : "memory");
 }
 
+// The forms for two CTAs of a cluster working as one (cta_group::2): M is split over the two, N over their B tiles; the
+// even CTA issues.
+__device__ __forceinline__ void tc_mma_i8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                               uint32_t accumulate) {
+    asm volatile(
+        "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p; }" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Arrives, when the MMAs issued so far have completed, on the barrier at this place in both CTAs.
+__device__ __forceinline__ void tc_commit_both(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_addr(bar)),
+        "h"(uint16_t(3))
+        : "memory");
+}
+
+__device__ __forceinline__ void tc_commit_pair_own(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+                 : "memory");
+}
+
+// Arrives on the barrier at this place in CTA `rank` of the cluster. What the arrival stands for has been observed on
+// this side (a completed copy, completed TMEM loads) and is used on the other by the tensor core alone; a release at
+// cluster scope would only add its flush, some 1500 cycles each.
+__device__ __forceinline__ void mbar_arrive_remote(uint64_t* bar, uint32_t rank) {
+    asm volatile(
+        "{ .reg .b32 a; mapa.shared::cluster.u32 a, %0, %1; mbarrier.arrive.shared::cluster.b64 _, [a]; }" ::"r"(
+            smem_addr(bar)),
+        "r"(rank)
+        : "memory");
+}
+
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 __device__ __forceinline__ void tc_ld32(uint32_t taddr, float (&v)[32]) {
     uint32_t r[32];
     asm volatile(
