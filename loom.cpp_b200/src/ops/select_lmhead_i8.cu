@@ -67,12 +67,11 @@ struct I8Tile {
 
 template <int kStages>
 struct I8Bars {
-    uint64_t full[kStages];       // this CTA's TMA -> the MMA (or, in a pair's odd CTA, the warp that passes it on)
-    uint64_t peer_full[kStages];  // pair, even CTA: the odd one's slice is there
-    uint64_t empty[kStages];      // MMA -> TMA, in both CTAs of a pair
-    uint64_t tfull[2];            // MMA -> epilogue, in both
-    uint64_t tempty[2];           // epilogue warps (of both) -> MMA
-    uint64_t drain;               // the MMA warp's final commit
+    uint64_t full[kStages];   // TMA -> MMA: a pair's both copies arrive at the even CTA's
+    uint64_t empty[kStages];  // MMA -> TMA, in both CTAs of a pair
+    uint64_t tfull[2];        // MMA -> epilogue, in both
+    uint64_t tempty[2];       // epilogue warps (of both) -> MMA
+    uint64_t drain;           // the MMA warp's final commit
     uint32_t tmem_base;
     int abort;
 };
@@ -95,6 +94,7 @@ template <int NR, bool kPair>
 struct I8Walk {
     static constexpr int kCtas = kPair ? 2 : 1;
     int64_t id, id_end;
+    int64_t tile_end;  // the end of the tile's ids, both CTAs'
     int64_t row;
     int64_t next, end;  // one tile of rows: units of ids; several: tiles
     __device__ __forceinline__ explicit I8Walk(const I8Args& a) {
@@ -122,10 +122,18 @@ struct I8Walk {
             row = next % a.r_tiles * NR;
             next += gridDim.x / kCtas;
         }
+        tile_end = past < a.n_vocab ? past : a.n_vocab;
         if (kPair && blockIdx.x % 2) id += kIds;
-        if (past > id + kIds) past = id + kIds;
-        id_end = past < a.n_vocab ? past : a.n_vocab;
+        id_end = tile_end < id + kIds ? tile_end : id + kIds;
         return true;
+    }
+    // TMA boxes of kUnit ids for the CTA whose ids begin at `from`; 0: one box for its whole tile. Where CTAs share the ids
+    // out, what is left of a share goes by small boxes (a whole tile by sixteen of them: 96 us for one row, where one
+    // box takes 61).
+    __device__ __forceinline__ int boxes(const I8Args& a, int64_t from, bool& none) const {
+        none = tile_end <= from;
+        const int64_t left = (tile_end - from + kUnit - 1) / kUnit;
+        return none || a.r_tiles > 1 || left >= kIds / kUnit ? 0 : int(left);
     }
 };
 
@@ -182,7 +190,6 @@ __global__ void __launch_bounds__(I8Tile<NR, kPair>::kThreads, 1)
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&bars->full[s], 1);
-            mbar_init(&bars->peer_full[s], 1);
             mbar_init(&bars->empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -222,11 +229,13 @@ __global__ void __launch_bounds__(I8Tile<NR, kPair>::kThreads, 1)
             const int64_t withheld = (blockIdx.x == 0 && wf.withhold > 0) ? int64_t(wf.withhold) - 1 : -1;
             bool ok = true;
             while (ok && walk.step(a)) {
-                // one box for a whole tile (sixteen 2 KiB boxes for each: 96 us for one row, where this takes 61),
-                // small ones for what is left of a CTA's share
-                const int left = walk.id_end > walk.id ? int((walk.id_end - walk.id + kUnit - 1) / kUnit) : 0;
-                const bool cut = left == 0 || (a.r_tiles == 1 && left < kIds / kUnit);
-                const uint32_t bytes = T::kTileBBytes + (cut ? uint32_t(left) * kUnit * kBK : T::kTileABytes);
+                bool none, peer_none = true;
+                const int boxes = walk.boxes(a, walk.id, none);
+                uint32_t bytes = T::kTileBBytes + (none ? 0u : boxes ? uint32_t(boxes) * kUnit * kBK : T::kTileABytes);
+                if (kPair && rank == 0) {  // the odd CTA's copies too
+                    const int peer = walk.boxes(a, walk.id + kIds, peer_none);
+                    bytes += T::kTileBBytes + (peer_none ? 0u : peer ? uint32_t(peer) * kUnit * kBK : T::kTileABytes);
+                }
                 for (int kb = 0; kb < a.k_blocks; ++kb, ++kc) {
                     const int s = int(kc % kStages);
                     const int64_t n = kc / kStages;
@@ -236,37 +245,31 @@ __global__ void __launch_bounds__(I8Tile<NR, kPair>::kThreads, 1)
                     }
                     if (kc == withheld) continue;  // test hook only: this slice never arrives
                     unsigned char* st = smem + size_t(s) * kStageBytes;
-                    mbar_arrive_expect_tx(&bars->full[s], bytes);
-                    if (!cut) tma_load_2d(st, &map_w, kb * kBK, int(walk.id), &bars->full[s]);
-                    else
-                        for (int u = 0; u < left; ++u)
-                            tma_load_2d(st + u * kUnit * kBK, &map_unit, kb * kBK, int(walk.id) + u * kUnit, &bars->full[s]);
-                    tma_load_2d(st + T::kTileABytes, &map_h, kb * kBK, int(walk.row) + int(rank) * T::kBRows, &bars->full[s]);
+                    if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], bytes);
+                    auto load = [&](void* to, const CUtensorMap* map, int64_t y) {
+                        if constexpr (kPair) tma_load_2d_pair(to, map, kb * kBK, int(y), &bars->full[s]);
+                        else tma_load_2d(to, map, kb * kBK, int(y), &bars->full[s]);
+                    };
+                    if (!none && boxes == 0) load(st, &map_w, walk.id);
+                    for (int u = 0; u < boxes; ++u) load(st + u * kUnit * kBK, &map_unit, walk.id + u * kUnit);
+                    load(st + T::kTileABytes, &map_h, walk.row + int(rank) * T::kBRows);
                 }
             }
-            // every copy issued lands before the CTA may exit (a withheld slice was never issued)
+            // Every copy issued lands before the CTA may exit (a withheld slice was never issued). A pair's odd CTA learns it
+            // from the MMAs that have read them; where those no longer come, its wait's limit is thousands of copies long.
             for (int s = 0; s < kStages; ++s) {
                 if (kc > s) {
                     int64_t last_kc = s + int64_t(kStages) * ((kc - 1 - s) / kStages);
                     if (last_kc == withheld) last_kc -= kStages;
-                    if (last_kc >= 0) mbar_wait_bounded(&bars->full[s], uint32_t((last_kc / kStages) & 1), a.status, lim);
+                    if (last_kc >= 0)
+                        mbar_wait_bounded(rank == 0 ? &bars->full[s] : &bars->empty[s], uint32_t((last_kc / kStages) & 1),
+                                          a.status, lim);
                 }
             }
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && rank != 0) {
-            // ---- a pair's odd CTA: passes on that its slices are there ----
-            int64_t kc = 0;
-            bool ok = true;
-            while (ok && walk.step(a)) {
-                for (int kb = 0; ok && kb < a.k_blocks; ++kb, ++kc) {
-                    const int s = int(kc % kStages);
-                    ok = lm_wait(&bars->full[s], uint32_t((kc / kStages) & 1), a.status, abort_flag, lim);
-                    if (ok) mbar_arrive_remote(&bars->peer_full[s], 0);
-                }
-            }
-        } else if (lane == 0) {
+        if (lane == 0 && rank == 0) {  // (of a pair, the even CTA's)
             // ---- MMA issuer ----
             int64_t kc = 0;
             int i = 0;
@@ -279,8 +282,7 @@ __global__ void __launch_bounds__(I8Tile<NR, kPair>::kThreads, 1)
                 for (int kb = 0; kb < a.k_blocks; ++kb, ++kc) {
                     const int s = int(kc % kStages);
                     const int64_t n = kc / kStages;
-                    if (!lm_wait(&bars->full[s], uint32_t(n & 1), a.status, abort_flag, lim) ||
-                        (kPair && !lm_wait(&bars->peer_full[s], uint32_t(n & 1), a.status, abort_flag, lim))) {
+                    if (!lm_wait(&bars->full[s], uint32_t(n & 1), a.status, abort_flag, lim)) {
                         ok = false;
                         break;
                     }

@@ -37,6 +37,16 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
         : "memory");
 }
 
+// The load for a pair of CTAs: into this CTA's memory, completing on the barrier at `bar`'s place in the even one.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+    asm volatile(
+        "{ .reg .b32 b; mapa.shared::cluster.u32 b, %2, 0; "
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+        "[b]; }" ::"r"(smem_addr(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(x), "r"(y)
+        : "memory");
+}
+
 // Shared-memory matrix descriptor of a K-major tile written by TMA with the 128-byte swizzle: rows of
 // 128 bytes, groups of 8 rows 1024 bytes apart (stride byte offset), descriptor version 1, layout
 // type 2 (128-byte swizzle). Stepping K by 16 elements inside the span adds 32 bytes to the start.
@@ -96,9 +106,8 @@ __device__ __forceinline__ void tc_commit_pair_own(uint64_t* bar) {
                  : "memory");
 }
 
-// Arrives on the barrier at this place in CTA `rank` of the cluster. What the arrival stands for has been observed on
-// this side (a completed copy, completed TMEM loads) and is used on the other by the tensor core alone; a release at
-// cluster scope would only add its flush, some 1500 cycles each.
+// Arrives on the barrier at this place in CTA `rank` of the cluster. (A release at cluster scope would add a flush of
+// some 1500 cycles; what these arrivals stand for -- completed TMEM loads -- needs none.)
 __device__ __forceinline__ void mbar_arrive_remote(uint64_t* bar, uint32_t rank) {
     asm volatile(
         "{ .reg .b32 a; mapa.shared::cluster.u32 a, %0, %1; mbarrier.arrive.shared::cluster.b64 _, [a]; }" ::"r"(
