@@ -457,22 +457,33 @@ def lm_head_argmax(hidden, weight, want_logit=True, want_lse=True, workspace=Non
 # ----------------------------------------------------------------------------------------------
 # log-probabilities of given tokens
 
-def _check_tensor(t, name, dtype, shape, device):
-    """A contiguous tensor of this type and shape on `device`, or None."""
-    if t is None:
+def _check_tensor(t, name, dtype, shape, dev):
+    """A contiguous tensor of this type and shape (a tuple) on CUDA device number `dev`, or None."""
+    if t is None or (t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous()):
         return
     if t.dtype != dtype:
         raise SelectError(EDTYPE, f"{name} is {t.dtype}, expected {dtype}")
-    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        raise SelectError(EINVAL, f"{name} must be contiguous, of shape {tuple(shape)}")
-    if t.device != device:
-        raise SelectError(EINVAL, f"{name} is on {t.device}, expected {device}")
+    if t.get_device() != dev:
+        raise SelectError(EINVAL, f"{name} is on {t.device}, expected cuda:{dev}")
+    raise SelectError(EINVAL, f"{name} must be contiguous, of shape {tuple(shape)}")
 
 
-def _check_device(t, name):
-    """The kernels run on the current device: a tensor elsewhere is an error, not a fault."""
-    if t.device.type != "cuda" or t.device.index != _torch().cuda.current_device():
+def _current_device(t, name):
+    """The number of the current CUDA device, where the kernels run: a tensor elsewhere is an error, not a fault."""
+    dev = t.get_device()
+    if dev < 0 or dev != _torch().cuda.current_device():
         raise SelectError(EINVAL, f"{name} is on {t.device}, not on the current CUDA device")
+    return dev
+
+
+def _addr(t):
+    """A tensor's address as ctypes takes it for a void pointer."""
+    return None if t is None else t.data_ptr()
+
+
+def _raw_stream(stream, dev):
+    """The handle of `stream`, or of the device's current one (without making a Stream object for it)."""
+    return stream.cuda_stream if stream is not None else _torch()._C._cuda_getCurrentRawStream(dev)
 
 
 def _on(stream):
@@ -488,8 +499,7 @@ def token_logprobs_into(logits, ids, out_logp=None, out_entropy=None, out_lse=No
     [rows, n] (n alternatives, at most MAX_TOP_LOGPROBS), each of them or None. See loom_token_logprobs."""
     torch = _torch()
     rows, n_vocab, stride = _rows_view(logits)
-    code, dev = _dtype_code(logits), logits.device
-    _check_device(logits, "logits")
+    code, dev = _dtype_code(logits), _current_device(logits, "logits")
     n_top = 0
     for t in (out_top_ids, out_top_logp):
         if t is not None:
@@ -505,9 +515,9 @@ def token_logprobs_into(logits, ids, out_logp=None, out_entropy=None, out_lse=No
                                   (out_top_ids, "out_top_ids", torch.int32, top),
                                   (out_top_logp, "out_top_logp", torch.float32, top)):
         _check_tensor(t, name, dtype, shape, dev)
-    check(_lib().loom_token_logprobs(_ptr(logits), code, rows, n_vocab, stride, _ptr(ids), temperature, n_top,
-                                     _ptr(out_logp), _ptr(out_entropy), _ptr(out_lse), _ptr(out_rank),
-                                     _ptr(out_top_ids), _ptr(out_top_logp), _stream_handle(stream)),
+    check(_lib().loom_token_logprobs(logits.data_ptr(), code, rows, n_vocab, stride, _addr(ids), temperature, n_top,
+                                     _addr(out_logp), _addr(out_entropy), _addr(out_lse), _addr(out_rank),
+                                     _addr(out_top_ids), _addr(out_top_logp), _raw_stream(stream, dev)),
           "loom_token_logprobs")
 
 
@@ -539,19 +549,19 @@ def token_logprobs_grad_into(logits, ids, lse, out_grad, grad_logp=None, grad_en
     (rows may be strided; out_grad may be the logits themselves). lse and entropy are the forward call's."""
     torch = _torch()
     rows, n_vocab, stride = _rows_view(logits)
-    code, dev = _dtype_code(logits), logits.device
-    _check_device(logits, "logits")
+    code, dev = _dtype_code(logits), _current_device(logits, "logits")
     if out_grad.dtype != logits.dtype:
         raise SelectError(EDTYPE, f"out_grad is {out_grad.dtype}, expected {logits.dtype}")
-    if out_grad.shape != logits.shape or out_grad.device != dev:
+    if out_grad.shape != logits.shape or out_grad.get_device() != dev:
         raise SelectError(EINVAL, "out_grad must have the logits' shape and device")
     _, _, grad_stride = _rows_view(out_grad)
     for t, name, dtype in ((ids, "ids", torch.int32), (lse, "lse", torch.float32), (entropy, "entropy", torch.float32),
                            (grad_logp, "grad_logp", torch.float32), (grad_entropy, "grad_entropy", torch.float32)):
         _check_tensor(t, name, dtype, (rows,), dev)
-    check(_lib().loom_token_logprobs_grad(_ptr(logits), code, rows, n_vocab, stride, _ptr(ids), temperature, _ptr(lse),
-                                          _ptr(entropy), _ptr(grad_logp), _ptr(grad_entropy), _ptr(out_grad),
-                                          grad_stride, _stream_handle(stream)), "loom_token_logprobs_grad")
+    check(_lib().loom_token_logprobs_grad(logits.data_ptr(), code, rows, n_vocab, stride, _addr(ids), temperature,
+                                          _addr(lse), _addr(entropy), _addr(grad_logp), _addr(grad_entropy),
+                                          out_grad.data_ptr(), grad_stride, _raw_stream(stream, dev)),
+          "loom_token_logprobs_grad")
     return out_grad
 
 
@@ -582,8 +592,7 @@ def rms_norm_i8_into(x, weight, out_q, out_scale, residual=None, out_sum=None, e
     itself) are like x or None. out_q * out_scale stands for the normed rows. See loom_rms_norm_i8."""
     torch = _torch()
     rows, dim, stride = _matrix_view(x, "x")
-    code, dev = _dtype_code(x), x.device
-    _check_device(x, "x")
+    code, dev = _dtype_code(x), _current_device(x, "x")
     wcode = _dtype_code(weight)
     _check_tensor(weight, "weight", weight.dtype, (dim,), dev)
     strides = []
@@ -591,14 +600,14 @@ def rms_norm_i8_into(x, weight, out_q, out_scale, residual=None, out_sum=None, e
         if t is not None:
             if t.dtype != x.dtype:
                 raise SelectError(EDTYPE, f"{name} is {t.dtype}, expected {x.dtype}")
-            if t.shape != x.shape or t.device != dev:
+            if t.shape != x.shape or t.get_device() != dev:
                 raise SelectError(EINVAL, f"{name} must have x's shape and device")
         strides.append(0 if t is None else _matrix_view(t, name)[2])
     _check_tensor(out_q, "out_q", torch.int8, x.shape, dev)
     _check_tensor(out_scale, "out_scale", torch.float32, (rows,), dev)
-    check(_lib().loom_rms_norm_i8(_ptr(x), code, rows, dim, stride, _ptr(residual), strides[0], _ptr(weight), wcode, eps,
-                                  _ptr(out_q), _ptr(out_scale), _ptr(out_sum), strides[1], _stream_handle(stream)),
-          "loom_rms_norm_i8")
+    check(_lib().loom_rms_norm_i8(x.data_ptr(), code, rows, dim, stride, _addr(residual), strides[0], weight.data_ptr(),
+                                  wcode, eps, out_q.data_ptr(), out_scale.data_ptr(), _addr(out_sum), strides[1],
+                                  _raw_stream(stream, dev)), "loom_rms_norm_i8")
     return out_q, out_scale
 
 
@@ -618,12 +627,11 @@ def quantize_rows_i8_into(x, out_q, out_scale, stream=None):
     """Rows of x [rows, dim] as 8-bit integers with a scale per row (asynchronous): q * scale stands for x."""
     torch = _torch()
     rows, dim, stride = _matrix_view(x, "x")
-    code, dev = _dtype_code(x), x.device
-    _check_device(x, "x")
+    code, dev = _dtype_code(x), _current_device(x, "x")
     _check_tensor(out_q, "out_q", torch.int8, x.shape, dev)
     _check_tensor(out_scale, "out_scale", torch.float32, (rows,), dev)
-    check(_lib().loom_quantize_rows_i8(_ptr(x), code, rows, dim, stride, _ptr(out_q), _ptr(out_scale),
-                                       _stream_handle(stream)), "loom_quantize_rows_i8")
+    check(_lib().loom_quantize_rows_i8(x.data_ptr(), code, rows, dim, stride, out_q.data_ptr(), out_scale.data_ptr(),
+                                       _raw_stream(stream, dev)), "loom_quantize_rows_i8")
     return out_q, out_scale
 
 
@@ -667,21 +675,21 @@ def lm_head_logits_i8_into(hidden, hidden_scale, weight, weight_scale, out, work
         raise SelectError(EINVAL, "hidden must be [rows, hidden_dim] and weight [n_vocab, hidden_dim]")
     rows = 1 if hidden.dim() == 1 else hidden.shape[0]
     n_vocab, hdim = weight.shape
-    dev = hidden.device
-    _check_device(hidden, "hidden")
+    dev = _current_device(hidden, "hidden")
     _check_tensor(hidden, "hidden", torch.int8, hidden.shape, dev)
     _check_tensor(hidden_scale, "hidden_scale", torch.float32, (rows,), dev)
     _check_tensor(weight, "weight", torch.int8, weight.shape, dev)
     _check_tensor(weight_scale, "weight_scale", torch.float32, (n_vocab,), dev)
     code = _dtype_code(out)
-    if tuple(out.shape) != ((n_vocab,) if hidden.dim() == 1 else (rows, n_vocab)) or out.device != dev:
+    if tuple(out.shape) != ((n_vocab,) if hidden.dim() == 1 else (rows, n_vocab)) or out.get_device() != dev:
         raise SelectError(EINVAL, "out must be [rows, n_vocab] on the hidden states' device")
     _, _, stride = _rows_view(out)
     ws = workspace or _status_workspace(stream)
     buf = ws.get(256, stream)
-    check(_lib().loom_lm_head_logits_i8(_ptr(hidden), _ptr(hidden_scale), _ptr(weight), _ptr(weight_scale), rows, hdim,
-                                        n_vocab, _ptr(out), code, stride, _ptr(buf), buf.numel(),
-                                        _stream_handle(stream)), "loom_lm_head_logits_i8")
+    check(_lib().loom_lm_head_logits_i8(hidden.data_ptr(), hidden_scale.data_ptr(), weight.data_ptr(),
+                                        weight_scale.data_ptr(), rows, hdim, n_vocab, out.data_ptr(), code, stride,
+                                        buf.data_ptr(), buf.numel(), _raw_stream(stream, dev)),
+          "loom_lm_head_logits_i8")
     return out
 
 

@@ -19,12 +19,6 @@
 #include "select_internal.h"
 #include "select_rows.cuh"
 
-#ifndef LP_NARROW
-#define LP_NARROW 2048
-#endif
-#ifndef LP_MINB1
-#define LP_MINB1 6
-#endif
 namespace cg = cooperative_groups;
 
 namespace loom_select {
@@ -432,10 +426,10 @@ __device__ __forceinline__ void block_sync() {
 // read again, from L2, and those elements sorted by counting the larger ones.
 //
 // Four blocks of eight warps to an SM (64 registers). Blocks of four warps: 121.8 us for [1024, 151936] f32 and 68.4 for
-// [256, 262144] bf16, of eight 115.1 and 51.3, of sixteen 131.2 and 52.5. Rows of at most kNarrow elements go a warp to a
-// row, four rows to a block.
+// [256, 262144] bf16, of eight 115.1 and 51.3, of sixteen 131.2 and 52.5. Narrow rows go a warp to a row, four rows to a
+// block, six blocks to an SM ([16384, 1025] f32 30.2 us; four blocks 35.8, eight 37.8).
 template <int kDtype, bool kTop, int kW>
-__global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? LP_MINB1 : 4) token_logprobs_kernel(const LpDev p) {
+__global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : 4) token_logprobs_kernel(const LpDev p) {
     constexpr int kEsz = kDtype == LOOM_SELECT_BF16 ? 2 : 4;
     constexpr int kPer = 16 / kEsz;
     constexpr int kU = 4;                // vectors per thread and step
@@ -731,7 +725,9 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? LP_MINB1 : 
 // elements a thread in each one's share. More blocks read faster, but each has its end to go through: [256, 262144] bf16
 // 51.3 us with two blocks a row, 53.8 with four, [77, 51865] bf16 13.4 and 18.6.
 constexpr int kLpWarps = 8;
-constexpr int32_t kNarrow = LP_NARROW;
+// A warp to a row, where there are rows for every SM: [8000, 8000] f32 67 us (a block to a row: 113), [700, 2048] 6.7 (11.8),
+// [1500, 16000] 35.7 (34.5). Very short rows always.
+constexpr int32_t kNarrow = 8192, kShort = 512;
 int lp_cluster(int64_t rows, int64_t n_vocab, int sms) {
     int c = 1;
     while (c < kMaxCluster && rows * c < 2 * int64_t(sms) && n_vocab > int64_t(c) * 16 * kLpWarps * 32) c *= 2;
@@ -755,7 +751,7 @@ cudaError_t launch_lp(const LpDev& p, int64_t rows, int C, cudaStream_t s) {
 
 template <int kDtype, bool kTop>
 cudaError_t launch_lp_any(const LpDev& p, int64_t rows, int sms, cudaStream_t s) {
-    if (p.width <= kNarrow) return launch_lp<kDtype, kTop, 1>(p, rows, 1, s);
+    if (p.width <= kShort || (p.width <= kNarrow && rows >= sms)) return launch_lp<kDtype, kTop, 1>(p, rows, 1, s);
     return launch_lp<kDtype, kTop, kLpWarps>(p, rows, lp_cluster(rows, p.width, sms), s);
 }
 
