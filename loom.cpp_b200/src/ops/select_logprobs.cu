@@ -187,6 +187,36 @@ __device__ __forceinline__ void fma2(uint64_t& d, uint64_t a, uint64_t b) {
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b));
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
+// The largest element of kU vectors (at least -inf; NaN left out).
+template <int kDtype, int kU>
+__device__ __forceinline__ float largest(const uint4 (&raw)[kU]) {
+    if constexpr (kDtype == LOOM_SELECT_BF16) {
+        __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162*>(&raw[0].x);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (u || q) m = __hmax2(m, *reinterpret_cast<const __nv_bfloat162*>(&w[q]));
+        }
+        return max3(__low2float(m), __high2float(m), neg_inf());
+    } else {
+        float m = neg_inf();
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            m = max3(m, __uint_as_float(raw[u].x), __uint_as_float(raw[u].y));
+            m = max3(m, __uint_as_float(raw[u].z), __uint_as_float(raw[u].w));
+        }
+        return m;
+    }
+}
+
 // One thread's running softmax sums and rank count over its elements of a row, which come as kU vectors of kPer
 // elements each: element q of vector u has id id0 + u * step + q; those whose id is not in [0, limit) hold -inf and
 // are not counted.
@@ -231,8 +261,8 @@ struct LpScan {
                 const Pairs<kDtype> x(raw[u]);
 #pragma unroll
                 for (int q = 0; q < Pairs<kDtype>::kPairs; ++q) {
-                    uint64_t d = mm;
-                    fma2(d, x.v[q], cc);
+                    uint64_t d;
+                    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(x.v[q]), "l"(cc), "l"(mm));
                     float d0, d1;
                     unpack2(d, d0, d1);
                     const uint64_t e = pack2(ex2(d0), ex2(d1));
@@ -498,9 +528,7 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : 4) toke
     float top = neg_inf(), second = neg_inf(), slot_top = neg_inf();
     int32_t top_slot = 0, slot = 0, in_slot = 0;
     auto step = [&](const uint4(&raw)[kU], int32_t at) {
-        float mx = vec_max<kDtype>(raw[0]);  // (NaN left out)
-#pragma unroll
-        for (int u = 1; u < kU; ++u) mx = fmaxf(mx, vec_max<kDtype>(raw[u]));
+        const float mx = largest<kDtype>(raw);
         st.add(raw, mx, at > whole);
         if (rank)
             st.count(raw, mx, (at + lane) * kPer - shift, kNT * kPer, limit, at * kPer - shift,
@@ -822,10 +850,10 @@ struct LpGradRow {
         unpack2(x, l0, l1);
         l0 = max_nan(l0, kMinExp2);
         l1 = max_nan(l1, kMinExp2);
-        fma2(g2, h2, pack2(l0, l1));
-        const uint64_t e = pack2(ex2(l0), ex2(l1));
-        asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(g2) : "l"(e));
-        return g2;
+        const uint64_t l = pack2(l0, l1), e = pack2(ex2(l0), ex2(l1));
+        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(x) : "l"(h2), "l"(l), "l"(g2));
+        asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(e));
+        return x;
     }
 };
 
