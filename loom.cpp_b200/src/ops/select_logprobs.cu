@@ -83,6 +83,7 @@ struct LpDev {
 // A thread keeps the maxima of its elements in up to this many equal runs of steps (32: 117.4 us for [1024, 151936] f32,
 // 16: 115.1, the shared memory being L1's).
 constexpr int kSlots = 16;
+static_assert(kSlots <= 32, "a thread's slots are bits of a word");
 constexpr int kMaxCluster = 8;
 constexpr int kGroups = 64;  // (32 in a block of one warp)
 
@@ -91,11 +92,10 @@ struct LpShared {
     static constexpr int kMaxCand = kW == 1 ? 256 : 512;
     static constexpr int kBlocks = kW == 1 ? 1 : kMaxCluster;
     uint64_t list[kW][32];
-    uint32_t group[kGroups];   // order keys of the maxima of the cluster's groups of threads
+    alignas(16) uint32_t group[kGroups];  // order keys of the maxima of the cluster's groups of threads
     uint32_t x_key;            // order key of the threshold
     int32_t n_cand;            // elements of this block that reach it
     int32_t overflow;          // some block of the cluster has more of them than it may hand on
-    uint16_t queue[kW][64];    // per warp: (slot, lane) pairs to look through
     float slot_max[kW][kSlots][32];
     // of the cluster's first block: what the blocks hand on
     SoftAcc acc[kBlocks * kW];  // of each warp
@@ -359,84 +359,64 @@ struct LpScan {
     }
 };
 
-// One block's view of its row, for looking through the slots again.
+// One warp's view of its row, for looking through the slots again.
 struct LpShare {
-    const unsigned char* vec;
+    const unsigned char* row;
     int32_t shift, v_start, v1, stride, per_slot, slots;  // v_start: the warp's first vector
     int n_top;
     float X;
 };
 
-// The slots whose maximum reaches X (and `own`, when the callback raises it), 32 (slot, lane) pairs at a time: each
-// lane gets a pair, and the callback the first vector of its run of steps.
-template <int kW, class F>
-__device__ __forceinline__ void for_slots(const LpShare& r, LpShared<kW>* sh, F&& look) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32 % kW;
-    int queued = 0;
-    float own = neg_inf();
-    auto flush = [&]() {
-        __syncwarp();
-        const int n = queued < 32 ? queued : 32;
-        const uint32_t g = lane < n ? sh->queue[warp][lane] : 0;
-        const uint16_t rest = sh->queue[warp][32 + lane];
-        own = look(r.v_start + int32_t(g >> 5) * r.per_slot * r.stride + int32_t(g & 31), lane < n);
-        __syncwarp();
-        sh->queue[warp][lane] = rest;
-        queued -= n;
-    };
-    for (int s = 0; s < r.slots; ++s) {
-        const bool hit = sh->slot_max[warp][s][lane] >= fmaxf(r.X, own);
-        const uint32_t b = __ballot_sync(0xffffffffu, hit);
-        if (b == 0) continue;
-        if (hit) sh->queue[warp][queued + __popc(b & ((1u << lane) - 1u))] = uint16_t(s * 32 + lane);
-        queued += __popc(b);
-        if (queued >= 32) flush();
+// The elements that the lanes in `hits` have in slot `slot` (each lane's own), spread over the warp 32 at a time: f gets a
+// value and its id, NaN where there is none, in all lanes. Four lanes' elements are requested together. A loop with
+// little code: unrolled over a thread's own elements, instruction fetches made this 7000 cycles and not 1500.
+template <int kDtype, int kU, int kNT, class F>
+__device__ __forceinline__ void visit(const LpShare& r, uint32_t hits, int32_t slot, F&& f) {
+    constexpr int kPer = kDtype == LOOM_SELECT_BF16 ? 8 : 4;
+    const int lane = threadIdx.x & 31;
+    while (hits) {
+        int32_t first[4];  // of each of four lanes, its first vector in the slot
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int src = __ffs(hits) - 1;
+            hits &= hits - 1;  // (0 stays 0)
+            const int32_t of = __shfl_sync(0xffffffffu, slot, src < 0 ? 0 : src);
+            first[k] = src < 0 ? r.v1 : r.v_start + src + of * r.per_slot * r.stride;
+        }
+        for (int e0 = 0; e0 < r.per_slot * kU * kPer; e0 += 32) {
+            const int e = e0 + lane;
+            const int32_t skip = e / (kU * kPer) * r.stride + e / kPer % kU * kNT;
+            float x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int32_t v = first[k] + skip;
+                x[k] = e < r.per_slot * kU * kPer && v < r.v1 ? load_global_elem<kDtype>(r.row, v * kPer - r.shift + e % kPer)
+                                                             : quiet_nan();
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f(x[k], (first[k] + skip) * kPer - r.shift + e % kPer);
+        }
     }
-    while (queued > 0) flush();
-}
-
-template <int kDtype>
-__device__ __forceinline__ uint4 load_or_nan(const unsigned char* vec, int32_t v, bool there) {
-    const uint32_t w = kDtype == LOOM_SELECT_BF16 ? 0xffffffffu : 0x7fffffffu;
-    return there ? ldg_stream_v4(vec + int64_t(v) * 16) : make_uint4(w, w, w, w);
 }
 
 // The warp's best 32 of its elements >= X, sorted, when too many of them reach X to be held (a row of few
-// values, or of almost nothing but -inf). In each round every lane offers its best element not offered yet, and
-// the offers, sorted, are merged into the list.
+// values, or of almost nothing but -inf).
 template <int kDtype, int kU, int kW>
 __device__ __noinline__ uint64_t list_slots(const LpShare& r, LpShared<kW>* sh) {
-    constexpr int kPer = kDtype == LOOM_SELECT_BF16 ? 8 : 4;
-    constexpr int kNT = kW * 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32 % kW;
     uint64_t key = 0;
-    for_slots<kW>(r, sh, [&](int32_t v, bool there) {
-        for (int i = 0; i < r.per_slot; ++i, v += r.stride) {
-            uint64_t below = ~0ull;  // keys from here on have been offered
-            for (;;) {
-                uint64_t best = 0;
-#pragma unroll 1
-                for (int u = 0; u < kU; ++u) {
-                    Vec16<kDtype> e;
-                    e.unpack(load_or_nan<kDtype>(r.vec, v + u * kNT, there && v + u * kNT < r.v1));
-#pragma unroll
-                    for (int q = 0; q < kPer; ++q) {
-                        if (e.x[q] >= r.X) {
-                            const uint64_t k = loom_rank_key(e.x[q], (v + u * kNT) * kPer - r.shift + q);
-                            best = k < below && k > best ? k : best;
-                        }
-                    }
-                }
-                const uint64_t last = __shfl_sync(0xffffffffu, key, r.n_top - 1);
-                if (best <= last) best = 0;
-                if (!__any_sync(0xffffffffu, best != 0)) break;
-                if (best) below = best;
-                key = merge_lists(key, sort_desc(best));
-            }
-        }
+    float own = neg_inf();
+    for (int32_t s = 0; s < r.slots; ++s) {
+        const uint32_t hits = __ballot_sync(0xffffffffu, sh->slot_max[warp][s][lane] >= fmaxf(r.X, own));
+        visit<kDtype, kU, kW * 32>(r, hits, s, [&](float x, int32_t id) {
+            const uint64_t cand = x >= r.X ? loom_rank_key(x, id) : 0ull;
+            if (__any_sync(0xffffffffu, cand > __shfl_sync(0xffffffffu, key, r.n_top - 1)))
+                key = merge_lists(key, sort_desc(cand));
+        });
         // a later slot's ids are above all earlier ones: only a larger value can displace the list's last
         const uint64_t last = __shfl_sync(0xffffffffu, key, r.n_top - 1);
-        return last ? order_key_to_float(uint32_t(last >> 32) + 1) : neg_inf();
-    });
+        own = last ? order_key_to_float(uint32_t(last >> 32) + 1) : neg_inf();
+    }
     return key;
 }
 
@@ -524,9 +504,8 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : 4) toke
     const float xt = has ? load_global_elem<kDtype>(rowp, t) : quiet_nan();
     const bool rank = p.out_rank != nullptr && has;
 
-    // this thread's maximum, the slot it is in, its largest maximum of another slot, and its maximum in the current slot
-    float top = neg_inf(), second = neg_inf(), slot_top = neg_inf();
-    int32_t top_slot = 0, slot = 0, in_slot = 0;
+    float top = neg_inf(), slot_top = neg_inf();  // this thread's maximum, and its maximum in the current slot
+    int32_t slot = 0, in_slot = 0;
     auto step = [&](const uint4(&raw)[kU], int32_t at) {
         const float mx = largest<kDtype>(raw);
         st.add(raw, mx, at > whole);
@@ -537,13 +516,7 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : 4) toke
             slot_top = fmaxf(slot_top, mx);
             if (++in_slot == per_slot || at + stride >= v1) {
                 sh.slot_max[warp][slot][lane] = slot_top;
-                if (slot_top > top) {
-                    second = top;
-                    top = slot_top;
-                    top_slot = slot;
-                } else {
-                    second = fmaxf(second, slot_top);
-                }
+                top = fmaxf(top, slot_top);
                 slot_top = neg_inf();
                 ++slot;
                 in_slot = 0;
@@ -574,7 +547,7 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : 4) toke
         first->acc[rank_in * kW + warp] = acc;
         first->ahead[rank_in * kW + warp] = ahead;
     }
-    LpShare r{vec, shift, v_start, v1, stride, per_slot, slot, p.n_top, 0.0f};
+    LpShare r{rowp, shift, v_start, v1, stride, per_slot, slot, p.n_top, 0.0f};
     if constexpr (kTop) {
         // the threshold: the n_top-th largest of the groups' maxima
         constexpr int kG = kW == 1 ? 32 : kGroups;
@@ -607,10 +580,11 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : 4) toke
             if (tid < kG) {
                 const uint32_t mine = sh.group[tid];
                 int larger = 0;
-#pragma unroll
-                for (int j = 0; j < kG; ++j) {
-                    const uint32_t o = sh.group[j];
-                    larger += o > mine || (o == mine && j < tid);
+#pragma unroll 2
+                for (int j = 0; j < kG; j += 4) {
+                    const uint4 o = *reinterpret_cast<const uint4*>(&sh.group[j]);
+                    larger += (o.x > mine || (o.x == mine && j < tid)) + (o.y > mine || (o.y == mine && j + 1 < tid)) +
+                              (o.z > mine || (o.z == mine && j + 2 < tid)) + (o.w > mine || (o.w == mine && j + 3 < tid));
                 }
                 if (larger == p.n_top - 1) sh.x_key = mine;
             }
@@ -622,33 +596,51 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : 4) toke
         const int most = LpShared<kW>::kMaxCand / C;
         uint64_t* to = first->cand + rank_in * most;
         auto add = [&](float x, int32_t id) {
-            const int at = atomicAdd(&sh.n_cand, 1);
-            if (at < most) to[at] = loom_rank_key(x, id);
+            const uint32_t b = __ballot_sync(0xffffffffu, x >= r.X);
+            if (b == 0) return;
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&sh.n_cand, __popc(b));
+            at = __shfl_sync(0xffffffffu, at, 0) + __popc(b & ((1u << lane) - 1u));
+            if (x >= r.X && at < most) to[at] = loom_rank_key(x, id);
         };
-        auto look = [&](int32_t v, bool there) {
-            for (int i = 0; i < r.per_slot; ++i, v += r.stride) {
-                uint4 w[kU];
+        uint32_t mine = 0;  // this thread's slots whose maximum does
+#pragma unroll 4
+        for (int32_t s = 0; s < slot; ++s) mine |= uint32_t(sh.slot_max[warp][s][lane] >= r.X) << s;
+        if constexpr (kW == 1) {
+            // most lanes have some (n_top of 32): each looks through its own
+            for (; mine; mine &= mine - 1) {
+                int32_t v = v_start + lane + (__ffs(mine) - 1) * per_slot * stride;
+                for (int i = 0; i < per_slot; ++i, v += stride) {
+                    uint4 w[kU];
 #pragma unroll
-                for (int u = 0; u < kU; ++u) w[u] = load_or_nan<kDtype>(r.vec, v + u * kNT, there && v + u * kNT < r.v1);
+                    for (int u = 0; u < kU; ++u)
+                        if (v + u * kNT < v1) w[u] = ldg_stream_v4(vec + int64_t(v + u * kNT) * 16);
 #pragma unroll
-                for (int u = 0; u < kU; ++u) {
-                    if (!(vec_max<kDtype>(w[u]) >= r.X)) continue;
-                    Vec16<kDtype> e;
-                    e.unpack(w[u]);
+                    for (int u = 0; u < kU; ++u) {
+                        if (v + u * kNT >= v1 || !(vec_max<kDtype>(w[u]) >= r.X)) continue;
+                        Vec16<kDtype> e;
+                        e.unpack(w[u]);
 #pragma unroll
-                    for (int q = 0; q < kPer; ++q)
-                        if (e.x[q] >= r.X) add(e.x[q], (v + u * kNT) * kPer - r.shift + q);
+                        for (int q = 0; q < kPer; ++q) {
+                            if (e.x[q] >= r.X) {
+                                const int at = atomicAdd(&sh.n_cand, 1);
+                                if (at < most) to[at] = loom_rank_key(e.x[q], (v + u * kNT) * kPer - shift + q);
+                            }
+                        }
+                    }
                 }
             }
-            return neg_inf();
-        };
-        // a thread's elements that reach it are in the slot of its maximum, mostly
-        if (!__any_sync(0xffffffffu, second >= r.X)) {
-            if (top >= r.X && slot > 0) look(v_start + lane + top_slot * per_slot * stride, true);
+            __syncwarp();
         } else {
-            for_slots<kW>(r, &sh, look);
+            for (;;) {  // one slot of every lane that has one
+                const uint32_t hits = __ballot_sync(0xffffffffu, mine != 0);
+                if (hits == 0) break;
+                const int32_t s = mine ? __ffs(mine) - 1 : 0;
+                mine &= mine - 1;
+                visit<kDtype, kU, kNT>(r, hits, s, add);
+            }
         }
-        if (eid >= 0 && ex >= r.X) add(ex, eid);
+        if (warp == 0 && rank_in == 0) add(eid >= 0 ? ex : quiet_nan(), eid);
         block_sync<kW>();
         if (tid == 0) {
             const int n = sh.n_cand;
