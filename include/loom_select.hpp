@@ -11,6 +11,8 @@
 //   loom::select::argmax_tensor_rows     argmax_tensor_rows               src/core/lua_bridge.cpp:343-365
 //   loom::select::ctc_greedy_decode      loom::ctc_greedy_decode          src/core/ctc_decode.cpp:7-31
 //   loom::select::sample_rows            (the sampling chain; no loom.cpp counterpart)
+//   loom::select::token_logprobs         (scores of given tokens; no loom.cpp counterpart)
+//   loom::select::lm_head_argmax_i8      (the final norm and the LM head in 8-bit integers, then Generator::argmax)
 //
 // Errors throw loom::Error -- the engine's own class when include/loom/loom_errors.h is on the
 // include path, otherwise a class of the same name and base declared here.
@@ -275,6 +277,90 @@ inline GreedyResult lm_head_argmax(const void* d_hidden, const void* d_weight, i
     const float* hl = reinterpret_cast<const float*>(h + 2 * col);
     r.logprob.resize(n);
     for (size_t i = 0; i < n; ++i) r.logprob[i] = r.logit[i] - hl[i];
+    return r;
+}
+
+struct TokenScores {
+    std::vector<float> logprob;        // per row: of the given token (0 for a negative id)
+    std::vector<float> entropy;        // of the row's distribution, nats
+    std::vector<int32_t> rank;         // ids ahead of the token (-1: no token)
+    std::vector<int32_t> top_ids;      // n_top per row, best first
+    std::vector<float> top_logprobs;   // theirs
+};
+
+// Log-probabilities of given tokens (loom_token_logprobs) over device logits [n_rows, n_vocab] (row stride
+// row_stride) and device ids [n_rows], with n_top alternatives per row; results on the host.
+inline TokenScores token_logprobs(const float* d_logits, int64_t n_vocab, int64_t n_rows, int64_t row_stride,
+                                  const int32_t* d_ids, float temperature = 1.0f, int32_t n_top = 0,
+                                  cudaStream_t stream = nullptr) {
+    const size_t n = static_cast<size_t>(n_rows > 0 ? n_rows : 0);
+    const size_t col = detail::align256(n * sizeof(float));
+    const size_t m = n * static_cast<size_t>(n_top > 0 ? n_top : 0);
+    const size_t top = detail::align256(m * sizeof(float));
+    detail::ThreadState& st = detail::state();
+    unsigned char* d = static_cast<unsigned char*>(st.device_out(3 * col + 2 * top + 1));
+    int32_t* top_ids = m ? reinterpret_cast<int32_t*>(d + 3 * col) : nullptr;
+    float* top_logp = m ? reinterpret_cast<float*>(d + 3 * col + top) : nullptr;
+    detail::check(loom_token_logprobs(d_logits, LOOM_SELECT_F32, n_rows, n_vocab, row_stride, d_ids, temperature, n_top,
+                                      reinterpret_cast<float*>(d), reinterpret_cast<float*>(d + col), nullptr,
+                                      reinterpret_cast<int32_t*>(d + 2 * col), top_ids, top_logp, stream),
+                  "token_logprobs");
+    const unsigned char* h = static_cast<const unsigned char*>(detail::read_back(d, 3 * col + 2 * top, stream));
+    const float* f = reinterpret_cast<const float*>(h);
+    const int32_t* rank = reinterpret_cast<const int32_t*>(h + 2 * col);
+    TokenScores r;
+    r.logprob.assign(f, f + n);
+    r.entropy.assign(f + col / sizeof(float), f + col / sizeof(float) + n);
+    r.rank.assign(rank, rank + n);
+    const int32_t* ti = reinterpret_cast<const int32_t*>(h + 3 * col);
+    const float* tl = reinterpret_cast<const float*>(h + 3 * col + top);
+    r.top_ids.assign(ti, ti + m);
+    r.top_logprobs.assign(tl, tl + m);
+    return r;
+}
+
+// The end of a greedy step with the LM head in 8-bit integers: the final RMS norm of d_x [rows, hidden_dim] bf16 (plus
+// d_residual, when given, which becomes the sum), d_norm_weight [hidden_dim] f32; the product with d_weight [n_vocab,
+// hidden_dim] int8 and its scales d_weight_scale [n_vocab] (loom_quantize_rows_i8 makes both); then Generator::argmax
+// (src/core/generation.cpp:64-74) with its log-probability. A NaN never wins; a row of nothing else has id -1.
+// The logits are held in this thread's device memory (rows * n_vocab floats). Results on the host.
+inline GreedyResult lm_head_argmax_i8(const void* d_x, void* d_residual, const float* d_norm_weight, double eps,
+                                      const int8_t* d_weight, const float* d_weight_scale, int64_t rows,
+                                      int64_t hidden_dim, int64_t n_vocab, cudaStream_t stream = nullptr) {
+    if (rows <= 0 || hidden_dim <= 0 || n_vocab <= 0) detail::check(LOOM_SELECT_EINVAL, "lm_head_argmax_i8");
+    const size_t n = static_cast<size_t>(rows);
+    const size_t col = detail::align256(n * sizeof(float));
+    const size_t q_bytes = detail::align256(n * static_cast<size_t>(hidden_dim));
+    detail::ThreadState& st = detail::state();
+    void* ws = st.workspace(loom_lm_head_logits_i8_workspace_size(rows, n_vocab), stream);
+    // device: [ids] [log-probabilities] [log-sum-exps] [hidden scales] [8-bit hidden states] [logits]
+    unsigned char* d = static_cast<unsigned char*>(
+        st.device_out(4 * col + q_bytes + n * static_cast<size_t>(n_vocab) * sizeof(float)));
+    int32_t* ids = reinterpret_cast<int32_t*>(d);
+    float* logp = reinterpret_cast<float*>(d + col);
+    float* lse = reinterpret_cast<float*>(d + 2 * col);
+    float* scale = reinterpret_cast<float*>(d + 3 * col);
+    int8_t* q = reinterpret_cast<int8_t*>(d + 4 * col);
+    float* logits = reinterpret_cast<float*>(d + 4 * col + q_bytes);
+    detail::check(loom_rms_norm_i8(d_x, LOOM_SELECT_BF16, rows, hidden_dim, hidden_dim, d_residual, hidden_dim,
+                                   d_norm_weight, LOOM_SELECT_F32, eps, q, scale, d_residual, hidden_dim, stream),
+                  "lm_head_argmax_i8");
+    detail::check(loom_lm_head_logits_i8(q, scale, d_weight, d_weight_scale, rows, hidden_dim, n_vocab, logits,
+                                         LOOM_SELECT_F32, n_vocab, ws, st.workspace_size(), stream),
+                  "lm_head_argmax_i8");
+    detail::check(loom_token_logprobs(logits, LOOM_SELECT_F32, rows, n_vocab, n_vocab, nullptr, 1.0f, 1, nullptr,
+                                      nullptr, lse, nullptr, ids, logp, stream),
+                  "lm_head_argmax_i8");
+    const int status = loom_select_read_status(ws, stream);
+    if (status != LOOM_SELECT_OK) detail::check(status, "lm_head_argmax_i8");
+    const unsigned char* h = static_cast<const unsigned char*>(detail::read_back(d, 3 * col, stream));
+    GreedyResult r;
+    r.ids.assign(reinterpret_cast<const int32_t*>(h), reinterpret_cast<const int32_t*>(h) + n);
+    const float* hp = reinterpret_cast<const float*>(h + col);
+    const float* hl = reinterpret_cast<const float*>(h + 2 * col);
+    r.logprob.assign(hp, hp + n);
+    r.logit.resize(n);
+    for (size_t i = 0; i < n; ++i) r.logit[i] = hp[i] + hl[i];
     return r;
 }
 
