@@ -12,7 +12,7 @@
 // persistent CTA per SM. Warp 0 streams 128-byte K slices of both tiles into a shared-memory ring with TMA (128-byte
 // swizzle, a K tail filled with zeros), warp 1 issues tcgen05.mma kind::i8 (M 128, N NR, K 32) into one of two TMEM
 // accumulators, the other warps drain the other one, scale it and write the logits.
-// Calls of more than 128 rows work in pairs of CTAs (cta_group::2, M 256, N 256): each loads its own ids and half of the
+// Calls of more than 128 rows work in pairs of CTAs (cta_group::2, M 256, N 160 to 256): each loads its own ids and half of the
 // rows, so a stage brings 32 KiB into an SM for the work that a CTA by itself would fetch 48 KiB for -- at 64 bytes a
 // cycle from L2 that fetch, 768 cycles, and not the MMA's 512, is what bound it.
 // With one tile of rows, each CTA (or pair) takes an equal share of the ids, to 16 (a TMA box): 151936 ids are 1187.0
@@ -54,12 +54,13 @@ struct I8Tile {
     // halves too (four drain a 256-row tile too slowly: 256 us for [1024, 2048] x [151936, 2048], bf16 logits).
     static constexpr int kEpiWarps = NR >= 64 ? 8 : 4;
     static constexpr int kThreads = 64 + 32 * kEpiWarps;
-    static constexpr int kEpiCols = NR / (kEpiWarps / 4);  // rows a warp drains of a tile
-    static constexpr uint32_t kScaleBytes = kEpiWarps * kEpiCols * 4;  // their scales, a copy for each warp
+    static constexpr int kEpiCols = NR / (kEpiWarps / 4);  // rows a warp drains of a tile, 32 at a time
+    static constexpr int kEpiScales = (kEpiCols + 31) / 32 * 32;
+    static constexpr uint32_t kScaleBytes = kEpiWarps * kEpiScales * 4;  // their scales, a copy for each warp
     static constexpr int kFit = int((227u * 1024u - 2048u - kScaleBytes) / kStageBytes);
     static constexpr int kStages = kFit < 12 ? kFit : 12;
     static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kScaleBytes + 512 + 1024;
-    static constexpr uint32_t kTmemCols = 2 * NR < 32 ? 32 : 2 * NR;  // two accumulators
+    static constexpr uint32_t kTmemCols = NR <= 16 ? 32 : NR <= 64 ? 128 : NR <= 128 ? 256 : 512;  // two accumulators
     // Instruction descriptor, kind::i8: s32 accumulator (2), signed A and B (1), K-major, N >> 3, M >> 4.
     static constexpr uint32_t kIdesc =
         (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(NR >> 3) << 17) | (uint32_t(kCtas * kIds >> 4) << 24);
@@ -312,7 +313,7 @@ __global__ void __launch_bounds__(I8Tile<NR, kPair>::kThreads, 1)
     } else {
         // ---- epilogue: a warp reads TMEM lanes 32 * (warp % 4) .. + 31, one id per thread ----
         const int q = warp & 3, col0 = (warp - 2) / 4 * T::kEpiCols;
-        float* scale = scales + (warp - 2) * T::kEpiCols;
+        float* scale = scales + (warp - 2) * T::kEpiScales;
         int64_t scale_row = -1;  // the tile whose scales are in `scale`
         for (int i = 0; walk.step(a); ++i) {
             const int b = i & 1, u = i >> 1;
@@ -320,7 +321,7 @@ __global__ void __launch_bounds__(I8Tile<NR, kPair>::kThreads, 1)
             if (walk.row != scale_row) {
                 scale_row = walk.row;
                 __syncwarp();
-                for (int j = lane; j < T::kEpiCols; j += 32) scale[j] = row + j < a.rows ? __ldg(a.row_scale + row + j) : 0.0f;
+                for (int j = lane; j < T::kEpiScales; j += 32) scale[j] = row + j < a.rows ? __ldg(a.row_scale + row + j) : 0.0f;
                 __syncwarp();
             }
             const int64_t id = walk.id + q * 32 + lane;
@@ -422,6 +423,11 @@ int launch_i8_any(const void* hidden, const void* weight, const I8Args& a, int64
     if (a.rows <= 16) return launch_i8<16, false, kOut>(hidden, weight, a, hidden_dim, sms, stream);
     if (a.rows <= 64) return launch_i8<64, false, kOut>(hidden, weight, a, hidden_dim, sms, stream);
     if (a.rows <= 128) return launch_i8<128, false, kOut>(hidden, weight, a, hidden_dim, sms, stream);
+    // as few tiles of rows as there have to be, no higher than they have to be
+    const int64_t tiles = (a.rows + 255) / 256, high = (a.rows + tiles - 1) / tiles;
+    if (high <= 160) return launch_i8<160, true, kOut>(hidden, weight, a, hidden_dim, sms, stream);
+    if (high <= 192) return launch_i8<192, true, kOut>(hidden, weight, a, hidden_dim, sms, stream);
+    if (high <= 224) return launch_i8<224, true, kOut>(hidden, weight, a, hidden_dim, sms, stream);
     return launch_i8<256, true, kOut>(hidden, weight, a, hidden_dim, sms, stream);
 }
 

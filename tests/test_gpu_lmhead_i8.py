@@ -311,3 +311,11 @@ def test_chain_from_hidden_states_to_scored_tokens(rows):
     step_w = w_scale.double() * (0.5 + 1e-4)
     bound = step_q * head.double().abs().sum(dim=1) + y.abs().sum(dim=1, keepdim=True) * step_w + hidden * step_q * step_w
     assert ((logits.double() - full).abs() <= bound * (1 + 1e-5)).all()
+
+
+@pytest.mark.parametrize("rows", [130, 160, 161, 193, 224, 225, 257, 321, 400, 449, 513, 700])
+def test_product_row_tiles(rows):
+    """Every height of a tile of rows, one tile and several, with a last tile that is not full."""
+    q, qs, w, ws = _operands(rows, 160, 1500, rows)
+    out = ls.lm_head_logits_i8(q, qs, w, ws)
+    assert torch.equal(out, _product(q, qs, w, ws, torch.float32))
