@@ -101,6 +101,7 @@ struct LpShared {
     SoftAcc acc[kBlocks * kW];  // of each warp
     int32_t ahead[kBlocks * kW];
     int32_t part_cand[kBlocks];
+    float m, lns;              // the row's, from the warp that has them to the one with the alternatives
     uint64_t cand[kMaxCand];   // kMaxCand / C from each block
     uint64_t sorting[kMaxCand + 8];
     uint64_t part_list[kBlocks][32];
@@ -672,71 +673,97 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : 4) toke
             }
         }
     }
-    if (rank_in != 0 || warp != 0) return;  // (nothing of the other blocks' shared memory is read from here on)
-    if constexpr (kTop) {
-        if (!listed) {
-            // all in one row, padded, and each one's place is the number of larger ones
-            int n = 0;
-            const int most = LpShared<kW>::kMaxCand / C;
-            for (int b = 0; b < C; ++b) {
-                const int m = sh.part_cand[b];
-                for (int i = lane; i < m; i += 32) sh.sorting[n + i] = sh.cand[b * most + i];
-                n += m;
-            }
-            if (lane < 8) sh.sorting[n + lane] = 0;  // (below every key)
-            sh.list[0][lane] = 0;
-            __syncwarp();
-            for (int i = lane; i < n; i += 32) {
-                const uint64_t mine = sh.sorting[i];
-                int larger = 0;
-                for (int j = 0; j < n; j += 8) {
+    // (nothing of the other blocks' shared memory is read from here on)
+    constexpr int kLast = kTop && kW > 1 ? 1 : 0;  // the warp that finishes the row's sums; the first, the alternatives
+    if (rank_in != 0 || warp > kLast) return;
+    if (kTop && warp == 0 && !listed) {
+        // Each candidate's place is the number of larger ones. (They come in a part for each block: candidate i is in the
+        // part in whose counts' running sum it falls.)
+        const int most = LpShared<kW>::kMaxCand / C;
+        int end = lane < C ? sh.part_cand[lane] : 0;
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) larger += sh.sorting[j + q] > mine;
+        for (int o = 1; o < LpShared<kW>::kBlocks; o <<= 1) {
+            const int below = __shfl_up_sync(0xffffffffu, end, o);
+            if (lane >= o) end += below;
+        }
+        const int n = __shfl_sync(0xffffffffu, end, C - 1);
+        for (int i0 = 0; i0 < n; i0 += 32) {
+            const int i = i0 + lane;
+            int part = 0, start = 0;
+#pragma unroll
+            for (int b = 0; b + 1 < LpShared<kW>::kBlocks; ++b) {
+                const int e = __shfl_sync(0xffffffffu, end, b);
+                if (b + 1 < C && i >= e) {
+                    part = b + 1;
+                    start = e;
                 }
-                if (larger < p.n_top) sh.list[0][larger] = mine;
             }
-            __syncwarp();
-            key = sh.list[0][lane];
+            if (i < n) sh.sorting[i] = sh.cand[part * most + i - start];
         }
-    }
-    if constexpr (kW > 1) {
-        acc = soft_init();
-        ahead = 0;
-        for (int w = lane; w < C * kW; w += 32) {  // (at most two to a lane)
-            const SoftAcc other = sh.acc[w];
-            const float M = fmaxf(acc.m, other.m);
-            const SoftAcc x = soft_move(acc, M, p.c), y = soft_move(other, M, p.c);
-            acc = {M, x.s + y.s, x.a + y.a};
-            ahead += sh.ahead[w];
+        if (lane < 8) sh.sorting[n + lane] = 0;  // (below every key)
+        sh.list[0][lane] = 0;
+        __syncwarp();
+        for (int i = lane; i < n; i += 32) {
+            const uint64_t mine = sh.sorting[i];
+            int larger = 0;
+            for (int j = 0; j < n; j += 8) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) larger += sh.sorting[j + q] > mine;
+            }
+            if (larger < p.n_top) sh.list[0][larger] = mine;
         }
-        acc = soft_reduce(acc, 32, p.c);
-        ahead = __reduce_add_sync(0xffffffffu, ahead);
+        __syncwarp();
+        key = sh.list[0][lane];
     }
-
     // x / T by the reciprocal in two parts (an infinite x, the product with whose second part may be NaN, by the first)
     auto over_t = [&](float x) {
         return fabsf(x) <= FLT_MAX ? __fmaf_rn(x, p.inv_t, __fmul_rn(x, p.inv_t_lo)) : __fmul_rn(x, p.inv_t);
     };
-    const float lns = logf(acc.s);  // -inf for an empty row, NaN where a logit was NaN or +inf
-    const bool empty = acc.s == 0.0f;
-    if (lane == 0) {
-        const float lse = empty ? neg_inf() : over_t(acc.m) + lns;
-        if (p.out_lse) p.out_lse[row] = lse;
-        if (p.out_entropy) p.out_entropy[row] = empty ? quiet_nan() : lns - kLn2 * __fdiv_rn(acc.a, acc.s);
-        if (p.out_logp) {
-            float lp = over_t(__fsub_rn(xt, acc.m)) - lns;
-            if (empty || (!has && t >= 0)) lp = quiet_nan();
-            p.out_logp[row] = t < 0 ? 0.0f : lp;
+    float m = acc.m, lns = 0.0f;
+    if (warp == kLast) {
+        if constexpr (kW > 1) {
+            acc = soft_init();
+            ahead = 0;
+            for (int w = lane; w < C * kW; w += 32) {  // (at most two to a lane)
+                const SoftAcc other = sh.acc[w];
+                const float M = fmaxf(acc.m, other.m);
+                const SoftAcc x = soft_move(acc, M, p.c), y = soft_move(other, M, p.c);
+                acc = {M, x.s + y.s, x.a + y.a};
+                ahead += sh.ahead[w];
+            }
+            acc = soft_reduce(acc, 32, p.c);
+            ahead = __reduce_add_sync(0xffffffffu, ahead);
         }
-        if (p.out_rank) p.out_rank[row] = has && xt == xt ? ahead : -1;
+        m = acc.m;
+        lns = logf(acc.s);  // -inf for an empty row, NaN where a logit was NaN or +inf
+        const bool empty = acc.s == 0.0f;
+        if (lane == 0) {
+            if (kLast > 0) {
+                sh.m = m;
+                sh.lns = lns;
+            }
+            if (p.out_lse) p.out_lse[row] = empty ? neg_inf() : over_t(m) + lns;
+            if (p.out_entropy) p.out_entropy[row] = empty ? quiet_nan() : lns - kLn2 * __fdiv_rn(acc.a, acc.s);
+            if (p.out_logp) {
+                float lp = over_t(__fsub_rn(xt, m)) - lns;
+                if (empty || (!has && t >= 0)) lp = quiet_nan();
+                p.out_logp[row] = t < 0 ? 0.0f : lp;
+            }
+            if (p.out_rank) p.out_rank[row] = has && xt == xt ? ahead : -1;
+        }
     }
     if constexpr (kTop) {
+        if constexpr (kLast > 0) {
+            named_barrier(1, 64);
+            if (warp != 0) return;
+            m = sh.m;
+            lns = sh.lns;
+        }
         if (lane < p.n_top) {
-            const float v = rank_key_value(key);
             if (p.out_top_ids) p.out_top_ids[row * p.n_top + lane] = key ? rank_key_id(key) : -1;
             if (p.out_top_logp)
                 p.out_top_logp[row * p.n_top + lane] =
-                    empty || !key ? quiet_nan() : over_t(__fsub_rn(v, acc.m)) - lns;
+                    lns == neg_inf() || !key ? quiet_nan() : over_t(__fsub_rn(rank_key_value(key), m)) - lns;
         }
     }
 }
