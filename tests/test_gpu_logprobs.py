@@ -370,3 +370,23 @@ def test_grad_captured_into_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(d, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", [(1, 30011), (3, 151936), (200, 3001), (400, 20000)])
+def test_fewer_finite_ids_than_alternatives(rows, vocab, dtype):
+    """Constrained decoding: a handful of ids allowed, the alternatives run into the masked ones, lowest ids first."""
+    x, ids = _logits(rows, vocab, seed=rows, dtype=dtype)
+    keep = torch.rand(rows, vocab, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda") < 10.0 / vocab
+    keep.scatter_(1, ids.long()[:, None], True)
+    x.masked_fill_(~keep, -math.inf)
+    _check(x, ids, n_top=32)
+
+
+@pytest.mark.parametrize("rows,vocab", [(2, 151936), (300, 20000), (500, 2000)])
+def test_many_ties_at_the_threshold(rows, vocab):
+    """More equal values at the n_top-th place than the candidates' store holds: the lowest ids win."""
+    x, ids = _logits(rows, vocab, seed=rows, dtype=torch.bfloat16)
+    x.copy_((x / 4).round())
+    x[:, vocab // 3:vocab // 3 + 7] = 50.0
+    _check(x, ids, n_top=20)
