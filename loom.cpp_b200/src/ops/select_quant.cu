@@ -9,7 +9,8 @@
 // the order of the summation: f32 squares are exact there up to 2^-53, and the one rounding of inv to f32
 // comes out the same for any order but for about one row in 10^8. q is then the same bit for bit whatever
 // the launch shape, as the plain definition gives it.
-// Bound: HBM (rows read once: a thread keeps its elements in registers between the passes).
+// Bound: HBM (rows read once: a thread keeps its elements in registers between the passes). [16384, 4096] f32 with the
+// residual takes 127.5 us (6.8 TB/s), [16384, 2048] bf16 38.5 us (6.1 TB/s), one row 2.8 us.
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
@@ -51,13 +52,12 @@ template <int kWords>
 struct Around {
     static constexpr int kVecs = (kWords + 3) / 4 + 1;
     uint32_t w[4 * kVecs];
-    // Those of the vectors that hold something before `end` (the others are not touched).
-    __device__ __forceinline__ void load(const unsigned char* at, const unsigned char* end, bool there) {
-        const unsigned char* v = at - (reinterpret_cast<uintptr_t>(at) & 15);
+    __device__ __forceinline__ void load(const unsigned char* at, bool there) {
+        const uint4* v = reinterpret_cast<const uint4*>(at - (reinterpret_cast<uintptr_t>(at) & 15));
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
             uint4 r = make_uint4(0, 0, 0, 0);
-            if (there && v + 16 * i < end) r = reinterpret_cast<const uint4*>(v)[i];
+            if (there) r = v[i];
             w[4 * i] = r.x, w[4 * i + 1] = r.y, w[4 * i + 2] = r.z, w[4 * i + 3] = r.w;
         }
     }
@@ -74,56 +74,50 @@ struct Around {
     }
 };
 
-// Elements [id, id + kN) of a row of dim elements, zeros outside it. kAligned: the row begins at a vector and the run is
-// either whole or outside.
+// kN neighbouring elements of a whole run, as raw words; zeros where there is none. kAligned: the address is a multiple of
+// their size (at most 16 bytes). Otherwise the vectors around them lie in the same row (see kBefore); f32 runs of four go
+// word by word, which is quicker ([30000, 1037] with the residual 108 us, by vectors 142, as both then stood).
 template <int kDtype, int kN, bool kAligned>
-__device__ __forceinline__ void load_run(const unsigned char* base, int32_t id, int32_t dim, float (&x)[kN]) {
-    constexpr int kEsz = kDtype == LOOM_SELECT_BF16 ? 2 : 4;
-    constexpr int kWords = kN * kEsz / 4;
-    const unsigned char* at = base + int64_t(id) * kEsz;
-    uint32_t w[kWords];
+struct RunLoad {
+    static constexpr int kWords = kN * (kDtype == LOOM_SELECT_BF16 ? 2 : 4) / 4;
+    static constexpr bool kByWord = !kAligned && kDtype == LOOM_SELECT_F32 && kN == 4;
+    Around<kWords> around;  // (its first words are the run itself where it is not loaded around it)
+    const unsigned char* at;
+    __device__ __forceinline__ void load(const unsigned char* from, bool there) {
+        at = from;
+        if constexpr (!kAligned && !kByWord) {
+            around.load(at, there);
+        } else {
 #pragma unroll
-    for (int q = 0; q < kWords; ++q) w[q] = 0;
-    if constexpr (kAligned) {
-        if (id + kN <= dim) {
-            if constexpr (kWords == 2) {
+            for (int q = 0; q < kWords; ++q) around.w[q] = 0;
+            if (!there) return;
+            if constexpr (kByWord) {
+#pragma unroll
+                for (int q = 0; q < kWords; ++q) around.w[q] = reinterpret_cast<const uint32_t*>(at)[q];
+            } else if constexpr (kWords == 2) {
                 const uint2 r = *reinterpret_cast<const uint2*>(at);
-                w[0] = r.x, w[1] = r.y;
+                around.w[0] = r.x, around.w[1] = r.y;
             } else {
 #pragma unroll
                 for (int q = 0; q < kWords; q += 4) {
                     const uint4 r = *reinterpret_cast<const uint4*>(at + 4 * q);
-                    w[q] = r.x, w[q + 1] = r.y, w[q + 2] = r.z, w[q + 3] = r.w;
-                }
-            }
-        }
-    } else {
-        // f32 word by word, which is quicker for four of them ([30000, 1037] 108 us; by vectors 142); others by the vectors
-        // around the run where those lie in the row
-        constexpr bool kByWord = kDtype == LOOM_SELECT_F32 && kN == 4;
-        const unsigned char* lo = kByWord ? at : at - (reinterpret_cast<uintptr_t>(at) & 15);
-        const unsigned char* hi = kByWord ? at + 16 : lo + 16 * ((kWords + 3) / 4 + 1);
-        if (id < dim && lo >= base && hi <= base + int64_t(dim) * kEsz) {
-            if constexpr (kByWord) {
-#pragma unroll
-                for (int q = 0; q < kWords; ++q) w[q] = reinterpret_cast<const uint32_t*>(at)[q];
-            } else {
-                Around<kWords> around;
-                around.load(at, hi, true);
-                around.get(at, w);
-            }
-        } else {
-#pragma unroll
-            for (int q = 0; q < kN; ++q) {
-                if (id + q >= 0 && id + q < dim) {
-                    if constexpr (kDtype == LOOM_SELECT_BF16)
-                        w[q / 2] |= uint32_t(reinterpret_cast<const unsigned short*>(base)[id + q]) << (16 * (q % 2));
-                    else
-                        w[q] = reinterpret_cast<const uint32_t*>(base)[id + q];
+                    around.w[q] = r.x, around.w[q + 1] = r.y, around.w[q + 2] = r.z, around.w[q + 3] = r.w;
                 }
             }
         }
     }
+    __device__ __forceinline__ void get(uint32_t (&out)[kWords]) const {
+        if constexpr (!kAligned && !kByWord) {
+            around.get(at, out);
+        } else {
+#pragma unroll
+            for (int q = 0; q < kWords; ++q) out[q] = around.w[q];
+        }
+    }
+};
+
+template <int kDtype, int kWords, int kN>
+__device__ __forceinline__ void words_to_floats(const uint32_t (&w)[kWords], float (&x)[kN]) {
 #pragma unroll
     for (int q = 0; q < kWords; ++q) {
         if constexpr (kDtype == LOOM_SELECT_BF16) {
@@ -135,34 +129,28 @@ __device__ __forceinline__ void load_run(const unsigned char* base, int32_t id, 
     }
 }
 
-// The four words of a run to elements [id, id + 16 / element size) of a row of dim elements, those outside it left out.
-template <int kDtype, bool kAligned>
-__device__ __forceinline__ void store_run(unsigned char* base, int32_t id, int32_t dim, const uint32_t (&w)[4]) {
-    constexpr int kEsz = kDtype == LOOM_SELECT_BF16 ? 2 : 4;
-    constexpr int kPer = 16 / kEsz;
-    unsigned char* at = base + int64_t(id) * kEsz;
-    const bool whole = id >= 0 && id + kPer <= dim;
+// The four words of a whole run to any element-aligned address (kAligned: a multiple of 16).
+template <bool kAligned>
+__device__ __forceinline__ void store_run(unsigned char* at, const uint32_t (&w)[4]) {
     if constexpr (kAligned) {
-        if (whole) *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else if (whole && (reinterpret_cast<uintptr_t>(at) & 3) == 0) {
+        *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else if ((reinterpret_cast<uintptr_t>(at) & 2) == 0) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) reinterpret_cast<uint32_t*>(at)[q] = w[q];
-    } else if (whole) {  // bf16 between words
+    } else {  // bf16 between words
         *reinterpret_cast<unsigned short*>(at) = (unsigned short)w[0];
 #pragma unroll
         for (int q = 0; q < 3; ++q) *reinterpret_cast<uint32_t*>(at + 2 + 4 * q) = __funnelshift_r(w[q], w[q + 1], 16);
         *reinterpret_cast<unsigned short*>(at + 14) = (unsigned short)(w[3] >> 16);
-    } else {
-#pragma unroll
-        for (int q = 0; q < kPer; ++q) {
-            if (id + q >= 0 && id + q < dim) {
-                if constexpr (kDtype == LOOM_SELECT_BF16)
-                    reinterpret_cast<unsigned short*>(base)[id + q] = (unsigned short)(w[q / 2] >> (16 * (q % 2)));
-                else
-                    reinterpret_cast<uint32_t*>(base)[id + q] = w[q];
-            }
-        }
     }
+}
+
+template <int kDtype>
+__device__ __forceinline__ float load_one(const unsigned char* base, int32_t i) {
+    if constexpr (kDtype == LOOM_SELECT_BF16)
+        return __uint_as_float(uint32_t(reinterpret_cast<const unsigned short*>(base)[i]) << 16);
+    else
+        return reinterpret_cast<const float*>(base)[i];
 }
 
 // A thread's kPer elements in the rows' own type, four registers: f32 x 4 or bf16 x 8.
@@ -170,17 +158,7 @@ template <int kDtype>
 struct Held {
     static constexpr int kPer = kDtype == LOOM_SELECT_BF16 ? 8 : 4;
     uint32_t w[4];
-    __device__ __forceinline__ void get(float (&x)[kPer]) const {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            if constexpr (kDtype == LOOM_SELECT_BF16) {
-                x[2 * q] = __uint_as_float(w[q] << 16);
-                x[2 * q + 1] = __uint_as_float(w[q] & 0xffff0000u);
-            } else {
-                x[q] = __uint_as_float(w[q]);
-            }
-        }
-    }
+    __device__ __forceinline__ void get(float (&x)[kPer]) const { words_to_floats<kDtype>(w, x); }
     __device__ __forceinline__ void set(const float (&x)[kPer]) {  // rounds to the type
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -198,7 +176,12 @@ struct Held {
 // several of those a warp or less holds. All of a thread's loads are in flight together, and its elements stay in
 // registers. Runs are laid out by the output: run k covers ids [k kPer - lead, (k + 1) kPer - lead), where out_q's row
 // begins `lead` bytes after a multiple of kPer, so that a whole run is one store. kAligned: every row of every tensor
-// begins at a vector (lead is 0).
+// begins at a vector (lead is 0). Otherwise runs within kBefore elements of the row's start or kAfter of its end are
+// left to single elements, at most 30 of them, so that the vectors around the others' elements lie in the row. (With the
+// odd elements inside each run's code, the loads of one run waited for the branches of the one before: [8192, 5001]
+// bf16 120 us, this way 86, the bytes 44; [100000, 1501] bf16 quantised 137 and 94, the bytes 69.)
+constexpr int kBefore = 8, kAfter = 16;
+constexpr int kMaxEdge = 32;
 //
 // Resident threads per SM asked of the compiler: 1024 (64 registers) where it takes registers to keep the loads in flight,
 // 1536 (40) for the plain aligned quantiser, whose [151936, 2048] bf16 takes 132.5 us then (1024: 134.7; the bytes at
@@ -228,44 +211,39 @@ __global__ void __launch_bounds__(kTPR < 64 ? 128 : kTPR, min_blocks(kNorm, kAli
     unsigned char* out = reinterpret_cast<unsigned char*>(p.q + row * p.dim);
     const int32_t lead = kAligned ? 0 : int32_t(reinterpret_cast<uintptr_t>(out) % kPer);
     auto first = [&](int j) { return (j * kTPR + tid) * kPer - lead; };
-
-    // The runs of one tensor's row. Unaligned bf16 rows but for the tensor's first and last: all the vectors around the
-    // runs are requested before any is shifted (what they hold of the neighbouring rows is masked off).
-    const bool inner = !kAligned && kDtype == LOOM_SELECT_BF16 && row > 0 && row + 1 < p.rows;
-    auto load_row = [&](const unsigned char* base, Held<kDtype>(&to)[kVPT]) {
-        if (inner) {
-            Around<4> around[kVPT];
-#pragma unroll
-            for (int j = 0; j < kVPT; ++j)
-                around[j].load(base + int64_t(first(j)) * kEsz, base + int64_t(dim) * kEsz, first(j) < dim);
-#pragma unroll
-            for (int j = 0; j < kVPT; ++j) {
-                const int32_t id = first(j);
-                around[j].get(base + int64_t(id) * kEsz, to[j].w);
-                if (id < 0 || id + kPer > dim) {
-                    float v[kPer];
-                    to[j].get(v);
-#pragma unroll
-                    for (int q = 0; q < kPer; ++q) v[q] = id + q >= 0 && id + q < dim ? v[q] : 0.0f;
-                    to[j].set(v);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < kVPT; ++j) {
-                float v[kPer];
-                load_run<kDtype, kPer, kAligned>(base, first(j), dim, v);
-                to[j].set(v);
-            }
-        }
+    auto whole = [&](int j) {
+        return kAligned ? first(j) + kPer <= dim : first(j) >= kBefore && first(j) + kAfter <= dim;
     };
+    // the single elements: ids [0, edge0) and [edge1, dim)
+    constexpr int kEdge = kAligned ? 0 : (kMaxEdge + kTPR - 1) / kTPR;
+    int32_t edge0 = 0, edge1 = dim;
+    if constexpr (!kAligned) {
+        const int32_t k0 = (kBefore + lead + kPer - 1) / kPer, k1 = dim >= kAfter ? (dim - kAfter + lead) / kPer : -1;
+        edge0 = k1 < k0 ? dim : k0 * kPer - lead;
+        edge1 = k1 < k0 ? dim : (k1 + 1) * kPer - lead;
+    }
+    auto edge_id = [&](int i) {
+        const int32_t e = i * kTPR + tid;
+        return e < edge0 ? e : edge1 + (e - edge0);  // (dim or more: none)
+    };
+
     Held<kDtype> h[kVPT];
-    load_row(p.x + row * p.x_stride * kEsz, h);
+    float he[kEdge > 0 ? kEdge : 1];
+    auto load_row = [&](const unsigned char* base, Held<kDtype>(&to)[kVPT], float(&edge)[kEdge > 0 ? kEdge : 1]) {
+        RunLoad<kDtype, kPer, kAligned> run[kVPT];  // (all requested before the first is shifted)
+#pragma unroll
+        for (int j = 0; j < kVPT; ++j) run[j].load(base + int64_t(first(j)) * kEsz, whole(j));
+#pragma unroll
+        for (int i = 0; i < kEdge; ++i) edge[i] = edge_id(i) < dim ? load_one<kDtype>(base, edge_id(i)) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < kVPT; ++j) run[j].get(to[j].w);
+    };
+    load_row(p.x + row * p.x_stride * kEsz, h, he);
     if (kNorm && p.residual) {
-        const unsigned char* r = p.residual + row * p.residual_stride * kEsz;
         unsigned char* s = p.sum ? p.sum + row * p.sum_stride * kEsz : nullptr;
         Held<kDtype> add[kVPT];
-        load_row(r, add);
+        float add_e[kEdge > 0 ? kEdge : 1];
+        load_row(p.residual + row * p.residual_stride * kEsz, add, add_e);
 #pragma unroll
         for (int j = 0; j < kVPT; ++j) {
             float v[kPer], u[kPer];
@@ -274,7 +252,18 @@ __global__ void __launch_bounds__(kTPR < 64 ? 128 : kTPR, min_blocks(kNorm, kAli
 #pragma unroll
             for (int q = 0; q < kPer; ++q) v[q] = __fadd_rn(v[q], u[q]);
             h[j].set(v);
-            if (s) store_run<kDtype, kAligned>(s, first(j), dim, h[j].w);
+            if (s && whole(j)) store_run<kAligned>(s + int64_t(first(j)) * kEsz, h[j].w);
+        }
+#pragma unroll
+        for (int i = 0; i < kEdge; ++i) {
+            he[i] = __fadd_rn(he[i], add_e[i]);
+            if constexpr (kDtype == LOOM_SELECT_BF16) he[i] = __bfloat162float(__float2bfloat16_rn(he[i]));
+            if (s && edge_id(i) < dim) {
+                if constexpr (kDtype == LOOM_SELECT_BF16)
+                    reinterpret_cast<__nv_bfloat16*>(s)[edge_id(i)] = __float2bfloat16_rn(he[i]);
+                else
+                    reinterpret_cast<float*>(s)[edge_id(i)] = he[i];
+            }
         }
     }
     float inv = 0.0f;
@@ -287,6 +276,8 @@ __global__ void __launch_bounds__(kTPR < 64 ? 128 : kTPR, min_blocks(kNorm, kAli
 #pragma unroll
             for (int q = 0; q < kPer; ++q) ss = __fma_rn(double(v[q]), double(v[q]), ss);
         }
+#pragma unroll
+        for (int i = 0; i < kEdge; ++i) ss = __fma_rn(double(he[i]), double(he[i]), ss);
 #pragma unroll
         for (int o = (kTPR < 32 ? kTPR : 32) / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         // (64-bit division and square root by one warp: every warp's would take turns at the unit)
@@ -312,12 +303,20 @@ __global__ void __launch_bounds__(kTPR < 64 ? 128 : kTPR, min_blocks(kNorm, kAli
     auto make = [&](int j, float (&v)[kPer]) {
         h[j].get(v);
         if constexpr (kNorm) {
+            constexpr int kWEsz = kWDtype == LOOM_SELECT_BF16 ? 2 : 4;
+            RunLoad<kWDtype, kPer, kAligned> run;
+            run.load(p.weight + int64_t(first(j)) * kWEsz, whole(j));
+            uint32_t raw[kPer * kWEsz / 4];
+            run.get(raw);
             float w[kPer];
-            load_run<kWDtype, kPer, kAligned>(p.weight, first(j), dim, w);
+            words_to_floats<kWDtype>(raw, w);
 #pragma unroll
             for (int q = 0; q < kPer; ++q) v[q] = __fmul_rn(__fmul_rn(v[q], inv), w[q]);
         }
     };
+#pragma unroll
+    for (int i = 0; i < kEdge; ++i)
+        if (kNorm && edge_id(i) < dim) he[i] = __fmul_rn(__fmul_rn(he[i], inv), load_one<kWDtype>(p.weight, edge_id(i)));
     float y[kHoldY ? kVPT : 1][kPer];
     float a = 0.0f;
 #pragma unroll
@@ -330,6 +329,8 @@ __global__ void __launch_bounds__(kTPR < 64 ? 128 : kTPR, min_blocks(kNorm, kAli
             if constexpr (kHoldY) y[j][q] = v[q];
         }
     }
+#pragma unroll
+    for (int i = 0; i < kEdge; ++i) a = nan_max(a, fabsf(he[i]));
 #pragma unroll
     for (int o = (kTPR < 32 ? kTPR : 32) / 2; o > 0; o >>= 1) a = nan_max(a, __shfl_xor_sync(0xffffffffu, a, o));
     if constexpr (kWarps > 1) {
@@ -363,15 +364,15 @@ __global__ void __launch_bounds__(kTPR < 64 ? 128 : kTPR, min_blocks(kNorm, kAli
             w[k] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
             if (!some) w[k] = 0;  // (a NaN row's products are not numbers)
         }
-        const int32_t id = first(j);
-        if ((kAligned || id >= 0) && id + kPer <= dim) {
-            if constexpr (kPer == 8) *reinterpret_cast<uint2*>(out + id) = make_uint2(w[0], w[1]);
-            else *reinterpret_cast<uint32_t*>(out + id) = w[0];
-        } else if (!kAligned) {
-#pragma unroll
-            for (int q = 0; q < kPer; ++q)
-                if (id + q >= 0 && id + q < dim) out[id + q] = (unsigned char)(w[q / 4] >> (8 * (q % 4)));
+        if (whole(j)) {
+            if constexpr (kPer == 8) *reinterpret_cast<uint2*>(out + first(j)) = make_uint2(w[0], w[1]);
+            else *reinterpret_cast<uint32_t*>(out + first(j)) = w[0];
         }
+    }
+#pragma unroll
+    for (int i = 0; i < kEdge; ++i) {
+        const uint32_t b = __float_as_uint(__fadd_rn(__fmul_rn(he[i], inv_scale), kMagic));
+        if (edge_id(i) < dim) out[edge_id(i)] = some ? (unsigned char)b : (unsigned char)0;
     }
 }
 

@@ -120,6 +120,25 @@ def test_norm_alignment_strides_and_untouched_gaps(offset, extra, dim, dtype):
     assert _same(q2, _quantise(x.cpu().float())[0]) and _same(s2, _quantise(x.cpu().float())[1])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [*range(1, 50), 255, 257, 509, 1023, 4097])
+def test_every_small_width_unaligned(dim, dtype):
+    rows = 5
+    for offset in (1, 6):
+        x, res = _rows(rows, dim, dtype, 1, offset), _rows(rows, dim, dtype, 2, offset + 1, dim + 1)
+        w = _rows(1, dim, torch.float32, 3, offset)[0]
+        wq, ws, h = _norm(x, w, res, 1e-6)
+        q, scale, total = ls.rms_norm_i8(x, w, res)
+        assert _same(q, wq) and _same(scale, ws) and torch.equal(total.cpu(), h)
+        wq, ws = _quantise(x.cpu().float())
+        qbuf = torch.full((rows * dim + 40,), 99, dtype=torch.int8, device="cuda")
+        q = qbuf[offset + 2:offset + 2 + rows * dim].view(rows, dim)
+        ls.quantize_rows_i8_into(x, q, scale)
+        assert _same(q, wq) and _same(scale, ws)
+        q.fill_(99)
+        assert (qbuf == 99).all()
+
+
 @pytest.mark.parametrize("into", ["x", "residual"])
 def test_norm_in_place(into):
     x, res = _rows(5, 4096, torch.bfloat16, 1), _rows(5, 4096, torch.bfloat16, 2)
