@@ -648,7 +648,7 @@ def quantize_rows_i8(x, stream=None):
 _STATUS_WS = {}
 
 
-def _status_workspace(stream):
+def _status_buffer(stream):
     """The workspace of a call that needs only the status word: one per device, never replaced. A captured call
     gets one of its own (zeroed by the graph), which the graph's memory pool keeps."""
     torch = _torch()
@@ -656,13 +656,13 @@ def _status_workspace(stream):
         dev = torch.cuda.current_device()
         capturing = torch.cuda.is_current_stream_capturing()
         if not capturing and dev in _STATUS_WS:
-            return _STATUS_WS[dev]
+            return _STATUS_WS[dev].buf
         ws = Workspace(torch.device("cuda", dev))
         ws.get(256, stream)
         if not capturing:
             torch.cuda.current_stream().synchronize()  # zeroed before another stream's call reads it
             _STATUS_WS[dev] = ws
-    return ws
+    return ws.buf
 
 
 def lm_head_logits_i8_into(hidden, hidden_scale, weight, weight_scale, out, workspace=None, stream=None):
@@ -684,8 +684,7 @@ def lm_head_logits_i8_into(hidden, hidden_scale, weight, weight_scale, out, work
     if tuple(out.shape) != ((n_vocab,) if hidden.dim() == 1 else (rows, n_vocab)) or out.get_device() != dev:
         raise SelectError(EINVAL, "out must be [rows, n_vocab] on the hidden states' device")
     _, _, stride = _rows_view(out)
-    ws = workspace or _status_workspace(stream)
-    buf = ws.get(256, stream)
+    buf = workspace.get(256, stream) if workspace is not None else _status_buffer(stream)
     check(_lib().loom_lm_head_logits_i8(hidden.data_ptr(), hidden_scale.data_ptr(), weight.data_ptr(),
                                         weight_scale.data_ptr(), rows, hdim, n_vocab, out.data_ptr(), code, stride,
                                         buf.data_ptr(), buf.numel(), _raw_stream(stream, dev)),
