@@ -110,8 +110,8 @@ LOOM_SELECT_API int loom_select_read_status(void* workspace, void* stream);
 
 /*
  * Test hook, no loom.cpp counterpart: drives the bounded-wait failure path of the streamed kernels
- * (argmax of long rows, the sampler for top_k <= 128) and of loom_lm_head_argmax (where the withheld
- * stage is the first CTA's K slice number withhold_stage) without any fault. It writes into the
+ * (argmax of long rows, the sampler for top_k <= 128) and of loom_lm_head_argmax and loom_lm_head_logits_i8 (where the
+ * withheld stage is the first CTA's K slice number withhold_stage) without any fault. It writes into the
  * workspace header, on `stream`: wait_limit_ns (> 0) replaces the 2 s bound of every wait of those
  * kernels, and withhold_stage >= 0 makes the first CTA's producer leave that stage of its range
  * unissued, so its consumers' waits run out. The next such call records LOOM_SELECT_ETIMEOUT (its
@@ -350,8 +350,8 @@ LOOM_SELECT_API int loom_quantize_rows_i8(const void* x, int dtype, int64_t rows
  * stays as it was. The integer sum is exact, each product above is one f32 rounding: the logits do not depend on the
  * device or the launch. hidden [rows, hidden_dim] and weight [n_vocab, hidden_dim] (ggml's lm_head layout) are packed
  * and 16-byte aligned; hidden_dim is a multiple of 16, at most 65536 (LOOM_SELECT_ESHAPE otherwise). The workspace
- * holds only the status word read by loom_select_read_status (a bounded wait that gave up), so calls on several
- * streams may share it.
+ * (zeroed once, as all are) holds only the status word read by loom_select_read_status (a bounded wait that gave up), so
+ * calls on several streams may share it.
  */
 LOOM_SELECT_API size_t loom_lm_head_logits_i8_workspace_size(int64_t rows, int64_t n_vocab);
 LOOM_SELECT_API int loom_lm_head_logits_i8(const int8_t* hidden, const float* hidden_scale, const int8_t* weight,

@@ -188,7 +188,8 @@ def _rows_view(logits):
         return 1, logits.shape[0], logits.shape[0]
     if logits.dim() != 2 or logits.stride(1) != 1:
         raise SelectError(EINVAL, "logits must be [rows, n_vocab] with contiguous rows")
-    return logits.shape[0], logits.shape[1], logits.stride(0)
+    # (one row's stride may be anything)
+    return logits.shape[0], logits.shape[1], logits.shape[1] if logits.shape[0] == 1 else logits.stride(0)
 
 
 class Workspace:
@@ -483,7 +484,11 @@ def _addr(t):
 
 def _raw_stream(stream, dev):
     """The handle of `stream`, or of the device's current one (without making a Stream object for it)."""
-    return stream.cuda_stream if stream is not None else _torch()._C._cuda_getCurrentRawStream(dev)
+    if stream is None:
+        return _torch()._C._cuda_getCurrentRawStream(dev)
+    if stream.device_index != dev:
+        raise SelectError(EINVAL, f"the stream is of device {stream.device_index}, the tensors of {dev}")
+    return stream.cuda_stream
 
 
 def _on(stream):
@@ -582,7 +587,7 @@ def _matrix_view(t, name):
         return 1, t.shape[0], t.shape[0]
     if t.dim() != 2 or t.stride(1) != 1:
         raise SelectError(EINVAL, f"{name} must be [rows, dim] with contiguous rows")
-    return t.shape[0], t.shape[1], t.stride(0)
+    return t.shape[0], t.shape[1], t.shape[1] if t.shape[0] == 1 else t.stride(0)
 
 
 def rms_norm_i8_into(x, weight, out_q, out_scale, residual=None, out_sum=None, eps=1e-6, stream=None):

@@ -250,13 +250,15 @@ def test_product_offsets_past_32_bits():
     assert torch.equal(r.top_ids, ls.token_logprobs(out.contiguous(), None, n_top=4).top_ids)
 
 
-def test_wait_that_gives_up_is_reported():
-    """The bounded waits' give-up path, through the test hook (nothing faults); the next call is exact again."""
-    q, qs, w, ws = _operands(40, 512, 60000, 9)
+@pytest.mark.parametrize("rows", [40, 300])
+def test_wait_that_gives_up_is_reported(rows):
+    """The bounded waits' give-up path, through the test hook (nothing faults), of single CTAs and of pairs; the next
+    call is exact again."""
+    q, qs, w, ws = _operands(rows, 512, 60000, 9)
     want = _product(q, qs, w, ws, torch.float32)
     mine = ls.Workspace(torch.device("cuda", torch.cuda.current_device()))
     buf = mine.get(256)
-    out = torch.empty(40, 60000, device="cuda")
+    out = torch.empty(rows, 60000, device="cuda")
     ls.check(ls.lib().loom_select_test_wait_fault(ls._ptr(buf), 50_000, 2, ls._stream_handle()), "hook")
     ls.lm_head_logits_i8_into(q, qs, w, ws, out, workspace=mine)
     assert mine.read_status() == ls.ETIMEOUT
@@ -264,6 +266,17 @@ def test_wait_that_gives_up_is_reported():
     ls.lm_head_logits_i8_into(q, qs, w, ws, out, workspace=mine)
     assert mine.read_status() == ls.OK
     assert torch.equal(out, want)
+
+
+def test_one_row_of_any_stride():
+    """A row's own stride means nothing when there is one: views that torch gives an odd one are taken."""
+    q, qs, w, ws = _operands(1, 256, 500, 4)
+    out = torch.empty(500, 1, device="cuda").t()
+    ls.lm_head_logits_i8_into(q, qs, w, ws, out)
+    assert torch.equal(out, _product(q, qs, w, ws, torch.float32))
+    x = torch.randn(64, 1, device="cuda").t()
+    assert _same(ls.quantize_rows_i8(x)[0], ls.quantize_rows_i8(x.contiguous())[0])
+    assert torch.equal(ls.token_logprobs(out).lse, ls.token_logprobs(out.contiguous()).lse)
 
 
 def test_two_streams_and_two_graphs_at_once():
