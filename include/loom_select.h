@@ -289,7 +289,8 @@ LOOM_SELECT_API int loom_lm_head_argmax(const void* hidden, const void* weight, 
  * Every output may be NULL, not all of them; ids may be NULL when out_logp and out_rank are. n_top is 0 .. min(V,
  * LOOM_SELECT_MAX_TOP_LOGPROBS), positive exactly when one of out_top_ids and out_top_logp is given. T is a
  * positive, finite, normal float (LOOM_SELECT_EPARAM otherwise, as for n_top out of range). Log-probabilities are
- * accurate to 1e-5 absolute or relative, whichever is larger. The comparisons are exact: -0 == +0.
+ * accurate to 3.6e-5 absolute, by the bound on every rounding (1e-6 as measured), besides 2^-22 of their own size. The
+ * comparisons are exact: -0 == +0. An out_lse beyond f32's range (the lowest finite values over T < 1) is infinite.
  *   - A negative id means "no token in this row" (padding): out_logp = 0, out_rank = -1, the rest as usual.
  *     An id >= V: out_logp = NaN, out_rank = -1.
  *   - -inf logits have probability 0 (masked ids). A row of nothing else: out_lse = -inf, out_logp, out_entropy and
@@ -311,7 +312,7 @@ LOOM_SELECT_API int loom_token_logprobs(const void* logits, int dtype, int64_t r
  * grad_logp or grad_entropy may be NULL (all zeros), not both; entropy may be NULL without grad_entropy, ids without
  * grad_logp. A negative id takes no part (its grad_logp counts as 0), an id >= V with a non-zero grad_logp makes its
  * row NaN. A row whose two weights are 0 gets zeros, whatever its logits hold; otherwise a row whose lse is NaN or
- * -inf gets NaN. -inf logits get 0. out_grad rows are grad_stride >= V elements apart; out_grad may be the logits
+ * infinite gets NaN. -inf logits get 0. out_grad rows are grad_stride >= V elements apart; out_grad may be the logits
  * themselves (same pointer, same stride: LOOM_SELECT_EINVAL otherwise), and must not overlap them in another way.
  * No workspace, no atomics: the result does not depend on timing.
  */

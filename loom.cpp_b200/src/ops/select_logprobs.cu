@@ -8,7 +8,7 @@
 // maximum rises (A moves with m: sum e^(y - M)(y - M) = f (A + (m - M) S), f = e^(m - M)). Everything is
 // held in f32: A <= 0 <= ln S, so H has no cancellation, and a thread adds at most a few thousand terms.
 // Bound: HBM (each logit read once) for many rows, [1024, 151936] f32 in 110.7 us (5.6 TB/s; 95.9 without rank and
-// alternatives); the latency of a row's end, some ten dependent steps, for few: 9.7 us for one row of 151936.
+// alternatives); the latency of a row's end, some ten dependent steps, for few: 8.5 us for one row of 151936.
 #include <cfloat>
 #include <cmath>
 #include <cooperative_groups.h>
@@ -440,11 +440,14 @@ __device__ __forceinline__ void block_sync() {
 // Four blocks of eight warps to an SM (64 registers). Blocks of four warps: 121.8 us for [1024, 151936] f32 and 68.4 for
 // [256, 262144] bf16, of eight 115.1 and 51.3, of sixteen 131.2 and 52.5. Narrow rows go a warp to a row, four rows to a
 // block, six blocks to an SM ([16384, 1025] f32 30.2 us; four blocks 35.8, eight 37.8).
-template <int kDtype, bool kTop, int kW>
-__global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : 4) token_logprobs_kernel(const LpDev p) {
+// kU: vectors per thread and step. Four ([1024, 151936] f32 110.9 us; two: 129.8, five: 117.2, eight: 123.7); eight where
+// every block has an SM to itself and two such steps or more to read (1 row of 151936 f32 8.5 us, with four 9.6, 18 rows
+// 10.1 and 10.9; with less to read, one of 51865 bf16 7.8 and 7.3, 18 of 151936 bf16 10.5 and 9.9).
+template <int kDtype, bool kTop, int kW, int kU>
+__global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8 ? 2 : 4)
+    token_logprobs_kernel(const LpDev p) {
     constexpr int kEsz = kDtype == LOOM_SELECT_BF16 ? 2 : 4;
     constexpr int kPer = 16 / kEsz;
-    constexpr int kU = 4;                // vectors per thread and step
     constexpr int kNT = kW * 32;
     constexpr int kRows = kW == 1 ? 4 : 1;
     __shared__ LpShared<kW> sh_of_row[kRows];
@@ -785,7 +788,7 @@ int lp_cluster(int64_t rows, int64_t n_vocab, int sms) {
     return c;
 }
 
-template <int kDtype, bool kTop, int kW>
+template <int kDtype, bool kTop, int kW, int kU>
 cudaError_t launch_lp(const LpDev& p, int64_t rows, int C, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(kW == 1 ? (rows + 3) / 4 : rows * C));
@@ -797,13 +800,16 @@ cudaError_t launch_lp(const LpDev& p, int64_t rows, int C, cudaStream_t s) {
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<kDtype, kTop, kW>, p);
+    return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<kDtype, kTop, kW, kU>, p);
 }
 
 template <int kDtype, bool kTop>
 cudaError_t launch_lp_any(const LpDev& p, int64_t rows, int sms, cudaStream_t s) {
-    if (p.width <= kShort || (p.width <= kNarrow && rows >= sms)) return launch_lp<kDtype, kTop, 1>(p, rows, 1, s);
-    return launch_lp<kDtype, kTop, kLpWarps>(p, rows, lp_cluster(rows, p.width, sms), s);
+    if (p.width <= kShort || (p.width <= kNarrow && rows >= sms)) return launch_lp<kDtype, kTop, 1, 4>(p, rows, 1, s);
+    const int C = lp_cluster(rows, p.width, sms);
+    constexpr int64_t kWide = int64_t(8) * kLpWarps * 32 * (kDtype == LOOM_SELECT_BF16 ? 8 : 4);  // a block's step, kU = 8
+    if (rows * C <= sms && p.width >= 2 * C * kWide) return launch_lp<kDtype, kTop, kLpWarps, 8>(p, rows, C, s);
+    return launch_lp<kDtype, kTop, kLpWarps, 4>(p, rows, C, s);
 }
 
 // ---- the gradient ----
