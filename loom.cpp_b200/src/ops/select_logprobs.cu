@@ -7,7 +7,7 @@
 // One pass over the logits: each thread keeps (m, S, A) of its elements and rescales S and A when its
 // maximum rises (A moves with m: sum e^(y - M)(y - M) = f (A + (m - M) S), f = e^(m - M)). Everything is
 // held in f32: A <= 0 <= ln S, so H has no cancellation, and a thread adds at most a few thousand terms.
-// Bound: HBM (each logit read once) for many rows, [1024, 151936] f32 in 110.7 us (5.6 TB/s; 95.9 without rank and
+// Bound: HBM (each logit read once) for many rows, [1024, 151936] f32 in 102.7 us (6.1 TB/s; 93.5 without rank and
 // alternatives); the latency of a row's end, some ten dependent steps, for few: 8.5 us for one row of 151936.
 #include <cfloat>
 #include <cmath>
@@ -86,12 +86,14 @@ struct LpDev {
 constexpr int kSlots = 16;
 static_assert(kSlots <= 32, "a thread's slots are bits of a word");
 constexpr int kMaxCluster = 8;
-constexpr int kGroups = 64;  // (32 in a block of one warp)
+constexpr int kGroups = 64;  // (32 where a row is one warp's)
+// Warps to a row: 8 in each block of a cluster, 4 (a block to a row), or 1 (four rows to a block).
+constexpr int kLpWarps = 8, kLpRowWarps = 4;
 
 template <int kW>
 struct LpShared {
-    static constexpr int kMaxCand = kW == 1 ? 256 : 512;
-    static constexpr int kBlocks = kW == 1 ? 1 : kMaxCluster;
+    static constexpr int kMaxCand = kW == kLpWarps ? 512 : 256;
+    static constexpr int kBlocks = kW == kLpWarps ? kMaxCluster : 1;
     uint64_t list[kW][32];
     alignas(16) uint32_t group[kGroups];  // order keys of the maxima of the cluster's groups of threads
     uint32_t x_key;            // order key of the threshold
@@ -437,14 +439,16 @@ __device__ __forceinline__ void block_sync() {
 // elements of the row reach, and few more do (64 -ln(1 - n / 64): 24 for 20). The slots whose maximum reaches it are
 // read again, from L2, and those elements sorted by counting the larger ones.
 //
-// Four blocks of eight warps to an SM (64 registers). Blocks of four warps: 121.8 us for [1024, 151936] f32 and 68.4 for
-// [256, 262144] bf16, of eight 115.1 and 51.3, of sixteen 131.2 and 52.5. Narrow rows go a warp to a row, four rows to a
-// block, six blocks to an SM ([16384, 1025] f32 30.2 us; four blocks 35.8, eight 37.8).
-// kU: vectors per thread and step. Four ([1024, 151936] f32 110.9 us; two: 129.8, five: 117.2, eight: 123.7); eight where
-// every block has an SM to itself and two such steps or more to read (1 row of 151936 f32 8.5 us, with four 9.6, 18 rows
-// 10.1 and 10.9; with less to read, one of 51865 bf16 7.8 and 7.3, 18 of 151936 bf16 10.5 and 9.9).
+// Thirty-two warps to an SM (64 registers). Where there are rows for every place of such blocks of eight warps, blocks of
+// four take a row each, with a row's end among more rows' streams and less lost to the last wave: [1024, 151936] f32 102.7 us
+// (eight warps: 111.1), [600, 51864] bf16 28.7 (33.7), [3000, 32000] bf16 78.0 (91.8), of two warps 150.1, 46.3 and 97.2.
+// With fewer rows blocks of eight, in clusters: [256, 262144] bf16 43.6 us, four warps 53.6. Narrow rows go a warp to a
+// row, four rows to a block, six blocks to an SM ([16384, 1025] f32 30.2 us; four blocks 35.8, eight 37.8).
+// kU: vectors per thread and step. Four ([1024, 151936] f32 102.8 us; three: 106.9, five: 106.1); eight where every block
+// has an SM to itself and two such steps or more to read (1 row of 151936 f32 8.4 us, with four 9.6, 18 rows 10.1 and 10.9;
+// with less to read, one of 51865 bf16 7.8 and 7.3, 18 of 151936 bf16 10.5 and 9.9).
 template <int kDtype, bool kTop, int kW, int kU>
-__global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8 ? 2 : 4)
+__global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8 ? 2 : 32 / kW)
     token_logprobs_kernel(const LpDev p) {
     constexpr int kEsz = kDtype == LOOM_SELECT_BF16 ? 2 : 4;
     constexpr int kPer = 16 / kEsz;
@@ -453,7 +457,7 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
     __shared__ LpShared<kW> sh_of_row[kRows];
     LpShared<kW>& sh = sh_of_row[kW == 1 ? threadIdx.x / 32 : 0];
     const cg::cluster_group cluster = cg::this_cluster();
-    const int C = kW == 1 ? 1 : int(cluster.num_blocks()), rank_in = kW == 1 ? 0 : int(cluster.block_rank());
+    const int C = kW == kLpWarps ? int(cluster.num_blocks()) : 1, rank_in = kW == kLpWarps ? int(cluster.block_rank()) : 0;
     const int tid = threadIdx.x % (kW * 32), lane = tid & 31, warp = tid >> 5;
     const int64_t row = kW == 1 ? int64_t(blockIdx.x) * kRows + threadIdx.x / 32 : blockIdx.x / unsigned(C);
     if (kW == 1 && row >= p.rows) return;
@@ -777,10 +781,9 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
 
 // Blocks per row: doubled, up to 8 (a portable cluster), while there are fewer than two a SM and more than one step of 16
 // elements a thread in each one's share. More blocks read faster, but each has its end to go through: [256, 262144] bf16
-// 51.3 us with two blocks a row, 53.8 with four, [77, 51865] bf16 13.4 and 18.6.
-constexpr int kLpWarps = 8;
-// A warp to a row, where there are rows for every SM: [8000, 8000] f32 67 us (a block to a row: 113), [700, 2048] 6.7 (11.8),
-// [1500, 16000] 35.7 (34.5). Very short rows always.
+// 43.6 us with two blocks a row, 48.1 with four, [77, 51865] bf16 12.4 and 16.2.
+// A warp to a row, where there are rows for every SM: [8000, 8000] f32 65.5 us (four warps to a row: 76.6), bf16 57.6 (81.2),
+// [2000, 5000] f32 16.4 (20.6). Very short rows always.
 constexpr int32_t kNarrow = 8192, kShort = 512;
 int lp_cluster(int64_t rows, int64_t n_vocab, int sms) {
     int c = 1;
@@ -806,6 +809,7 @@ cudaError_t launch_lp(const LpDev& p, int64_t rows, int C, cudaStream_t s) {
 template <int kDtype, bool kTop>
 cudaError_t launch_lp_any(const LpDev& p, int64_t rows, int sms, cudaStream_t s) {
     if (p.width <= kShort || (p.width <= kNarrow && rows >= sms)) return launch_lp<kDtype, kTop, 1, 4>(p, rows, 1, s);
+    if (rows > 4 * int64_t(sms)) return launch_lp<kDtype, kTop, kLpRowWarps, 4>(p, rows, 1, s);
     const int C = lp_cluster(rows, p.width, sms);
     constexpr int64_t kWide = int64_t(8) * kLpWarps * 32 * (kDtype == LOOM_SELECT_BF16 ? 8 : 4);  // a block's step, kU = 8
     if (rows * C <= sms && p.width >= 2 * C * kWide) return launch_lp<kDtype, kTop, kLpWarps, 8>(p, rows, C, s);

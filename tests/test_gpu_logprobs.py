@@ -159,6 +159,22 @@ def test_few_long_rows(dtype, offset):
         _check(x, ids, T=0.9, n_top=n_top)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,offset", [(700, 8193, 0), (640, 12007, 3), (1201, 20000, 1)])
+def test_many_rows(rows, vocab, offset, dtype):
+    """Rows enough for every block of the device, some of them masked, tied, empty or with their token at the ends."""
+    x, ids = _logits(rows, vocab, seed=rows, dtype=dtype, offset=offset, stride=vocab + offset)
+    x[0::7] = x[0::7].round().clamp(-2, 2)
+    x[1::7, 40:] = -math.inf
+    x[2::49, :] = -math.inf
+    x[3::7, ::3] = -math.inf
+    x[4::7, 3:] = -math.inf
+    x[5::49, :] = torch.finfo(dtype).min
+    ids[::5], ids[1::5], ids[2::25] = 0, vocab - 1, -1
+    for n_top in (0, 7, 32):
+        _check(x, ids, T=1.0, n_top=n_top)
+
+
 def test_ids_outside_the_vocabulary():
     x, ids = _logits(4, 1000, seed=2)
     ids[0], ids[1], ids[2] = -1, -100, 1000
