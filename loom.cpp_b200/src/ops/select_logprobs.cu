@@ -371,8 +371,8 @@ struct LpShare {
     float X;
 };
 
-// The elements that the lanes in `hits` have in slot `slot` (each lane's own), spread over the warp 32 at a time: f gets a
-// value and its id, NaN where there is none, in all lanes. Four lanes' elements are requested together. A loop with
+// The elements that the lanes in `hits` have in slot `slot` (each lane's own), spread over the warp 32 at a time: f gets
+// four values and their ids, NaN where there is none, in all lanes. Four lanes' elements are requested together. A loop with
 // little code: unrolled over a thread's own elements, instruction fetches made this 7000 cycles and not 1500.
 template <int kDtype, int kU, int kNT, class F>
 __device__ __forceinline__ void visit(const LpShare& r, uint32_t hits, int32_t slot, F&& f) {
@@ -391,6 +391,7 @@ __device__ __forceinline__ void visit(const LpShare& r, uint32_t hits, int32_t s
             const int e = e0 + lane;
             const int32_t skip = e / (kU * kPer) * r.stride + e / kPer % kU * kNT;
             float x[4];
+            int32_t id[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int32_t v = first[k] + skip;
@@ -398,7 +399,8 @@ __device__ __forceinline__ void visit(const LpShare& r, uint32_t hits, int32_t s
                                                              : quiet_nan();
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) f(x[k], (first[k] + skip) * kPer - r.shift + e % kPer);
+            for (int k = 0; k < 4; ++k) id[k] = (first[k] + skip) * kPer - r.shift + e % kPer;
+            f(x, id);
         }
     }
 }
@@ -412,10 +414,15 @@ __device__ __noinline__ uint64_t list_slots(const LpShare& r, LpShared<kW>* sh) 
     float own = neg_inf();
     for (int32_t s = 0; s < r.slots; ++s) {
         const uint32_t hits = __ballot_sync(0xffffffffu, sh->slot_max[warp][s][lane] >= fmaxf(r.X, own));
-        visit<kDtype, kU, kW * 32>(r, hits, s, [&](float x, int32_t id) {
-            const uint64_t cand = x >= r.X ? loom_rank_key(x, id) : 0ull;
-            if (__any_sync(0xffffffffu, cand > __shfl_sync(0xffffffffu, key, r.n_top - 1)))
-                key = merge_lists(key, sort_desc(cand));
+        visit<kDtype, kU, kW * 32>(r, hits, s, [&](const float(&x)[4], const int32_t(&id)[4]) {
+#pragma unroll 1
+            for (int k = 0; k < 4; ++k) {
+                const float xk = k == 0 ? x[0] : k == 1 ? x[1] : k == 2 ? x[2] : x[3];
+                const int32_t ik = k == 0 ? id[0] : k == 1 ? id[1] : k == 2 ? id[2] : id[3];
+                const uint64_t cand = xk >= r.X ? loom_rank_key(xk, ik) : 0ull;
+                if (__any_sync(0xffffffffu, cand > __shfl_sync(0xffffffffu, key, r.n_top - 1)))
+                    key = merge_lists(key, sort_desc(cand));
+            }
         });
         // a later slot's ids are above all earlier ones: only a larger value can displace the list's last
         const uint64_t last = __shfl_sync(0xffffffffu, key, r.n_top - 1);
@@ -513,8 +520,9 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
     const float xt = has ? load_global_elem<kDtype>(rowp, t) : quiet_nan();
     const bool rank = p.out_rank != nullptr && has;
 
-    float top = neg_inf(), slot_top = neg_inf();  // this thread's maximum, and its maximum in the current slot
-    int32_t slot = 0, in_slot = 0;
+    float slot_top = neg_inf();  // this thread's maximum in the current slot
+    float* slot_at = &sh.slot_max[warp][0][lane];
+    int32_t left = per_slot;  // steps of that slot to come
     auto step = [&](const uint4(&raw)[kU], int32_t at) {
         const float mx = largest<kDtype>(raw);
         st.add(raw, mx, at > whole);
@@ -523,12 +531,11 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
                      (at + (kU - 1) * kNT + 32) * kPer - shift, xt, t);
         if constexpr (kTop) {
             slot_top = fmaxf(slot_top, mx);
-            if (++in_slot == per_slot || at + stride >= v1) {
-                sh.slot_max[warp][slot][lane] = slot_top;
-                top = fmaxf(top, slot_top);
+            if (--left == 0) {
+                *slot_at = slot_top;
+                slot_at += 32;
                 slot_top = neg_inf();
-                ++slot;
-                in_slot = 0;
+                left = per_slot;
             }
         }
     };
@@ -541,6 +548,10 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
         step(raw_b, v);
         v += stride;
     }
+    if (kTop && left != per_slot) {
+        *slot_at = slot_top;
+        slot_at += 32;
+    }
     if (warp == 0 && rank_in == 0) {
         if (ex > st.acc.m) st.acc = soft_move(st.acc, ex, p.c);
         st.add_one(ex, st.acc.s, st.acc.a);
@@ -548,6 +559,8 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
     }
     LpShared<kW>* first = C > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
 
+    // this thread's maximum (none: s is 0, or NaN, as nothing above -FLT_MAX shows)
+    const float top = st.acc.m > -FLT_MAX || st.acc.s > 0.0f ? st.acc.m : neg_inf();
     // softmax state and rank of the warp, and the maxima of the groups of threads
     SoftAcc acc = soft_reduce(st.acc, 32, p.c);
     int32_t ahead = __reduce_add_sync(0xffffffffu, st.ahead);
@@ -556,12 +569,13 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
         first->acc[rank_in * kW + warp] = acc;
         first->ahead[rank_in * kW + warp] = ahead;
     }
-    LpShare r{rowp, shift, v_start, v1, stride, per_slot, slot, p.n_top, 0.0f};
+    const int32_t slots = int32_t(slot_at - &sh.slot_max[warp][0][lane]) / 32;
+    LpShare r{rowp, shift, v_start, v1, stride, per_slot, slots, p.n_top, 0.0f};
     if constexpr (kTop) {
         // the threshold: the n_top-th largest of the groups' maxima
         constexpr int kG = kW == 1 ? 32 : kGroups;
         const int threads = C * kNT / kG;  // of one group: 1 to 32 neighbours
-        float most_top = fmaxf(top, ex);
+        float most_top = top;
         for (int o = 1; o < threads; o <<= 1) most_top = fmaxf(most_top, __shfl_xor_sync(0xffffffffu, most_top, o));
         if ((lane & (threads - 1)) == 0) {
             const uint32_t k = loom_order_key(most_top);
@@ -586,17 +600,19 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
                 }
             }
         } else {
-            if (tid < kG) {
-                const uint32_t mine = sh.group[tid];
-                int larger = 0;
+            constexpr int kPerKey = kNT / kG;  // threads that count the larger ones of one maximum together
+            const int i = tid / kPerKey;
+            const uint32_t mine = sh.group[i];
+            int larger = 0;
 #pragma unroll 2
-                for (int j = 0; j < kG; j += 4) {
-                    const uint4 o = *reinterpret_cast<const uint4*>(&sh.group[j]);
-                    larger += (o.x > mine || (o.x == mine && j < tid)) + (o.y > mine || (o.y == mine && j + 1 < tid)) +
-                              (o.z > mine || (o.z == mine && j + 2 < tid)) + (o.w > mine || (o.w == mine && j + 3 < tid));
-                }
-                if (larger == p.n_top - 1) sh.x_key = mine;
+            for (int j = tid % kPerKey * 4; j < kG; j += kPerKey * 4) {
+                const uint4 o = *reinterpret_cast<const uint4*>(&sh.group[j]);
+                larger += (o.x > mine || (o.x == mine && j < i)) + (o.y > mine || (o.y == mine && j + 1 < i)) +
+                          (o.z > mine || (o.z == mine && j + 2 < i)) + (o.w > mine || (o.w == mine && j + 3 < i));
             }
+#pragma unroll
+            for (int o = 1; o < kPerKey; o <<= 1) larger += __shfl_xor_sync(0xffffffffu, larger, o);
+            if (larger == p.n_top - 1) sh.x_key = mine;
             block_sync<kW>();
             x_key = sh.x_key;
         }
@@ -604,20 +620,31 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
         // the elements that reach it, to the first block
         const int most = LpShared<kW>::kMaxCand / C;
         uint64_t* to = first->cand + rank_in * most;
-        auto add = [&](float x, int32_t id) {
-            const uint32_t b = __ballot_sync(0xffffffffu, x >= r.X);
-            if (b == 0) return;
+        auto add = [&](const float(&x)[4], const int32_t(&id)[4]) {
+            uint32_t b[4];
+            int n = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                b[k] = __ballot_sync(0xffffffffu, x[k] >= r.X);
+                n += __popc(b[k]);
+            }
+            if (n == 0) return;
             int at = 0;
-            if (lane == 0) at = atomicAdd(&sh.n_cand, __popc(b));
-            at = __shfl_sync(0xffffffffu, at, 0) + __popc(b & ((1u << lane) - 1u));
-            if (x >= r.X && at < most) to[at] = loom_rank_key(x, id);
+            if (lane == 0) at = atomicAdd(&sh.n_cand, n);
+            at = __shfl_sync(0xffffffffu, at, 0);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int here = at + __popc(b[k] & ((1u << lane) - 1u));
+                if (x[k] >= r.X && here < most) to[here] = loom_rank_key(x[k], id[k]);
+                at += __popc(b[k]);
+            }
         };
         // (a threshold of -inf lets everything through: to the lists at once, in every block alike)
         const bool all = r.X == neg_inf();
         if (all && tid == 0) sh.overflow = 1;
         uint32_t mine = 0;  // this thread's slots whose maximum does
 #pragma unroll 4
-        for (int32_t s = 0; s < slot && !all; ++s) mine |= uint32_t(sh.slot_max[warp][s][lane] >= r.X) << s;
+        for (int32_t s = 0; s < slots && !all; ++s) mine |= uint32_t(sh.slot_max[warp][s][lane] >= r.X) << s;
         if constexpr (kW == 1) {
             // most lanes have some (n_top of 32): each looks through its own
             for (; mine; mine &= mine - 1) {
@@ -652,7 +679,10 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
                 visit<kDtype, kU, kNT>(r, hits, s, add);
             }
         }
-        if (warp == 0 && rank_in == 0 && !all) add(eid >= 0 ? ex : quiet_nan(), eid);
+        if (!all && eid >= 0 && ex >= r.X) {  // (eid: of lanes of the first warp of the first block only)
+            const int at = atomicAdd(&sh.n_cand, 1);
+            if (at < most) to[at] = loom_rank_key(ex, eid);
+        }
         block_sync<kW>();
         if (tid == 0) {
             const int n = sh.n_cand;
