@@ -7,8 +7,8 @@
 // One pass over the logits: each thread keeps (m, S, A) of its elements and rescales S and A when its
 // maximum rises (A moves with m: sum e^(y - M)(y - M) = f (A + (m - M) S), f = e^(m - M)). Everything is
 // held in f32: A <= 0 <= ln S, so H has no cancellation, and a thread adds at most a few thousand terms.
-// Bound: HBM (each logit read once) for many rows, [1024, 151936] f32 in 102.7 us (6.1 TB/s; 93.5 without rank and
-// alternatives); the latency of a row's end, some ten dependent steps, for few: 8.5 us for one row of 151936.
+// Bound: HBM (each logit read once) for many rows, [1024, 151936] f32 in 100.0 us (6.2 TB/s; 93.5 without rank and
+// alternatives); the latency of a row's end, some ten dependent steps, for few: 8.0 us for one row of 151936.
 #include <cfloat>
 #include <cmath>
 #include <cooperative_groups.h>
@@ -90,23 +90,27 @@ constexpr int kGroups = 64;  // (32 where a row is one warp's)
 // Warps to a row: 8 in each block of a cluster, 4 (a block to a row), or 1 (four rows to a block).
 constexpr int kLpWarps = 8, kLpRowWarps = 4;
 
-template <int kW>
+template <int kW, bool kTop>
 struct LpShared {
-    static constexpr int kMaxCand = kW == kLpWarps ? 512 : 256;
+    static constexpr int kMaxCand = !kTop ? 1 : kW == kLpWarps ? 512 : 256;
+    static constexpr int kSlotsHere = kTop ? kSlots : 1;
     static constexpr int kBlocks = kW == kLpWarps ? kMaxCluster : 1;
     uint64_t list[kW][32];
     alignas(16) uint32_t group[kGroups];  // order keys of the maxima of the cluster's groups of threads
     uint32_t x_key;            // order key of the threshold
     int32_t n_cand;            // elements of this block that reach it
     int32_t overflow;          // some block of the cluster has more of them than it may hand on
-    float slot_max[kW][kSlots][32];
+    union {  // (sorted once the slots have been looked through)
+        float slot_max[kW][kSlotsHere][32];
+        uint64_t sorting[kMaxCand + 8];
+    };
+    float edge[32];            // the elements apart from the vectors (the first block's)
     // of the cluster's first block: what the blocks hand on
     SoftAcc acc[kBlocks * kW];  // of each warp
     int32_t ahead[kBlocks * kW];
     int32_t part_cand[kBlocks];
     float m, lns;              // the row's, from the warp that has them to the one with the alternatives
     uint64_t cand[kMaxCand];   // kMaxCand / C from each block
-    uint64_t sorting[kMaxCand + 8];
     uint64_t part_list[kBlocks][32];
 };
 
@@ -229,7 +233,7 @@ struct LpScan {
     static constexpr int kPer = kDtype == LOOM_SELECT_BF16 ? 8 : 4;
     SoftAcc acc;
     float c;         // log2(e) / T
-    float mc, r, g;  // rn(m c), what its rounding lost, 2^-r
+    float mc;        // rn(m c)
     bool slow;
     int32_t ahead;
 
@@ -237,10 +241,21 @@ struct LpScan {
         acc = soft_init();
         c = c_;
         mc = -neg_inf();  // (until there is a maximum, the common path gives NaN)
-        r = 0.0f;
-        g = 1.0f;
         slow = false;
         ahead = 0;
+    }
+
+    // A maximum above the last one.
+    __device__ __forceinline__ void rise(float mx) {
+        acc = soft_move(acc, mx, c);
+        mc = __fmul_rn(mx, c);
+        slow = slow || !(fabsf(mc) <= 65536.0f);
+    }
+
+    // One element apart from the vectors.
+    __device__ __forceinline__ void add_edge(float x) {
+        if (x > acc.m) rise(x);
+        add_one(x, acc.s, acc.a);
     }
 
     // Two elements per instruction (f32x2). The common path takes 2^(x c - rn(m c)), one fused operation, one ex2 and
@@ -248,13 +263,7 @@ struct LpScan {
     // product with the exponent is NaN), a NaN, or a maximum so large that rounding m c loses much send the thread
     // to the other path from then on: (x - m) c, clamped. `partial`: some elements are not there.
     __device__ __forceinline__ void add(const uint4 (&raw)[kU], float mx, bool partial) {
-        if (mx > acc.m) {
-            acc = soft_move(acc, mx, c);
-            mc = __fmul_rn(mx, c);
-            r = __fmaf_rn(mx, c, -mc);
-            g = exp2f(-r);
-            slow = slow || !(fabsf(mc) <= 65536.0f);
-        }
+        if (mx > acc.m) rise(mx);
         float s, a;
         bool clamped = slow || partial;
         if (!clamped) {
@@ -278,6 +287,7 @@ struct LpScan {
             unpack2(s2, s0, s1);
             unpack2(a2, a0, a1);
             s = s0 + s1;
+            const float r = __fmaf_rn(acc.m, c, -mc), g = ex2(-r);  // what rounding m c lost
             a = __fmaf_rn(-r, s, a0 + a1) * g;
             s *= g;
             clamped = slow = a != a;
@@ -408,7 +418,7 @@ __device__ __forceinline__ void visit(const LpShare& r, uint32_t hits, int32_t s
 // The warp's best 32 of its elements >= X, sorted, when too many of them reach X to be held (a row of few
 // values, or of almost nothing but -inf).
 template <int kDtype, int kU, int kW>
-__device__ __noinline__ uint64_t list_slots(const LpShare& r, LpShared<kW>* sh) {
+__device__ __noinline__ uint64_t list_slots(const LpShare& r, LpShared<kW, true>* sh) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32 % kW;
     uint64_t key = 0;
     float own = neg_inf();
@@ -431,6 +441,11 @@ __device__ __noinline__ uint64_t list_slots(const LpShare& r, LpShared<kW>* sh) 
     return key;
 }
 
+// Up to this width, and for more than 8 alternatives, the lanes of a row's one warp look through their own slots, of few
+// elements and most of them hit ([16384, 1025] f32 with 20 45.3 us, by the warp together 63.5; [8000, 8000] bf16 70.1 and
+// 65.8; with 5 [700, 2048] f32 8.6 and 7.7).
+constexpr int32_t kOwnSlots = 4096;
+
 template <int kW>
 __device__ __forceinline__ void block_sync() {
     if constexpr (kW == 1) __syncwarp();
@@ -446,23 +461,23 @@ __device__ __forceinline__ void block_sync() {
 // elements of the row reach, and few more do (64 -ln(1 - n / 64): 24 for 20). The slots whose maximum reaches it are
 // read again, from L2, and those elements sorted by counting the larger ones.
 //
-// Thirty-two warps to an SM (64 registers). Where there are rows for every place of such blocks of eight warps, blocks of
-// four take a row each, with a row's end among more rows' streams and less lost to the last wave: [1024, 151936] f32 102.7 us
-// (eight warps: 111.1), [600, 51864] bf16 28.7 (33.7), [3000, 32000] bf16 78.0 (91.8), of two warps 150.1, 46.3 and 97.2.
-// With fewer rows blocks of eight, in clusters: [256, 262144] bf16 43.6 us, four warps 53.6. Narrow rows go a warp to a
-// row, four rows to a block, six blocks to an SM ([16384, 1025] f32 30.2 us; four blocks 35.8, eight 37.8).
-// kU: vectors per thread and step. Four ([1024, 151936] f32 102.8 us; three: 106.9, five: 106.1); eight where every block
-// has an SM to itself and two such steps or more to read (1 row of 151936 f32 8.4 us, with four 9.6, 18 rows 10.1 and 10.9;
+// Blocks of eight warps, in clusters where there are few rows: four to an SM ([256, 262144] bf16 41.5 us, four warps 50.2).
+// Where there are rows for all of them, blocks of four take a row each, with a row's end among more rows' streams and less
+// lost to the last wave: [1024, 151936] f32 100.0 us (eight warps 111.1, two 150.1), [600, 51864] bf16 25.0 (33.7). Seven of
+// them to an SM (72 registers; eight, of 64, 101.1 and 26.9, [3000, 32000] bf16 71.9 where seven take 64.8), and seven of
+// four rows a warp each ([8000, 8000] f32 53.6 us, six 62.4).
+// kU: vectors per thread and step. Four ([1024, 151936] f32 102.8 us as it then was; three: 106.9, five: 106.1); eight where every block
+// has an SM to itself and two such steps or more to read (1 row of 151936 f32 8.4 us as it then was, with four 9.6, 18 rows 10.1 and 10.9;
 // with less to read, one of 51865 bf16 7.8 and 7.3, 18 of 151936 bf16 10.5 and 9.9).
 template <int kDtype, bool kTop, int kW, int kU>
-__global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8 ? 2 : 32 / kW)
+__global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 7 : kU == 8 ? 2 : kW == 4 ? 7 : 4)
     token_logprobs_kernel(const LpDev p) {
     constexpr int kEsz = kDtype == LOOM_SELECT_BF16 ? 2 : 4;
     constexpr int kPer = 16 / kEsz;
     constexpr int kNT = kW * 32;
     constexpr int kRows = kW == 1 ? 4 : 1;
-    __shared__ LpShared<kW> sh_of_row[kRows];
-    LpShared<kW>& sh = sh_of_row[kW == 1 ? threadIdx.x / 32 : 0];
+    __shared__ LpShared<kW, kTop> sh_of_row[kRows];
+    LpShared<kW, kTop>& sh = sh_of_row[kW == 1 ? threadIdx.x / 32 : 0];
     const cg::cluster_group cluster = cg::this_cluster();
     const int C = kW == kLpWarps ? int(cluster.num_blocks()) : 1, rank_in = kW == kLpWarps ? int(cluster.block_rank()) : 0;
     const int tid = threadIdx.x % (kW * 32), lane = tid & 31, warp = tid >> 5;
@@ -475,7 +490,6 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
     const int32_t nv = (shift + p.width + kPer - 1) / kPer;
     const int32_t v0 = shift ? 1 : 0;                      // first vector inside the row
     const int32_t v1 = max((shift + p.width) / kPer, v0);  // end of those inside it
-    const int32_t limit = v1 * kPer - shift;  // (an id past the whole vectors may be inside the row: an edge's)
     const unsigned char* vec = rowp - shift * kEsz;
     const int32_t stride = C * kU * kNT;
     const int32_t steps = (v1 - v0 + stride - 1) / stride;
@@ -483,10 +497,10 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
 
     // A step's vectors for this lane; in a step that the row's end cuts, those past it are -inf throughout.
     const int32_t v_start = v0 + rank_in * kU * kNT + warp * 32;
-    const int32_t whole = v1 - (kU - 1) * kNT - 32;  // a warp's step at v is whole when v <= this
+    auto whole = [&](int32_t v) { return v + (kU - 1) * kNT + 32 <= v1; };  // (the warp's step at v)
     auto load = [&](uint4(&raw)[kU], int32_t v) {
         const unsigned char* at = vec + int64_t(v + lane) * 16;
-        if (v <= whole) {
+        if (whole(v)) {
 #pragma unroll
             for (int u = 0; u < kU; ++u) raw[u] = ldg_stream_v4(at + u * kNT * 16);
         } else {
@@ -501,16 +515,14 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
     int32_t v = v_start;
     uint4 raw_a[kU], raw_b[kU];  // the step being added and the next one, whose loads are in flight
     if (v < v1) load(raw_a, v);
-    // the elements of the vectors that the row only partly fills, at most one to a lane of the first warp: those
-    // of the first in lanes 0 .. kPer - 1, those of the last in kPer .. 2 kPer - 1
-    float ex = neg_inf();
-    int32_t eid = -1;
-    if (warp == 0 && rank_in == 0) {
-        if (lane < kPer && v0 > 0) eid = lane - shift;
-        if (lane >= kPer && lane < 2 * kPer && v1 < nv && nv - 1 >= v0) eid = (nv - 1) * kPer - shift + lane - kPer;
-        if (eid >= p.width) eid = -1;
-        if (eid >= 0) ex = load_global_elem<kDtype>(rowp, eid);
-    }
+    // the elements of the vectors that the row only partly fills, at most one to a lane of the cluster's first warp: those
+    // of the first in lanes 0 .. kPer - 1, those of the last in kPer .. 2 kPer - 1; -1: none
+    auto edge_id = [&] {
+        int32_t id = -1;
+        if (lane < kPer && v0 > 0) id = lane - shift;
+        if (lane >= kPer && lane < 2 * kPer && v1 < nv && nv - 1 >= v0) id = (nv - 1) * kPer - shift + lane - kPer;
+        return warp == 0 && rank_in == 0 && id < p.width ? id : -1;
+    };
     if (tid == 0) sh.n_cand = sh.overflow = 0;
     if (C > 1) cluster.barrier_arrive();  // (waited for before the first remote store: all blocks have begun)
 
@@ -519,15 +531,22 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
     const bool has = t >= 0 && t < p.width;
     const float xt = has ? load_global_elem<kDtype>(rowp, t) : quiet_nan();
     const bool rank = p.out_rank != nullptr && has;
+    if (warp == 0 && rank_in == 0) {
+        const int32_t id = edge_id();
+        const float x = id >= 0 ? load_global_elem<kDtype>(rowp, id) : neg_inf();
+        st.add_edge(x);
+        st.ahead += rank && id >= 0 && (x > xt || (x == xt && id < t));
+        if (kTop) sh.edge[lane] = x;
+    }
 
     float slot_top = neg_inf();  // this thread's maximum in the current slot
     float* slot_at = &sh.slot_max[warp][0][lane];
     int32_t left = per_slot;  // steps of that slot to come
     auto step = [&](const uint4(&raw)[kU], int32_t at) {
         const float mx = largest<kDtype>(raw);
-        st.add(raw, mx, at > whole);
+        st.add(raw, mx, !whole(at));
         if (rank)
-            st.count(raw, mx, (at + lane) * kPer - shift, kNT * kPer, limit, at * kPer - shift,
+            st.count(raw, mx, (at + lane) * kPer - shift, kNT * kPer, v1 * kPer - shift, at * kPer - shift,
                      (at + (kU - 1) * kNT + 32) * kPer - shift, xt, t);
         if constexpr (kTop) {
             slot_top = fmaxf(slot_top, mx);
@@ -552,12 +571,7 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
         *slot_at = slot_top;
         slot_at += 32;
     }
-    if (warp == 0 && rank_in == 0) {
-        if (ex > st.acc.m) st.acc = soft_move(st.acc, ex, p.c);
-        st.add_one(ex, st.acc.s, st.acc.a);
-        st.ahead += rank && eid >= 0 && (ex > xt || (ex == xt && eid < t));
-    }
-    LpShared<kW>* first = C > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
+    LpShared<kW, kTop>* first = C > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
 
     // this thread's maximum (none: s is 0, or NaN, as nothing above -FLT_MAX shows)
     const float top = st.acc.m > -FLT_MAX || st.acc.s > 0.0f ? st.acc.m : neg_inf();
@@ -618,7 +632,7 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
         }
         r.X = order_key_to_float(x_key);
         // the elements that reach it, to the first block
-        const int most = LpShared<kW>::kMaxCand / C;
+        const int most = LpShared<kW, kTop>::kMaxCand / C;
         uint64_t* to = first->cand + rank_in * most;
         auto add = [&](const float(&x)[4], const int32_t(&id)[4]) {
             uint32_t b[4];
@@ -645,7 +659,8 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
         uint32_t mine = 0;  // this thread's slots whose maximum does
 #pragma unroll 4
         for (int32_t s = 0; s < slots && !all; ++s) mine |= uint32_t(sh.slot_max[warp][s][lane] >= r.X) << s;
-        if constexpr (kW == 1) {
+        const bool own = kW == 1 && p.n_top > 8 && p.width <= kOwnSlots;
+        if (own) {
             // most lanes have some (n_top of 32): each looks through its own
             for (; mine; mine &= mine - 1) {
                 int32_t v = v_start + lane + (__ffs(mine) - 1) * per_slot * stride;
@@ -679,9 +694,9 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
                 visit<kDtype, kU, kNT>(r, hits, s, add);
             }
         }
-        if (!all && eid >= 0 && ex >= r.X) {  // (eid: of lanes of the first warp of the first block only)
+        if (const int32_t id = edge_id(); !all && id >= 0 && sh.edge[lane] >= r.X) {
             const int at = atomicAdd(&sh.n_cand, 1);
-            if (at < most) to[at] = loom_rank_key(ex, eid);
+            if (at < most) to[at] = loom_rank_key(sh.edge[lane], id);
         }
         block_sync<kW>();
         if (tid == 0) {
@@ -700,7 +715,10 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
         listed = sh.overflow != 0;
         if (listed) {  // too many to hand on: each warp sorts its own, then lists by halves, warps and blocks
             key = list_slots<kDtype, kU, kW>(r, &sh);
-            if (warp == 0) key = merge_lists(key, sort_desc(eid >= 0 && ex >= r.X ? loom_rank_key(ex, eid) : 0ull));
+            if (warp == 0) {
+                const int32_t id = edge_id();
+                key = merge_lists(key, sort_desc(id >= 0 && sh.edge[lane] >= r.X ? loom_rank_key(sh.edge[lane], id) : 0ull));
+            }
             for (int h = kW / 2; h > 0; h >>= 1) {
                 if (warp >= h && warp < 2 * h) sh.list[warp][lane] = key;
                 block_sync<kW>();
@@ -720,10 +738,10 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
     if (kTop && warp == 0 && !listed) {
         // Each candidate's place is the number of larger ones. (They come in a part for each block: candidate i is in the
         // part in whose counts' running sum it falls.)
-        const int most = LpShared<kW>::kMaxCand / C;
+        const int most = LpShared<kW, kTop>::kMaxCand / C;
         int end = lane < C ? sh.part_cand[lane] : 0;
 #pragma unroll
-        for (int o = 1; o < LpShared<kW>::kBlocks; o <<= 1) {
+        for (int o = 1; o < LpShared<kW, kTop>::kBlocks; o <<= 1) {
             const int below = __shfl_up_sync(0xffffffffu, end, o);
             if (lane >= o) end += below;
         }
@@ -732,7 +750,7 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
             const int i = i0 + lane;
             int part = 0, start = 0;
 #pragma unroll
-            for (int b = 0; b + 1 < LpShared<kW>::kBlocks; ++b) {
+            for (int b = 0; b + 1 < LpShared<kW, kTop>::kBlocks; ++b) {
                 const int e = __shfl_sync(0xffffffffu, end, b);
                 if (b + 1 < C && i >= e) {
                     part = b + 1;
@@ -812,8 +830,11 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 6 : kU == 8
 // Blocks per row: doubled, up to 8 (a portable cluster), while there are fewer than two a SM and more than one step of 16
 // elements a thread in each one's share. More blocks read faster, but each has its end to go through: [256, 262144] bf16
 // 43.6 us with two blocks a row, 48.1 with four, [77, 51865] bf16 12.4 and 16.2.
-// A warp to a row, where there are rows for every SM: [8000, 8000] f32 65.5 us (four warps to a row: 76.6), bf16 57.6 (81.2),
-// [2000, 5000] f32 16.4 (20.6). Very short rows always.
+// A warp to a row, where its row is short beside the number of rows: those up to 1024 wide for a row or more to an SM
+// ([2000, 800] f32 9.2 us, four warps to a row 17.0), to 2048 for four ([700, 2048] bf16 9.9 and 9.2, [1000, 2048] 10.1
+// and 11.4), to 8192 for fourteen ([1300, 8000] bf16 25.3 and 19.1, [8000, 8000] 66.1 and 92.6); very short rows always.
+// Four warps to a row, up to 8192 wide, for more rows than SMs ([200, 8000] bf16 8.0 us, by clusters 11.2), and any with more
+// than four to an SM; with fewer, long rows go by clusters ([590, 32000] f32 21.5 us, four warps 23.4).
 constexpr int32_t kNarrow = 8192, kShort = 512;
 int lp_cluster(int64_t rows, int64_t n_vocab, int sms) {
     int c = 1;
@@ -838,8 +859,9 @@ cudaError_t launch_lp(const LpDev& p, int64_t rows, int C, cudaStream_t s) {
 
 template <int kDtype, bool kTop>
 cudaError_t launch_lp_any(const LpDev& p, int64_t rows, int sms, cudaStream_t s) {
-    if (p.width <= kShort || (p.width <= kNarrow && rows >= sms)) return launch_lp<kDtype, kTop, 1, 4>(p, rows, 1, s);
-    if (rows > 4 * int64_t(sms)) return launch_lp<kDtype, kTop, kLpRowWarps, 4>(p, rows, 1, s);
+    const int64_t per_sm = p.width <= 1024 ? 1 : p.width <= 2048 ? 4 : 14;
+    if (p.width <= kShort || (p.width <= kNarrow && rows >= per_sm * sms)) return launch_lp<kDtype, kTop, 1, 4>(p, rows, 1, s);
+    if (rows > (p.width <= kNarrow ? 1 : 4) * int64_t(sms)) return launch_lp<kDtype, kTop, kLpRowWarps, 4>(p, rows, 1, s);
     const int C = lp_cluster(rows, p.width, sms);
     constexpr int64_t kWide = int64_t(8) * kLpWarps * 32 * (kDtype == LOOM_SELECT_BF16 ? 8 : 4);  // a block's step, kU = 8
     if (rows * C <= sms && p.width >= 2 * C * kWide) return launch_lp<kDtype, kTop, kLpWarps, 8>(p, rows, C, s);

@@ -160,7 +160,8 @@ def test_few_long_rows(dtype, offset):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("rows,vocab,offset", [(700, 8193, 0), (640, 12007, 3), (1201, 20000, 1)])
+@pytest.mark.parametrize("rows,vocab,offset", [(160, 3001, 1), (151, 8000, 0), (700, 8193, 0), (640, 12007, 3),
+                                               (1201, 20000, 1)])
 def test_many_rows(rows, vocab, offset, dtype):
     """Rows enough for every block of the device, some of them masked, tied, empty or with their token at the ends."""
     x, ids = _logits(rows, vocab, seed=rows, dtype=dtype, offset=offset, stride=vocab + offset)
