@@ -466,11 +466,13 @@ __device__ __forceinline__ void block_sync() {
 // lost to the last wave: [1024, 151936] f32 100.0 us (eight warps 111.1, two 150.1), [600, 51864] bf16 25.0 (33.7). Seven of
 // them to an SM (72 registers; eight, of 64, 101.1 and 26.9, [3000, 32000] bf16 71.9 where seven take 64.8), and seven of
 // four rows a warp each ([8000, 8000] f32 53.6 us, six 62.4).
-// kU: vectors per thread and step. Four ([1024, 151936] f32 102.8 us as it then was; three: 106.9, five: 106.1); eight where every block
-// has an SM to itself and two such steps or more to read (1 row of 151936 f32 8.4 us as it then was, with four 9.6, 18 rows 10.1 and 10.9;
-// with less to read, one of 51865 bf16 7.8 and 7.3, 18 of 151936 bf16 10.5 and 9.9).
+// kU: vectors per thread and step. Four ([1024, 151936] f32 102.8 us as it then was; three: 106.9, five: 106.1). Eight where
+// every block has an SM to itself and two such steps or more to read (then 1 row of 151936 f32 8.4 us, with four 9.6, 18
+// rows 10.1 and 10.9; with less to read, one of 51865 bf16 7.8 and 7.3, 18 of 151936 bf16 10.5 and 9.9). Two for a warp's
+// row of at most two such steps, eight blocks to an SM ([20000, 300] bf16 without alternatives 15.6 us, with four 21.0;
+// [20000, 800] f32 23.5 and 19.9).
 template <int kDtype, bool kTop, int kW, int kU>
-__global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kW == 1 ? 7 : kU == 8 ? 2 : kW == 4 ? 7 : 4)
+__global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kU == 2 ? 8 : kU == 8 ? 2 : kW < 8 ? 7 : 4)
     token_logprobs_kernel(const LpDev p) {
     constexpr int kEsz = kDtype == LOOM_SELECT_BF16 ? 2 : 4;
     constexpr int kPer = 16 / kEsz;
@@ -860,7 +862,11 @@ cudaError_t launch_lp(const LpDev& p, int64_t rows, int C, cudaStream_t s) {
 template <int kDtype, bool kTop>
 cudaError_t launch_lp_any(const LpDev& p, int64_t rows, int sms, cudaStream_t s) {
     const int64_t per_sm = p.width <= 1024 ? 1 : p.width <= 2048 ? 4 : 14;
-    if (p.width <= kShort || (p.width <= kNarrow && rows >= per_sm * sms)) return launch_lp<kDtype, kTop, 1, 4>(p, rows, 1, s);
+    if (p.width <= kShort || (p.width <= kNarrow && rows >= per_sm * sms)) {
+        constexpr int kStep = 2 * 32 * (kDtype == LOOM_SELECT_BF16 ? 8 : 4);  // a warp's step, kU = 2
+        if (p.width <= 2 * kStep) return launch_lp<kDtype, kTop, 1, 2>(p, rows, 1, s);
+        return launch_lp<kDtype, kTop, 1, 4>(p, rows, 1, s);
+    }
     if (rows > (p.width <= kNarrow ? 1 : 4) * int64_t(sms)) return launch_lp<kDtype, kTop, kLpRowWarps, 4>(p, rows, 1, s);
     const int C = lp_cluster(rows, p.width, sms);
     constexpr int64_t kWide = int64_t(8) * kLpWarps * 32 * (kDtype == LOOM_SELECT_BF16 ? 8 : 4);  // a block's step, kU = 8
