@@ -97,15 +97,15 @@ struct I8Walk {
     int64_t id, id_end;
     int64_t tile_end;  // the end of the tile's ids, both CTAs'
     int64_t row;
-    int64_t next, end;  // one tile of rows: units of ids; several: tiles
+    uint32_t next, end;  // one tile of rows: units of ids; several: tiles (fewer than 2^31, in 32 bits: a division each)
     __device__ __forceinline__ explicit I8Walk(const I8Args& a) {
-        const int64_t worker = blockIdx.x / kCtas, workers = gridDim.x / kCtas;
+        const uint32_t worker = blockIdx.x / kCtas, workers = gridDim.x / kCtas;
         if (a.r_tiles == 1) {
-            next = a.units * worker / workers;
-            end = a.units * (worker + 1) / workers;
+            next = uint32_t(a.units * worker / workers);
+            end = uint32_t(a.units * (worker + 1) / workers);
         } else {
             next = worker;
-            end = a.v_tiles * a.r_tiles;
+            end = uint32_t(a.v_tiles * a.r_tiles);
         }
     }
     __device__ __forceinline__ bool step(const I8Args& a) {
@@ -113,14 +113,15 @@ struct I8Walk {
         int64_t past;
         if (a.r_tiles == 1) {
             constexpr int kUnits = kCtas * kIds / kUnit;
-            id = next * kUnit;
+            id = int64_t(next) * kUnit;
             next = next + kUnits < end ? next + kUnits : end;
-            past = next * kUnit;
+            past = int64_t(next) * kUnit;
             row = 0;
         } else {
-            id = next / a.r_tiles * (kCtas * kIds);
+            const uint32_t v = next / uint32_t(a.r_tiles);
+            id = int64_t(v) * (kCtas * kIds);
             past = id + kCtas * kIds;
-            row = next % a.r_tiles * NR;
+            row = int64_t(next - v * uint32_t(a.r_tiles)) * NR;
             next += gridDim.x / kCtas;
         }
         tile_end = past < a.n_vocab ? past : a.n_vocab;
@@ -224,9 +225,13 @@ __global__ void __launch_bounds__(I8Tile<NR, kPair>::kThreads, 1)
     I8Walk<NR, kPair> walk(a);
 
     if (warp == 0) {
-        if (lane == 0) {
+        if (elect_one()) {
             // ---- producer ----
+            // (stage and parity are counted along: dividing the slice's number cost 300 cycles a slice, [1, 2048] x
+            // [151936, 2048] 59 us and [12000, 8192] 47)
             int64_t kc = 0;
+            int s = 0;
+            uint32_t round = 0;  // the ring's passes so far, of which the last bit is the parity
             const int64_t withheld = (blockIdx.x == 0 && wf.withhold > 0) ? int64_t(wf.withhold) - 1 : -1;
             bool ok = true;
             while (ok && walk.step(a)) {
@@ -237,15 +242,13 @@ __global__ void __launch_bounds__(I8Tile<NR, kPair>::kThreads, 1)
                     const int peer = walk.boxes(a, walk.id + kIds, peer_none);
                     bytes += T::kTileBBytes + (peer_none ? 0u : peer ? uint32_t(peer) * kUnit * kBK : T::kTileABytes);
                 }
-                for (int kb = 0; kb < a.k_blocks; ++kb, ++kc) {
-                    const int s = int(kc % kStages);
-                    const int64_t n = kc / kStages;
-                    if (n >= 1 && !lm_wait(&bars->empty[s], uint32_t((n - 1) & 1), a.status, abort_flag, lim)) {
+                for (int kb = 0; kb < a.k_blocks; ++kb, ++kc, s = s + 1 == kStages ? 0 : s + 1, round += s == 0) {
+                    if (round > 0 && !lm_wait(&bars->empty[s], (round - 1) & 1, a.status, abort_flag, lim)) {
                         ok = false;
                         break;
                     }
                     if (kc == withheld) continue;  // test hook only: this slice never arrives
-                    unsigned char* st = smem + size_t(s) * kStageBytes;
+                    unsigned char* st = smem + uint32_t(s) * kStageBytes;
                     if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], bytes);
                     auto load = [&](void* to, const CUtensorMap* map, int64_t y) {
                         if constexpr (kPair) tma_load_2d_pair(to, map, kb * kBK, int(y), &bars->full[s]);
@@ -258,46 +261,46 @@ __global__ void __launch_bounds__(I8Tile<NR, kPair>::kThreads, 1)
             }
             // Every copy issued lands before the CTA may exit (a withheld slice was never issued). A pair's odd CTA learns it
             // from the MMAs that have read them; where those no longer come, its wait's limit is thousands of copies long.
-            for (int s = 0; s < kStages; ++s) {
-                if (kc > s) {
-                    int64_t last_kc = s + int64_t(kStages) * ((kc - 1 - s) / kStages);
-                    if (last_kc == withheld) last_kc -= kStages;
-                    if (last_kc >= 0)
-                        mbar_wait_bounded(rank == 0 ? &bars->full[s] : &bars->empty[s], uint32_t((last_kc / kStages) & 1),
-                                          a.status, lim);
-                }
+            for (int t = 0; t < kStages; ++t) {
+                // the last pass in which stage t was used: this one, or the one before
+                int64_t pass = int64_t(round) - (t < s ? 0 : 1);
+                if (withheld >= 0 && pass * kStages + t == withheld) --pass;
+                if (pass >= 0)
+                    mbar_wait_bounded(rank == 0 ? &bars->full[t] : &bars->empty[t], uint32_t(pass & 1), a.status, lim);
             }
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {  // (of a pair, the even CTA's)
+        if (rank == 0 && elect_one()) {  // (of a pair, the even CTA's)
             // ---- MMA issuer ----
-            int64_t kc = 0;
-            int i = 0;
+            int i = 0, s = 0;
+            uint32_t parity = 0;
             bool ok = true;
+            const uint64_t desc_a = smem_desc_sw128(smem_addr(smem)), desc_b = smem_desc_sw128(smem_addr(smem) + T::kTileABytes);
             for (; ok && walk.step(a); ++i) {
                 const int b = i & 1, u = i >> 1;
                 if (u >= 1 && !lm_wait(&bars->tempty[b], uint32_t((u - 1) & 1), a.status, abort_flag, lim)) break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + uint32_t(b * NR);
-                for (int kb = 0; kb < a.k_blocks; ++kb, ++kc) {
-                    const int s = int(kc % kStages);
-                    const int64_t n = kc / kStages;
-                    if (!lm_wait(&bars->full[s], uint32_t(n & 1), a.status, abort_flag, lim)) {
+                for (int kb = 0; kb < a.k_blocks; ++kb) {
+                    if (!lm_wait(&bars->full[s], parity, a.status, abort_flag, lim)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t sa = smem_addr(smem + size_t(s) * kStageBytes);
-                    const uint32_t sb = sa + T::kTileABytes;
+                    const uint64_t at = uint32_t(s) * (kStageBytes >> 4);  // (descriptors hold the address's bits from 4 on)
 #pragma unroll
                     for (int kk = 0; kk < kBK / kUK; ++kk) {
-                        const uint64_t da = smem_desc_sw128(sa + kk * kUK), db = smem_desc_sw128(sb + kk * kUK);
+                        const uint64_t da = desc_a + at + (kk * kUK >> 4), db = desc_b + at + (kk * kUK >> 4);
                         if constexpr (kPair) tc_mma_i8_pair(d_tmem, da, db, T::kIdesc, (kb | kk) != 0 ? 1u : 0u);
                         else tc_mma_i8(d_tmem, da, db, T::kIdesc, (kb | kk) != 0 ? 1u : 0u);
                     }
                     if constexpr (kPair) tc_commit_both(&bars->empty[s]);
                     else tc_commit(&bars->empty[s]);
+                    if (++s == kStages) {
+                        s = 0;
+                        parity ^= 1;
+                    }
                 }
                 if (ok) {
                     if constexpr (kPair) tc_commit_both(&bars->tfull[b]);

@@ -47,6 +47,14 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
         : "memory");
 }
 
+// True in one lane of a converged warp, the same one every time. The branch on it tells the compiler that one thread
+// issues what follows, which it can then do from uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(one));
+    return one != 0;
+}
+
 // Shared-memory matrix descriptor of a K-major tile written by TMA with the 128-byte swizzle: rows of
 // 128 bytes, groups of 8 rows 1024 bytes apart (stride byte offset), descriptor version 1, layout
 // type 2 (128-byte swizzle). Stepping K by 16 elements inside the span adds 32 bytes to the start.
