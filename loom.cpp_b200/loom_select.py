@@ -654,17 +654,17 @@ _STATUS_WS = {}
 
 
 def _status_buffer(stream):
-    """The workspace of a call that needs only the status word: one per device, never replaced. A captured call
-    gets one of its own (zeroed by the graph), which the graph's memory pool keeps."""
+    """The workspace of a call that needs only the status word: one per device, never replaced, which captured calls
+    use too. A call captured before there is one gets one of its own (zeroed by the graph: a node of 2 us each time
+    it is replayed), which the graph's memory pool keeps."""
     torch = _torch()
     with _on(stream):
         dev = torch.cuda.current_device()
-        capturing = torch.cuda.is_current_stream_capturing()
-        if not capturing and dev in _STATUS_WS:
+        if dev in _STATUS_WS:
             return _STATUS_WS[dev].buf
         ws = Workspace(torch.device("cuda", dev))
         ws.get(256, stream)
-        if not capturing:
+        if not torch.cuda.is_current_stream_capturing():
             torch.cuda.current_stream().synchronize()  # zeroed before another stream's call reads it
             _STATUS_WS[dev] = ws
     return ws.buf
