@@ -12,9 +12,12 @@
 // persistent CTA per SM. Warp 0 streams 128-byte K slices of both tiles into a shared-memory ring with TMA (128-byte
 // swizzle, a K tail filled with zeros), warp 1 issues tcgen05.mma kind::i8 (M 128, N NR, K 32) into one of two TMEM
 // accumulators, the other warps drain the other one, scale it and write the logits.
-// Calls of more than 128 rows work in pairs of CTAs (cta_group::2, M 256, N 160 to 256): each loads its own ids and half of the
-// rows, so a stage brings 32 KiB into an SM for the work that a CTA by itself would fetch 48 KiB for -- at 64 bytes a
-// cycle from L2 that fetch, 768 cycles, and not the MMA's 512, is what bound it.
+// Copies and products are issued by an elected lane: behind `lane == 0` alone the compiler does not know that one thread
+// issues, and a slice's four products and their commit took 304 cycles in place of 52, its copies 620 in place of 414
+// ([1024, 2048] x [151936, 2048] 262 us, now 230; [1, 8192] x [12000, 8192] 46 and 23).
+// Calls of more than 128 rows work in pairs of CTAs (cta_group::2, M 256, N 160 to 256) where they fill the device: each
+// loads its own ids and half of the rows, so a stage brings 32 KiB into an SM for the work that a CTA by itself would fetch
+// 48 KiB for ([1024, 2048] x [151936, 2048] bf16 logits 230 us, by single CTAs 263).
 // With one tile of rows, each CTA (or pair) takes an equal share of the ids, to 16 (a TMA box): 151936 ids are 1187.0
 // tiles, whose whole ones would leave 3 of 148 SMs a ninth. With several, they take whole tiles, rows fastest, so that
 // those running together share a weight tile through L2.
@@ -51,7 +54,7 @@ struct I8Tile {
     static constexpr uint32_t kStageBytes = kTileABytes + kTileBBytes;
     static_assert(kStageBytes % 1024 == 0, "stage alignment");
     // Warp 0 TMA, warp 1 MMA and TMEM, then the epilogue: four warps cover the accumulator's lanes, eight its columns by
-    // halves too (four drain a 256-row tile too slowly: 256 us for [1024, 2048] x [151936, 2048], bf16 logits).
+    // halves too (four drained a 256-row tile too slowly: [1024, 2048] x [151936, 2048] bf16 logits 256 us before there were pairs).
     static constexpr int kEpiWarps = NR >= 64 ? 8 : 4;
     static constexpr int kThreads = 64 + 32 * kEpiWarps;
     static constexpr int kEpiCols = NR / (kEpiWarps / 4);  // rows a warp drains of a tile, 32 at a time
@@ -131,7 +134,7 @@ struct I8Walk {
     }
     // TMA boxes of kUnit ids for the CTA whose ids begin at `from`; 0: one box for its whole tile. Where CTAs share the ids
     // out, what is left of a share goes by small boxes (a whole tile by sixteen of them: 96 us for one row, where one
-    // box takes 61).
+    // box took 61).
     __device__ __forceinline__ int boxes(const I8Args& a, int64_t from, bool& none) const {
         none = tile_end <= from;
         const int64_t left = (tile_end - from + kUnit - 1) / kUnit;
@@ -227,8 +230,7 @@ __global__ void __launch_bounds__(I8Tile<NR, kPair>::kThreads, 1)
     if (warp == 0) {
         if (elect_one()) {
             // ---- producer ----
-            // (stage and parity are counted along: dividing the slice's number cost 300 cycles a slice, [1, 2048] x
-            // [151936, 2048] 59 us and [12000, 8192] 47)
+            // (stage and parity are counted along: dividing the slice's number for them cost 60 cycles a slice)
             int64_t kc = 0;
             int s = 0;
             uint32_t round = 0;  // the ring's passes so far, of which the last bit is the parity
@@ -426,6 +428,11 @@ int launch_i8_any(const void* hidden, const void* weight, const I8Args& a, int64
     if (a.rows <= 16) return launch_i8<16, false, kOut>(hidden, weight, a, hidden_dim, sms, stream);
     if (a.rows <= 64) return launch_i8<64, false, kOut>(hidden, weight, a, hidden_dim, sms, stream);
     if (a.rows <= 128) return launch_i8<128, false, kOut>(hidden, weight, a, hidden_dim, sms, stream);
+    // a tile for each CTA at most: by themselves, 64 rows a tile if there are CTAs for them ([500, 8192] x [1000, 8192] 17.0
+    // us, in pairs 24.7; [200, 8192] x [4000, 8192] 17.4 and 25.4; [500, 8192] x [4000, 8192] of 128 rows 19.6 and 25.4)
+    const int64_t v_tiles = (a.n_vocab + kIds - 1) / kIds;
+    if ((a.rows + 63) / 64 * v_tiles <= sms) return launch_i8<64, false, kOut>(hidden, weight, a, hidden_dim, sms, stream);
+    if ((a.rows + 127) / 128 * v_tiles <= sms) return launch_i8<128, false, kOut>(hidden, weight, a, hidden_dim, sms, stream);
     // as few tiles of rows as there have to be, no higher than they have to be
     const int64_t tiles = (a.rows + 255) / 256, high = (a.rows + tiles - 1) / tiles;
     if (high <= 160) return launch_i8<160, true, kOut>(hidden, weight, a, hidden_dim, sms, stream);

@@ -205,6 +205,18 @@ def test_product_many_rows(rows, hidden, vocab):
         assert torch.equal(out[:, v:v + 32768], _product(q, qs, w[v:v + 32768], ws[v:v + 32768], torch.bfloat16))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,hidden,vocab", [
+    (150, 272, 20011), (185, 144, 20011), (220, 48, 20011), (256, 1040, 20011), (260, 128, 30000), (700, 400, 20011),
+    (129, 8192, 130), (300, 1040, 500), (600, 400, 1900), (1000, 272, 1100), (1024, 2048, 100),
+])
+def test_product_tile_shapes(rows, hidden, vocab, dtype):
+    """Every height of tile, of pairs and of single CTAs, with rows and ids left over."""
+    q, qs, w, ws = _operands(rows, hidden, vocab, rows + vocab, lo=-128)
+    out = ls.lm_head_logits_i8(q, qs, w, ws, dtype=dtype)
+    assert torch.equal(out, _product(q, qs, w, ws, dtype))
+
+
 @pytest.mark.parametrize("hidden", [2048, 65536])
 def test_product_extremes(hidden):
     """The largest sums of either sign: 2^14 hidden, at most 2^30."""
@@ -351,3 +363,23 @@ def test_product_row_tiles(rows):
     q, qs, w, ws = _operands(rows, 160, 1500, rows)
     out = ls.lm_head_logits_i8(q, qs, w, ws)
     assert torch.equal(out, _product(q, qs, w, ws, torch.float32))
+
+
+def test_captured_calls_use_the_status_word_that_is_there():
+    """Two graphs and an eager call, which share the device's status word, side by side."""
+    q, qs, w, ws = _operands(9, 512, 4099, 6)
+    want = ls.lm_head_logits_i8(q, qs, w, ws)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g, out = torch.cuda.CUDAGraph(), torch.empty_like(want)
+        with torch.cuda.graph(g):
+            ls.lm_head_logits_i8_into(q, qs, w, ws, out)
+        graphs.append((g, out, torch.cuda.Stream()))
+    for _ in range(10):
+        for g, out, s in graphs:
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = ls.lm_head_logits_i8(q, qs, w, ws)
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for _, out, _ in graphs) and torch.equal(eager, want)
