@@ -314,7 +314,12 @@ LOOM_SELECT_API int loom_token_logprobs(const void* logits, int dtype, int64_t r
  * row NaN. A row whose two weights are 0 gets zeros, whatever its logits hold; otherwise a row whose lse is NaN or
  * infinite gets NaN. -inf logits get 0. out_grad rows are grad_stride >= V elements apart; out_grad may be the logits
  * themselves (same pointer, same stride: LOOM_SELECT_EINVAL otherwise), and must not overlap them in another way.
- * No workspace, no atomics: the result does not depend on timing.
+ * Accuracy: an entry is off by 2^-24 (|lse| + 4 |log2 p| + 13) of p times its row's weights (|grad_logp| + |grad_entropy|
+ * (|log2 p| + entropy + 1), over T), |lse| being lse's own rounding, besides the output's. An id with p above 3/4 has an
+ * entry that is small beside that: where the row's entries add up to zero, as they do for this row's own lse and
+ * entropy (to 2^-16 + 2^-22 |lse| of the weights), its entry is minus the sum of the others, and off by what they are.
+ * With an lse of more ids than the row's it is the formula's, and off by lse's rounding of the weights.
+ * No workspace, no sums by atomics: the result does not depend on timing.
  */
 LOOM_SELECT_API int loom_token_logprobs_grad(const void* logits, int dtype, int64_t rows, int64_t n_vocab,
                                              int64_t row_stride, const int32_t* ids, float temperature,

@@ -878,8 +878,11 @@ cudaError_t launch_lp_any(const LpDev& p, int64_t rows, int sms, cudaStream_t s)
 //
 // L = sum_r g_r log p_r(t_r) + h_r H_r. With l_j = y_j - lse and p_j = e^(l_j):
 //   dL/dx_j = (1/T) [ g (delta_jt - p_j) - h p_j (l_j + H) ]   (dH/dy_j = -p_j (l_j + H)).
-// Elementwise once lse and H are there (the forward pass returns them): reads the logits and writes
-// the gradient, nothing else. Bound: HBM ([1024, 151936] f32 in 193 us, 6.4 TB/s).
+// Elementwise once lse and H are there (the forward pass returns them), but for an id with p near 1: lse is an f32, so
+// log p is off by half a unit of lse's last place, and 1 - p by as much in absolute terms, of a small number that is the
+// row's largest entry. A row's entries add up to zero, and the others' are off by that only relative to themselves: such
+// an id's entry is minus the sum of the others. A row therefore belongs to one warp, block or cluster, which joins
+// its threads' sums at the end. Bound: HBM ([1024, 151936] f32 in 192 us, 6.5 TB/s).
 struct LpGradDev {
     const unsigned char* base;
     int64_t rows, width, row_stride;
@@ -892,6 +895,9 @@ struct LpGradDev {
     const float* g_entropy;
     unsigned char* out;
     int64_t out_stride;
+    float likely;       // a likely id's x - lse T is above this
+    float low_entropy;  // a row with one has less than this
+    bool in_place;
 };
 
 template <int kDtype>
@@ -916,132 +922,285 @@ __device__ __forceinline__ uint4 plain_v4(const void* p) {
     return r;
 }
 
+// An id is likely, its entry taken from the others', where log2 p is above this (p above 0.758, so one id of a row at most:
+// below it the entry's own error is at most three times p's).
+constexpr float kLikely = -0.4f;
+// The others' sum is taken where it agrees with the formula's own value to this much, and 2^-22 of lse, of the weights. (The
+// forward call's lse is off by about 1e-6 and its rounding. With an lse of more ids than the row's the entries do not add up
+// to zero.)
+constexpr float kLseError = 1.52587890625e-5f;  // 2^-16
+
 // What a row's elements share. l / ln 2 = ((x - lse T) log2(e) / T), with lse T in two f32 parts: near the row's
-// likely elements the first difference is exact, so l is off by a few units of its own size and not of lse's.
+// likely elements the first difference is exact, so l is off by what lse is, and a few units of its own size.
 struct LpGradRow {
-    float hi, lo;   // lse T
-    float g, h;     // the gradient is -p (g + h l / ln 2), plus `at` at t
-    float c;        // log2(e) / T
+    float hi, lo_c;  // lse T; the second part's product with c, negated
+    float g, h;      // the gradient is p (g + h l / ln 2), plus `at` at t
+    float c;         // log2(e) / T
     float at;
 
-    __device__ __forceinline__ float grad(float x, bool is_t) const {
+    __device__ __forceinline__ float exponent(float x) const {
         // (clamped: p is 0 there, and stays finite times l)
-        const float l = max_nan(__fmul_rn(__fsub_rn(__fsub_rn(x, hi), lo), c), kMinExp2);
-        const float d = __fmul_rn(ex2(l), __fmaf_rn(h, l, g));
-        return is_t ? at - d : -d;
+        return max_nan(__fmaf_rn(__fsub_rn(x, hi), c, lo_c), kMinExp2);
     }
 
-    // Two at a time; the signs of g and h are turned, so that no negation is left.
-    __device__ __forceinline__ uint64_t grad2(uint64_t x, uint64_t hi2, uint64_t lo2, uint64_t c2, uint64_t h2,
+    __device__ __forceinline__ float grad(float l, bool is_t) const {
+        return __fadd_rn(__fmul_rn(ex2(l), __fmaf_rn(h, l, g)), is_t ? at : 0.0f);
+    }
+
+    // Two at a time, without `at`.
+    __device__ __forceinline__ uint64_t grad2(uint64_t x, uint64_t hi2, uint64_t lo_c2, uint64_t c2, uint64_t h2,
                                               uint64_t g2) const {
+        uint64_t l;
         asm("sub.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(hi2));
-        asm("sub.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(lo2));
-        asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(c2));
+        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(l) : "l"(x), "l"(c2), "l"(lo_c2));
         float l0, l1;
-        unpack2(x, l0, l1);
+        unpack2(l, l0, l1);
         l0 = max_nan(l0, kMinExp2);
         l1 = max_nan(l1, kMinExp2);
-        const uint64_t l = pack2(l0, l1), e = pack2(ex2(l0), ex2(l1));
+        const uint64_t e = pack2(ex2(l0), ex2(l1));
+        l = pack2(l0, l1);
         asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(x) : "l"(h2), "l"(l), "l"(g2));
         asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(e));
         return x;
     }
 };
 
-constexpr int kGradNT = 256;
-// Four vectors a thread keep the reads and the writes both going: [1024, 151936] f32 193.7 us (2 vectors: 202.6, 8: 188.3)
-// and bf16 96.6 us (114.6, 108.7), where a copy of the same bytes takes 190 and 95 us.
-constexpr int kGradU = 4;
-// Rows up to this wide go a warp to a row: [16384, 1025] f32 32.7 us (a block to a row: 110).
-constexpr int64_t kGradNarrow = 4096;
+// Element q of a 16-byte vector, q not known to the compiler.
+template <int kDtype>
+__device__ __forceinline__ float pick(uint4 raw, int q) {
+    const int word = kDtype == LOOM_SELECT_BF16 ? q >> 1 : q;
+    const uint32_t a = word & 1 ? raw.y : raw.x, b = word & 1 ? raw.w : raw.z, w = word & 2 ? b : a;
+    if constexpr (kDtype == LOOM_SELECT_BF16) return __uint_as_float(q & 1 ? w & 0xffff0000u : w << 16);
+    else return __uint_as_float(w);
+}
 
-// kTPR threads per piece of a row (kGradU vectors a thread), 256 / kTPR pieces to a block. Rows of logits and of the gradient that start at the same
-// place within 16 bytes go by vectors, but for the ones the row only partly fills; others element by element.
-template <int kDtype, int kTPR>
-__global__ void __launch_bounds__(kGradNT) token_logprobs_grad_kernel(const LpGradDev p, int32_t pieces) {
+constexpr int kGradNT = 256;  // threads of a block that holds a row to each warp
+constexpr int kGradU = 4;
+// Shares of a row. A warp: rows of one step, and up to 4096 wide where there are 32 or more to an SM ([16384, 1025] f32 25.6 us,
+// blocks of four warps 40.7; [1000, 4000] f32 14.6 and 8.6). A block of four warps, two steps: [8000, 8000] bf16 51.5 us (of eight
+// 54.7). Wider rows by blocks of eight warps with three to six steps each, in clusters ([1024, 151936] f32, a cluster of
+// 8: 191.5 us, 4: 197.5, 2: 203; bf16, 4: 100.6, 2: 103.3, 8: 103.3; [3000, 32000] f32, 2: 119.8, 1: 126.6, 8: 137), and with
+// fewer steps where there are less than three blocks to an SM ([77, 51865] bf16, 8: 6.7 us, 4: 7.5, 2: 8.2). A row or a few
+// long ones by blocks of 32 warps (one of 151936 f32 5.0 us, of eight warps 6.0).
+// With a likely id in every row, whose entries have to be summed, [1024, 151936] f32 takes 204 us and bf16 112.
+constexpr int64_t kGradNarrow = 4096, kGradFew = 4;
+
+// What a block found in its part of a row.
+struct GradPart {
+    float sum;      // of the entries, the likely id's left out
+    float direct;   // its entry by the formula
+    int32_t id, n;  // the likely id; how many there were
+};
+
+template <int kWarps>
+struct GradShared {
+    float direct;
+    int32_t id;
+    float warp_sum[kWarps];
+    GradPart part[kWarps > 1 ? kMaxCluster : 1];  // of the cluster's blocks, in its first
+};
+
+// A row to kWarps warps in each block of a cluster (kWarps == 1: to a warp, eight rows to a block), kGradU vectors a thread
+// and step. Rows of logits and of the gradient that start at the same place within 16 bytes go by vectors, the elements of
+// those that the row only partly fills apart; others element by element.
+template <int kDtype, int kWarps>
+__global__ void __launch_bounds__(kWarps == 1 ? kGradNT : kWarps * 32, kWarps == 4 ? 10 : kWarps == 32 ? 1 : 5)
+    token_logprobs_grad_kernel(const LpGradDev p) {
     constexpr int kEsz = kDtype == LOOM_SELECT_BF16 ? 2 : 4;
     constexpr int kPer = 16 / kEsz;
-    const uint32_t unit = blockIdx.x * (kGradNT / kTPR) + threadIdx.x / kTPR;
-    const int64_t row = unit / unsigned(pieces);
-    const int32_t piece = int32_t(unit % unsigned(pieces));
-    const int32_t thread = threadIdx.x % kTPR;
-    if (row >= p.rows) return;
+    constexpr int kNT = kWarps * 32;
+    constexpr int kRows = kWarps == 1 ? kGradNT / 32 : 1;
+    __shared__ GradShared<kWarps> sh_of_row[kRows];
+    GradShared<kWarps>& sh = sh_of_row[kWarps == 1 ? threadIdx.x / 32 : 0];
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int C = kWarps == 1 ? 1 : int(cluster.num_blocks()), rank_in = kWarps == 1 ? 0 : int(cluster.block_rank());
+    const int64_t row = kWarps == 1 ? int64_t(blockIdx.x) * kRows + threadIdx.x / 32 : blockIdx.x / unsigned(C);
+    const int32_t thread = threadIdx.x % kNT;
+    if (kWarps == 1 && row >= p.rows) return;
     const unsigned char* in = p.base + row * p.row_stride * kEsz;
     unsigned char* out = p.out + row * p.out_stride * kEsz;
-    const int32_t shift = int32_t((reinterpret_cast<uintptr_t>(in) & 15) / kEsz);
+    const int32_t width = int32_t(p.width), shift = int32_t((reinterpret_cast<uintptr_t>(in) & 15) / kEsz);
     const bool vectors = shift == int32_t((reinterpret_cast<uintptr_t>(out) & 15) / kEsz);
-    const int32_t v = piece * kGradU * kTPR + thread;  // this thread's first vector, the others kTPR apart
 
     const int32_t t = p.ids ? p.ids[row] : -1;
-    const float g = p.g_logp && t >= 0 ? p.g_logp[row] : 0.0f;
+    const float g_any = p.g_logp ? p.g_logp[row] : 0.0f;
     const float h = p.g_entropy ? p.g_entropy[row] : 0.0f;
+    const float ent = p.g_entropy ? p.entropy[row] : 0.0f;
     const float lse = p.lse[row];
-    const float ent = h != 0.0f ? p.entropy[row] : 0.0f;
-    const bool zero = g == 0.0f && h == 0.0f;
+    const float g = t >= 0 ? g_any : 0.0f;
+    // vectors [v_first, v_end) are inside the row
+    const int32_t v_first = shift ? 1 : 0, v_end = max((shift + width) / kPer, v_first);
+    const unsigned char* vin = in - shift * kEsz;
+    unsigned char* vout = out - shift * kEsz;
+    // the others' elements: the first's by threads 0 .. kPer - 1, the last's by the next kPer
+    auto edge = [&] {
+        int32_t id = -1;
+        if (thread < kPer && v_first > 0) id = thread - shift;
+        if (thread >= kPer && thread < 2 * kPer && v_end * kPer < shift + width) id = v_end * kPer - shift + thread - kPer;
+        return rank_in == 0 && id < width ? id : -1;
+    };
+    if (g == 0.0f && h == 0.0f) {
+        if (!vectors) {
+            for (int32_t id = rank_in * kNT + thread; id < width; id += C * kNT) store_elem<kDtype>(out, id, 0.0f);
+        } else {
+            if (const int32_t id = edge(); id >= 0) store_elem<kDtype>(out, id, 0.0f);
+            for (int32_t v = v_first + rank_in * kNT + thread; v < v_end; v += C * kNT)
+                *reinterpret_cast<uint4*>(vout + int64_t(v) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        return;
+    }
+    // The vectors of the next step are requested as those of this one are done with.
+    int32_t v = vectors ? v_first + rank_in * kGradU * kNT + thread : v_end;
     uint4 raw[kGradU];
 #pragma unroll
-    for (int u = 0; u < kGradU; ++u) {
-        const int32_t first = (v + u * kTPR) * kPer - shift;
-        if (vectors && !zero && first >= 0 && first + kPer <= p.width)
-            raw[u] = plain_v4(in + int64_t(first) * kEsz);
-    }
+    for (int u = 0; u < kGradU; ++u)
+        if (v + u * kNT < v_end) raw[u] = plain_v4(vin + int64_t(v + u * kNT) * 16);
+    const int32_t edge_id = vectors ? edge() : -1;
+    const float edge_x = edge_id >= 0 ? plain_elem<kDtype>(in, edge_id) : 0.0f;
+    // (its own logit may be gone when the gradient is written over it)
+    const float xt = h == 0.0f && !p.in_place && t >= 0 && t < width ? plain_elem<kDtype>(in, t) : 0.0f;
     LpGradRow r;
     const double lt = double(lse) * p.T;
     r.hi = __double2float_rn(lt);
-    r.lo = __double2float_rn(lt - double(r.hi));
     r.c = p.c;
+    r.lo_c = -__fmul_rn(__double2float_rn(lt - double(r.hi)), p.c);
     r.at = __fmul_rn(g, p.inv_t);
     const float hs = __fmul_rn(h, p.inv_t);
-    r.g = h != 0.0f ? __fmaf_rn(hs, ent, r.at) : r.at;
-    r.h = __fmul_rn(hs, kLn2);
+    r.g = h != 0.0f ? -__fmaf_rn(hs, ent, r.at) : -r.at;
+    r.h = -__fmul_rn(hs, kLn2);
     // an id past the vocabulary, an empty row, a row with NaN or +inf: NaN throughout
-    if (!(fabsf(lse) <= FLT_MAX) || (t >= p.width && g != 0.0f)) r.g = quiet_nan();
-    const uint64_t hi2 = pack2(r.hi, r.hi), lo2 = pack2(r.lo, r.lo), c2 = pack2(r.c, r.c), h2 = pack2(-r.h, -r.h),
-                   g2 = pack2(-r.g, -r.g);
-#pragma unroll
-    for (int u = 0; u < kGradU; ++u) {
-        const int32_t first = (v + u * kTPR) * kPer - shift;
-        if (vectors && first >= 0 && first + kPer <= p.width) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (!zero) {
-                const Pairs<kDtype> x(raw[u]);
-                float d[kPer];
-#pragma unroll
-                for (int q = 0; q < kPer / 2; ++q) unpack2(r.grad2(x.v[q], hi2, lo2, c2, h2, g2), d[2 * q], d[2 * q + 1]);
-                if (t >= first && t < first + kPer) {
-#pragma unroll
-                    for (int q = 0; q < kPer; ++q) d[q] += first + q == t ? r.at : 0.0f;
-                }
-                if constexpr (kDtype == LOOM_SELECT_BF16) {
-                    uint32_t b[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const __nv_bfloat162 pr = __floats2bfloat162_rn(d[2 * q], d[2 * q + 1]);
-                        b[q] = *reinterpret_cast<const uint32_t*>(&pr);
-                    }
-                    w = make_uint4(b[0], b[1], b[2], b[3]);
-                } else {
-                    w = make_uint4(__float_as_uint(d[0]), __float_as_uint(d[1]), __float_as_uint(d[2]),
-                                   __float_as_uint(d[3]));
-                }
-            }
-            *reinterpret_cast<uint4*>(out + int64_t(first) * kEsz) = w;
-        } else if (vectors) {
-            for (int q = 0; q < kPer; ++q) {
-                const int32_t id = first + q;
-                if (id >= 0 && id < p.width)
-                    store_elem<kDtype>(out, id, zero ? 0.0f : r.grad(plain_elem<kDtype>(in, id), id == t));
-            }
+    if (!(fabsf(lse) <= FLT_MAX) || (t >= width && g != 0.0f)) r.g = quiet_nan();
+    const uint64_t hi2 = pack2(r.hi, r.hi), lo_c2 = pack2(r.lo_c, r.lo_c), c2 = pack2(r.c, r.c), h2 = pack2(r.h, r.h),
+                   g2 = pack2(r.g, r.g);
+    // Whether the row may have a likely id whose entry matters: any with an entropy term, else the given token.
+    const bool sums = h != 0.0f ? ent < p.low_entropy : t < width && (p.in_place || __fsub_rn(xt, r.hi) > p.likely);
+    if (C > 1 && sums) cluster.barrier_arrive();  // (waited for before the first remote store: all blocks have begun)
+    uint64_t sum2 = 0;
+    float sum = 0.0f;
+    bool found = false;
+    // one element apart from the pairs
+    auto element = [&](float x, int32_t id) {
+        const float d = r.grad(r.exponent(x), id == t);
+        if (sums && __fsub_rn(x, r.hi) > p.likely) {
+            if (found) sum = quiet_nan();  // (two: an lse of other logits; nothing is made of the sum)
+            found = true;
+            sh.direct = d;
+            sh.id = id;
+        } else {
+            sum += d;
         }
-    }
+        store_elem<kDtype>(out, id, d);
+    };
     if (!vectors) {
-        const int32_t begin = piece * kGradU * kTPR * kPer;
-        for (int j = 0; j < kGradU * kPer; ++j) {
-            const int32_t id = begin + j * kTPR + thread;
-            if (id < p.width)
-                store_elem<kDtype>(out, id, zero ? 0.0f : r.grad(plain_elem<kDtype>(in, id), id == t));
+#pragma unroll 1
+        for (int32_t id = rank_in * kNT + thread; id < width; id += C * kNT) element(plain_elem<kDtype>(in, id), id);
+    } else {
+        if (edge_id >= 0) element(edge_x, edge_id);
+#pragma unroll 1
+        for (; v < v_end; v += C * kGradU * kNT) {
+#pragma unroll
+            for (int u = 0; u < kGradU; ++u) {
+                if (v + u * kNT >= v_end) break;
+                const int32_t first = (v + u * kNT) * kPer - shift;
+                unsigned char* to = vout + int64_t(v + u * kNT) * 16;
+                const int32_t next = v + u * kNT + C * kGradU * kNT;
+                if (uint32_t(t - first) < uint32_t(kPer) || (sums && __fsub_rn(vec_max<kDtype>(raw[u]), r.hi) > p.likely)) {
+#pragma unroll 1
+                    for (int q = 0; q < kPer; ++q) element(pick<kDtype>(raw[u], q), first + q);
+                    if (next < v_end) raw[u] = plain_v4(vin + int64_t(next) * 16);
+                    continue;
+                }
+                const Pairs<kDtype> x(raw[u]);
+                uint32_t w[4];
+#pragma unroll
+                for (int q = 0; q < kPer / 2; ++q) {
+                    const uint64_t d2 = r.grad2(x.v[q], hi2, lo_c2, c2, h2, g2);
+                    add2(sum2, d2);
+                    float d0, d1;
+                    unpack2(d2, d0, d1);
+                    if constexpr (kDtype == LOOM_SELECT_BF16) {
+                        const __nv_bfloat162 pr = __floats2bfloat162_rn(d0, d1);
+                        w[q] = *reinterpret_cast<const uint32_t*>(&pr);
+                    } else {
+                        w[2 * q] = __float_as_uint(d0), w[2 * q + 1] = __float_as_uint(d1);
+                    }
+                }
+                if (next < v_end) raw[u] = plain_v4(vin + int64_t(next) * 16);
+                *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
         }
     }
+    if (!sums) return;  // (the whole row's threads)
+    float s0, s1;
+    unpack2(sum2, s0, s1);
+    sum += s0 + s1;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    GradPart all;
+    all.sum = sum;
+    if constexpr (kWarps == 1) {
+        all.n = __popc(__ballot_sync(0xffffffffu, found));
+        __syncwarp();
+    } else {
+        if (threadIdx.x % 32 == 0) sh.warp_sum[threadIdx.x / 32] = sum;
+        all.n = __syncthreads_count(found);
+    }
+    all.direct = sh.direct, all.id = sh.id;
+    if constexpr (kWarps > 1) {
+        if (thread == 0) {
+            all.sum = 0.0f;
+            for (int w = 0; w < kWarps; ++w) all.sum += sh.warp_sum[w];
+        }
+        if (C > 1) {
+            cluster.barrier_wait();
+            if (thread == 0) *cluster.map_shared_rank(&sh.part[rank_in], 0) = all;
+            cluster.barrier_arrive();
+            if (rank_in != 0) return;  // (nobody reads this block's shared memory)
+            cluster.barrier_wait();
+            if (thread == 0) {
+                all = sh.part[0];
+                for (int b = 1; b < C; ++b) {
+                    const GradPart o = sh.part[b];
+                    all.sum += o.sum;
+                    if (o.n) all.direct = o.direct, all.id = o.id;
+                    all.n += o.n;
+                }
+            }
+        }
+    }
+    if (thread != 0 || all.n != 1) return;
+    const float weight = (p.g_logp && t >= 0 ? fabsf(p.g_logp[row]) : 0.0f) +
+                         (p.g_entropy ? fabsf(p.g_entropy[row]) * (4.0f + 2.0f * p.entropy[row]) : 0.0f);
+    const float off = weight * p.inv_t * (kLseError + 2.0f * FLT_EPSILON * fabsf(p.lse[row]));
+    if (fabsf(-all.sum - all.direct) <= off) store_elem<kDtype>(out, all.id, -all.sum);
+}
+
+template <int kDtype, int kWarps>
+cudaError_t launch_grad(const LpGradDev& p, int C, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(kWarps == 1 ? (p.rows + kGradNT / 32 - 1) / (kGradNT / 32) : p.rows * C));
+    cfg.blockDim = dim3(kWarps == 1 ? kGradNT : kWarps * 32);
+    cfg.stream = s;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = unsigned(C);
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, token_logprobs_grad_kernel<kDtype, kWarps>, p);
+}
+
+template <int kDtype>
+cudaError_t launch_grad_any(const LpGradDev& p, int sms, cudaStream_t s) {
+    constexpr int kPer = kDtype == LOOM_SELECT_BF16 ? 8 : 4;
+    const int64_t nv = (p.width + kPer - 2) / kPer + 1;  // (a row may start inside a vector)
+    if (nv <= 32 * kGradU || (p.width <= kGradNarrow && p.rows >= 32 * int64_t(sms))) return launch_grad<kDtype, 1>(p, 1, s);
+    if (nv <= 2 * 4 * 32 * kGradU) return launch_grad<kDtype, 4>(p, 1, s);
+    const int64_t steps = (nv + 8 * 32 * kGradU - 1) / (8 * 32 * kGradU);
+    if (p.rows <= kGradFew && steps > 2 * kMaxCluster) return launch_grad<kDtype, 32>(p, kMaxCluster, s);
+    int C = 1;
+    while (C < kMaxCluster && (steps >= 6 * C || (steps > C && p.rows * C < 3 * int64_t(sms)))) C *= 2;
+    return launch_grad<kDtype, 8>(p, C, s);
 }
 
 bool dtype_ok(int dtype) { return dtype == LOOM_SELECT_F32 || dtype == LOOM_SELECT_BF16; }
@@ -1135,22 +1294,16 @@ LOOM_SELECT_API int loom_token_logprobs_grad(const void* logits, int dtype, int6
     p.g_entropy = grad_entropy;
     p.out = static_cast<unsigned char*>(out_grad);
     p.out_stride = grad_stride;
+    p.likely = float(kLikely * 0.6931471805599453 * p.T);
+    p.low_entropy = float(0.57 + 0.25 * std::log(double(n_vocab)));  // (at p = 3/4, the rest evenly spread: 0.563 + ln(V - 1) / 4)
+    p.in_place = logits == out_grad;
     const auto s = static_cast<cudaStream_t>(stream);
-    const bool narrow = n_vocab <= kGradNarrow;
-    const int64_t per_piece = int64_t(kGradU) * (narrow ? 32 : kGradNT) * (dtype == LOOM_SELECT_BF16 ? 8 : 4);
-    const int64_t pieces = (n_vocab + 7 + per_piece - 1) / per_piece;  // (a row may start inside a vector)
-    const int64_t per_block = narrow ? kGradNT / 32 : 1, blocks = (rows * pieces + per_block - 1) / per_block;
-    if (rows * pieces > INT32_MAX) return LOOM_SELECT_ESHAPE;
-    const unsigned grid = unsigned(blocks);
-    const int32_t n = int32_t(pieces);
-    if (dtype == LOOM_SELECT_BF16) {
-        if (narrow) token_logprobs_grad_kernel<LOOM_SELECT_BF16, 32><<<grid, kGradNT, 0, s>>>(p, n);
-        else token_logprobs_grad_kernel<LOOM_SELECT_BF16, kGradNT><<<grid, kGradNT, 0, s>>>(p, n);
-    } else {
-        if (narrow) token_logprobs_grad_kernel<LOOM_SELECT_F32, 32><<<grid, kGradNT, 0, s>>>(p, n);
-        else token_logprobs_grad_kernel<LOOM_SELECT_F32, kGradNT><<<grid, kGradNT, 0, s>>>(p, n);
-    }
-    return cudaGetLastError() == cudaSuccess ? LOOM_SELECT_OK : LOOM_SELECT_ECUDA;
+    int st = LOOM_SELECT_OK;
+    const int sms = device_sm_count(&st);
+    if (st != LOOM_SELECT_OK) return st;
+    const cudaError_t e = dtype == LOOM_SELECT_BF16 ? launch_grad_any<LOOM_SELECT_BF16>(p, sms, s)
+                                                    : launch_grad_any<LOOM_SELECT_F32>(p, sms, s);
+    return e == cudaSuccess ? LOOM_SELECT_OK : LOOM_SELECT_ECUDA;
 }
 
 }  // extern "C"
