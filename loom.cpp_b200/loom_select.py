@@ -24,6 +24,7 @@ import collections
 import contextlib
 import ctypes
 import os
+import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libloom_select.so")
@@ -651,30 +652,53 @@ def quantize_rows_i8(x, stream=None):
 
 
 _STATUS_WS = {}
+_STATUS_LOCK = threading.Lock()
+_CAPTURED_WS = {}
 
 
 def _status_buffer(stream):
     """The workspace of a call that needs only the status word: one per device, never replaced, which captured calls
     use too. A call captured before there is one gets one of its own (zeroed by the graph: a node of 2 us each time
-    it is replayed), which the graph's memory pool keeps."""
+    it is replayed). read_status() reads them all, so they stay."""
     torch = _torch()
     with _on(stream):
         dev = torch.cuda.current_device()
         if dev in _STATUS_WS:
             return _STATUS_WS[dev].buf
         ws = Workspace(torch.device("cuda", dev))
-        ws.get(256, stream)
-        if not torch.cuda.is_current_stream_capturing():
-            torch.cuda.current_stream().synchronize()  # zeroed before another stream's call reads it
-            _STATUS_WS[dev] = ws
-    return ws.buf
+        if torch.cuda.is_current_stream_capturing():
+            ws.get(256, stream)
+            _CAPTURED_WS.setdefault(dev, []).append(ws)
+            return ws.buf
+        with _STATUS_LOCK:  # (the first of several host threads: the others, and what they capture, use its word)
+            if dev not in _STATUS_WS:
+                ws.get(256, stream)
+                torch.cuda.current_stream().synchronize()  # zeroed before another stream's call reads it
+                _STATUS_WS[dev] = ws
+            return _STATUS_WS[dev].buf
+
+
+def read_status(stream=None):
+    """The first device-side error (EHISTORY, ETIMEOUT) that calls without a workspace of their own have recorded on the
+    current device since this was last asked, or OK. Waits for `stream`: ask on the one that the calls, or the replayed
+    graphs, ran on. After ETIMEOUT the outputs of such calls are invalid; the calls that follow are not affected."""
+    dev = _torch().cuda.current_device()
+    status = OK
+    for ws in (_DEFAULT_WS.get(dev), _STATUS_WS.get(dev), *_CAPTURED_WS.get(dev, ())):
+        found = OK if ws is None else ws.read_status(stream)
+        if found == ETIMEOUT:
+            check(_lib().loom_select_workspace_init(_ptr(ws.buf), ws.buf.numel(), _stream_handle(stream)),
+                  "loom_select_workspace_init")
+        status = status or found
+    return status
 
 
 def lm_head_logits_i8_into(hidden, hidden_scale, weight, weight_scale, out, workspace=None, stream=None):
     """out[r, v] = (hidden[r] . weight[v]) * hidden_scale[r] * weight_scale[v] (asynchronous).
 
     hidden int8 [rows, hidden_dim] with hidden_scale f32 [rows], weight int8 [n_vocab, hidden_dim] with weight_scale
-    f32 [n_vocab], all contiguous; out f32 or bf16 [rows, n_vocab], rows of any stride. See loom_lm_head_logits_i8."""
+    f32 [n_vocab], all contiguous; out f32 or bf16 [rows, n_vocab], rows of any stride. See loom_lm_head_logits_i8.
+    Without a workspace, read_status() tells whether a wait gave up."""
     torch = _torch()
     if hidden.dim() not in (1, 2) or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
         raise SelectError(EINVAL, "hidden must be [rows, hidden_dim] and weight [n_vocab, hidden_dim]")
