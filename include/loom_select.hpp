@@ -323,11 +323,20 @@ inline TokenScores token_logprobs(const float* d_logits, int64_t n_vocab, int64_
 // d_residual, when given, which becomes the sum), d_norm_weight [hidden_dim] f32; the product with d_weight [n_vocab,
 // hidden_dim] int8 and its scales d_weight_scale [n_vocab] (loom_quantize_rows_i8 makes both); then Generator::argmax
 // (src/core/generation.cpp:64-74) with its log-probability. A NaN never wins; a row of nothing else has id -1.
+// GreedyResult::logit is the log-probability plus the row's log-sum-exp: within a unit of the larger one's last place (and of
+// its own) of the logit that was written. d_x's and d_weight's checks come before anything is enqueued: when an argument
+// is refused, d_residual is as it was.
 // The logits are held in this thread's device memory (rows * n_vocab floats). Results on the host.
 inline GreedyResult lm_head_argmax_i8(const void* d_x, void* d_residual, const float* d_norm_weight, double eps,
                                       const int8_t* d_weight, const float* d_weight_scale, int64_t rows,
                                       int64_t hidden_dim, int64_t n_vocab, cudaStream_t stream = nullptr) {
-    if (rows <= 0 || hidden_dim <= 0 || n_vocab <= 0) detail::check(LOOM_SELECT_EINVAL, "lm_head_argmax_i8");
+    // what the second and third call would refuse, before the first adds to d_residual
+    const auto bad = [](const void* p, size_t a) { return !p || reinterpret_cast<uintptr_t>(p) % a != 0; };
+    if (rows <= 0 || hidden_dim <= 0 || n_vocab <= 0 || bad(d_weight, 16) || bad(d_weight_scale, 4))
+        detail::check(LOOM_SELECT_EINVAL, "lm_head_argmax_i8");
+    if (hidden_dim % 16 != 0 || rows > INT32_MAX / 16 || n_vocab > (int64_t(1) << 30) ||
+        (rows + 255) / 256 * ((n_vocab + 127) / 128) > INT32_MAX)
+        detail::check(LOOM_SELECT_ESHAPE, "lm_head_argmax_i8");
     const size_t n = static_cast<size_t>(rows);
     const size_t col = detail::align256(n * sizeof(float));
     const size_t q_bytes = detail::align256(n * static_cast<size_t>(hidden_dim));
@@ -336,6 +345,7 @@ inline GreedyResult lm_head_argmax_i8(const void* d_x, void* d_residual, const f
     // device: [ids] [log-probabilities] [log-sum-exps] [hidden scales] [8-bit hidden states] [logits]
     unsigned char* d = static_cast<unsigned char*>(
         st.device_out(4 * col + q_bytes + n * static_cast<size_t>(n_vocab) * sizeof(float)));
+    st.host_out(3 * col);
     int32_t* ids = reinterpret_cast<int32_t*>(d);
     float* logp = reinterpret_cast<float*>(d + col);
     float* lse = reinterpret_cast<float*>(d + 2 * col);
