@@ -776,9 +776,11 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kU == 2 ? 8 : kU == 8
         __syncwarp();
         key = sh.list[0][lane];
     }
-    // x / T by the reciprocal in two parts (an infinite x, the product with whose second part may be NaN, by the first)
+    // x / T by the reciprocal in two parts; where the product with the first is infinite already, that is it (with the second it
+    // may be of the other sign, or NaN)
     auto over_t = [&](float x) {
-        return fabsf(x) <= FLT_MAX ? __fmaf_rn(x, p.inv_t, __fmul_rn(x, p.inv_t_lo)) : __fmul_rn(x, p.inv_t);
+        const float y = __fmul_rn(x, p.inv_t);
+        return fabsf(y) <= FLT_MAX ? __fmaf_rn(x, p.inv_t, __fmul_rn(x, p.inv_t_lo)) : y;
     };
     float m = acc.m, lns = 0.0f;
     if (warp == kLast) {
