@@ -538,6 +538,8 @@ def token_logprobs(logits, ids=None, temperature=1.0, n_top=0, want_entropy=True
     dev = logits.device
     if want_rank and ids is None:
         raise SelectError(EINVAL, "a rank needs ids")
+    if n_top < 0:
+        raise SelectError(EPARAM, f"{n_top} alternatives")
     with _on(stream):
         f32 = [torch.empty(rows, dtype=torch.float32, device=dev) if w else None
                for w in (ids is not None, want_entropy, True)]
@@ -724,6 +726,8 @@ def lm_head_logits_i8_into(hidden, hidden_scale, weight, weight_scale, out, work
 def lm_head_logits_i8(hidden, hidden_scale, weight, weight_scale, dtype=None, workspace=None, stream=None):
     """lm_head_logits_i8_into a new tensor of `dtype` (f32 by default, or bf16)."""
     torch = _torch()
+    if hidden.dim() not in (1, 2) or weight.dim() != 2:
+        raise SelectError(EINVAL, "hidden must be [rows, hidden_dim] and weight [n_vocab, hidden_dim]")
     shape = (weight.shape[0],) if hidden.dim() == 1 else (hidden.shape[0], weight.shape[0])
     with _on(stream):
         out = torch.empty(shape, dtype=dtype or torch.float32, device=hidden.device)
