@@ -979,12 +979,14 @@ __device__ __forceinline__ float pick(uint4 raw, int q) {
 constexpr int kGradNT = 256;  // threads of a block that holds a row to each warp
 constexpr int kGradU = 4;
 // Shares of a row. A warp: rows of one step, and up to 4096 wide where there are 32 or more to an SM ([16384, 1025] f32 25.6 us,
-// blocks of four warps 40.7; [1000, 4000] f32 14.6 and 8.6). A block of four warps, two steps: [8000, 8000] bf16 51.5 us (of eight
-// 54.7). Wider rows by blocks of eight warps with three to six steps each, in clusters ([1024, 151936] f32, a cluster of
-// 8: 191.5 us, 4: 197.5, 2: 203; bf16, 4: 100.6, 2: 103.3, 8: 103.3; [3000, 32000] f32, 2: 119.8, 1: 126.6, 8: 137), and with
-// fewer steps where there are less than three blocks to an SM ([77, 51865] bf16, 8: 6.7 us, 4: 7.5, 2: 8.2). A row or a few
-// long ones by blocks of 32 warps (one of 151936 f32 5.0 us, of eight warps 6.0).
-// With a likely id in every row, whose entries have to be summed, [1024, 151936] f32 takes 204 us and bf16 112.
+// blocks of four warps 40.7; [1000, 4000] f32 14.6 and 8.6). A block of sixteen warps, one step, where there is no more
+// than a row to an SM ([148, 8000] f32 3.5 us, eight warps 4.5); else of four, two steps ([8000, 8000] bf16 51.5 us, eight
+// warps 54.7). Wider rows: a few by clusters of blocks of sixteen warps, a step each while there are blocks (one of 151936
+// f32 4.7 us, eight warps 5.5; of 20000 2.5 and 2.8); many by blocks of eight with three to six steps each
+// ([1024, 151936] f32, clusters of 8: 191.5 us, 4: 197.5, 2: 203; bf16, 4: 100.6, 2: 103.3, 8: 103.3; [3000, 32000] f32,
+// 2: 119.8, 1: 126.6, 8: 137), and with fewer steps where there are less than three blocks to an SM ([77, 51865] bf16,
+// 8: 6.7 us, 4: 7.5, 2: 8.2). With a likely id in every row, whose entries have to be summed, [1024, 151936] f32 takes 204 us
+// and bf16 112.
 constexpr int64_t kGradNarrow = 4096, kGradFew = 4;
 
 // What a block found in its part of a row.
@@ -1006,7 +1008,7 @@ struct GradShared {
 // and step. Rows of logits and of the gradient that start at the same place within 16 bytes go by vectors, the elements of
 // those that the row only partly fills apart; others element by element.
 template <int kDtype, int kWarps>
-__global__ void __launch_bounds__(kWarps == 1 ? kGradNT : kWarps * 32, kWarps == 4 ? 10 : kWarps == 32 ? 1 : 5)
+__global__ void __launch_bounds__(kWarps == 1 ? kGradNT : kWarps * 32, kWarps == 4 ? 10 : kWarps == 16 ? 2 : 5)
     token_logprobs_grad_kernel(const LpGradDev p) {
     constexpr int kEsz = kDtype == LOOM_SELECT_BF16 ? 2 : 4;
     constexpr int kPer = 16 / kEsz;
@@ -1196,12 +1198,16 @@ template <int kDtype>
 cudaError_t launch_grad_any(const LpGradDev& p, int sms, cudaStream_t s) {
     constexpr int kPer = kDtype == LOOM_SELECT_BF16 ? 8 : 4;
     const int64_t nv = (p.width + kPer - 2) / kPer + 1;  // (a row may start inside a vector)
-    if (nv <= 32 * kGradU || (p.width <= kGradNarrow && p.rows >= 32 * int64_t(sms))) return launch_grad<kDtype, 1>(p, 1, s);
-    if (nv <= 2 * 4 * 32 * kGradU) return launch_grad<kDtype, 4>(p, 1, s);
-    const int64_t steps = (nv + 8 * 32 * kGradU - 1) / (8 * 32 * kGradU);
-    if (p.rows <= kGradFew && steps > 2 * kMaxCluster) return launch_grad<kDtype, 32>(p, kMaxCluster, s);
+    auto steps = [&](int warps) { return (nv + warps * 32 * kGradU - 1) / (warps * 32 * kGradU); };
+    if (steps(1) == 1 || (p.width <= kGradNarrow && p.rows >= 32 * int64_t(sms))) return launch_grad<kDtype, 1>(p, 1, s);
+    if (steps(16) == 1 && p.rows <= sms) return launch_grad<kDtype, 16>(p, 1, s);
+    if (steps(4) <= 2) return launch_grad<kDtype, 4>(p, 1, s);
     int C = 1;
-    while (C < kMaxCluster && (steps >= 6 * C || (steps > C && p.rows * C < 3 * int64_t(sms)))) C *= 2;
+    if (p.rows <= kGradFew) {
+        while (C < kMaxCluster && steps(16) > C) C *= 2;
+        return launch_grad<kDtype, 16>(p, C, s);
+    }
+    while (C < kMaxCluster && (steps(8) >= 6 * C || (steps(8) > C && p.rows * C < 3 * int64_t(sms)))) C *= 2;
     return launch_grad<kDtype, 8>(p, C, s);
 }
 

@@ -56,7 +56,8 @@ def test_scores(rows, vocab, offset, dtype):
     (700, 4000, 2), (500, 8100, 0),                      # a block of four warps
     (460, 12007, 0), (500, 30011, 1), (300, 51865, 0),   # clusters of 1, 2, 4 (f32)
     (60, 51865, 3), (9, 151936, 0),                      # and of 8
-    (4, 151936, 1), (3, 262147, 0),                      # blocks of 32 warps
+    (4, 151936, 1), (3, 262147, 0), (2, 30011, 0),       # blocks of sixteen warps
+    (9, 1025, 1), (140, 8100, 0),                        # and one to a row
 ])
 def test_gradients(rows, vocab, offset, dtype):
     """Rows with a likely id and without one, padded and weightless rows between them; what lies between the rows stays."""
