@@ -69,6 +69,17 @@ struct LmTile {
         (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(BN >> 3) << 17) | (uint32_t(kBM >> 4) << 24);
 };
 
+template <int kStages>
+struct LmBars {
+    uint64_t full[kStages];    // TMA -> MMA
+    uint64_t empty[kStages];   // MMA -> TMA
+    uint64_t tfull[2];         // MMA -> epilogue
+    uint64_t tempty[2];        // epilogue -> MMA (4 arrivals: one per epilogue warp)
+    uint64_t drain;            // the MMA warp's final commit
+    uint32_t tmem_base;
+    int abort;
+};
+
 // The running (maximum, lowest id) of one row over W logits at tile columns [c0, c0 + W).
 template <int W>
 __device__ __forceinline__ void scan_chunk(const float (&v)[W], int c0, int valid, float& bv, int& bi) {

@@ -1215,7 +1215,8 @@ bool dtype_ok(int dtype) { return dtype == LOOM_SELECT_F32 || dtype == LOOM_SELE
 size_t esz_of(int dtype) { return dtype == LOOM_SELECT_BF16 ? 2 : 4; }
 bool misaligned(const void* p, size_t a) { return p && reinterpret_cast<uintptr_t>(p) % a != 0; }
 
-// T and log2(e) / T have to be normal numbers.
+// A normal number: 1 / T and log2(e) / T are finite then. (Where they are subnormal, for T above 8.5e37, they are off by 2e-7 of
+// themselves and x / T is below 4.)
 bool temperature_ok(float T) { return T >= FLT_MIN && T <= FLT_MAX; }
 
 }  // namespace

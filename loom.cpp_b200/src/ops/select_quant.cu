@@ -5,10 +5,9 @@
 //   inv = 1 / sqrt(sum h^2 / D + eps)      in 64 bits, rounded once to f32
 //   y = (h * inv) * w                      two f32 roundings
 //   a = max |y|,  scale = a / 127,  q = rint(y * ((1 / a) * 127))      each step one f32 rounding, |q| <= 127
-// quantize_rows_i8 takes y = x. The sum of squares is held in 64 bits so that the result does not depend on
-// the order of the summation: f32 squares are exact there up to 2^-53, and the one rounding of inv to f32
-// comes out the same for any order but for about one row in 10^8. q is then the same bit for bit whatever
-// the launch shape, as the plain definition gives it.
+// quantize_rows_i8 takes y = x. The sum of squares is held in 64 bits, where the order of the summation shows only
+// at 2^-53: the one rounding of inv to f32 comes out the same for any order, and q as the plain definition gives it
+// whatever the launch shape, but for about one row in 10^8.
 // Bound: HBM (rows read once: a thread keeps its elements in registers between the passes). [16384, 4096] f32 with the
 // residual takes 127.5 us (6.8 TB/s), [16384, 2048] bf16 38.5 us (6.1 TB/s), one row 2.8 us.
 #include <cfloat>

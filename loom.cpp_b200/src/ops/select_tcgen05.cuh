@@ -1,5 +1,5 @@
-// select_tcgen05.cuh -- what the LM-head kernels share: TMA tile loads, the tcgen05 instructions, the
-// barriers of their ring and accumulators, and the bounded wait that also honours a CTA's abort flag.
+// select_tcgen05.cuh -- what the LM-head kernels share: TMA tile loads, the tcgen05 instructions, and the
+// bounded wait that also honours a CTA's abort flag.
 #pragma once
 
 #include <cstdint>
@@ -12,17 +12,6 @@
 #include "select_device.cuh"
 
 namespace loom_select {
-
-template <int kStages>
-struct LmBars {
-    uint64_t full[kStages];    // TMA -> MMA
-    uint64_t empty[kStages];   // MMA -> TMA
-    uint64_t tfull[2];         // MMA -> epilogue
-    uint64_t tempty[2];        // epilogue -> MMA (4 arrivals: one per epilogue warp)
-    uint64_t drain;            // the MMA warp's final commit
-    uint32_t tmem_base;
-    int abort;
-};
 
 // ---- tcgen05 / TMA wrappers ----
 
@@ -154,12 +143,6 @@ __device__ __forceinline__ void tc_ld16(uint32_t taddr, float (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
-}
-
-template <int W>
-__device__ __forceinline__ void tc_ld(uint32_t taddr, float (&v)[W]) {
-    if constexpr (W == 32) tc_ld32(taddr, v);
-    else tc_ld16(taddr, v);
 }
 
 // Bounded wait that also gives up as soon as another role of the CTA has aborted.
