@@ -1108,7 +1108,7 @@ __global__ void __launch_bounds__(kWarps == 1 ? kGradNT : kWarps * 32, kWarps ==
                 const int32_t first = (v + u * kNT) * kPer - shift;
                 unsigned char* to = vout + int64_t(v + u * kNT) * 16;
                 const int32_t next = v + u * kNT + C * kGradU * kNT;
-                if (uint32_t(t - first) < uint32_t(kPer) || (sums && __fsub_rn(vec_max<kDtype>(raw[u]), r.hi) > p.likely)) {
+                if (uint32_t(t) - uint32_t(first) < uint32_t(kPer) || (sums && __fsub_rn(vec_max<kDtype>(raw[u]), r.hi) > p.likely)) {
 #pragma unroll 1
                     for (int q = 0; q < kPer; ++q) element(pick<kDtype>(raw[u], q), first + q);
                     if (next < v_end) raw[u] = plain_v4(vin + int64_t(next) * 16);
@@ -1158,9 +1158,8 @@ __global__ void __launch_bounds__(kWarps == 1 ? kGradNT : kWarps * 32, kWarps ==
         if (C > 1) {
             cluster.barrier_wait();
             if (thread == 0) *cluster.map_shared_rank(&sh.part[rank_in], 0) = all;
-            cluster.barrier_arrive();
+            cluster.sync();
             if (rank_in != 0) return;  // (nobody reads this block's shared memory)
-            cluster.barrier_wait();
             if (thread == 0) {
                 all = sh.part[0];
                 for (int b = 1; b < C; ++b) {
