@@ -1108,7 +1108,8 @@ __global__ void __launch_bounds__(kWarps == 1 ? kGradNT : kWarps * 32, kWarps ==
                 const int32_t first = (v + u * kNT) * kPer - shift;
                 unsigned char* to = vout + int64_t(v + u * kNT) * 16;
                 const int32_t next = v + u * kNT + C * kGradU * kNT;
-                if (uint32_t(t) - uint32_t(first) < uint32_t(kPer) || (sums && __fsub_rn(vec_max<kDtype>(raw[u]), r.hi) > p.likely)) {
+                if (uint32_t(t) - uint32_t(first) < uint32_t(kPer) ||
+                    (sums && __fsub_rn(vec_max<kDtype>(raw[u]), r.hi) > p.likely)) {
 #pragma unroll 1
                     for (int q = 0; q < kPer; ++q) element(pick<kDtype>(raw[u], q), first + q);
                     if (next < v_end) raw[u] = plain_v4(vin + int64_t(next) * 16);
@@ -1172,8 +1173,8 @@ __global__ void __launch_bounds__(kWarps == 1 ? kGradNT : kWarps * 32, kWarps ==
         }
     }
     if (thread != 0 || all.n != 1) return;
-    const float weight = (p.g_logp && t >= 0 ? fabsf(p.g_logp[row]) : 0.0f) +
-                         (p.g_entropy ? fabsf(p.g_entropy[row]) * (4.0f + 2.0f * p.entropy[row]) : 0.0f);
+    const float g_abs = p.g_logp && t >= 0 ? fabsf(p.g_logp[row]) : 0.0f, h_abs = p.g_entropy ? fabsf(p.g_entropy[row]) : 0.0f;
+    const float weight = g_abs + (h_abs != 0.0f ? h_abs * (4.0f + 2.0f * p.entropy[row]) : 0.0f);
     const float off = weight * p.inv_t * (kLseError + 2.0f * FLT_EPSILON * fabsf(p.lse[row]));
     if (fabsf(-all.sum - all.direct) <= off) store_elem<kDtype>(out, all.id, -all.sum);
 }

@@ -168,6 +168,19 @@ def test_lse_of_a_larger_row():
     assert ((got.double() - want).abs() <= lp.exp() * U * (4 * lp.abs() / math.log(2) + 9) + 4 * U * want.abs()).all()
 
 
+def test_entropy_of_rows_without_its_weight_is_not_read():
+    """Rows whose entropy weight is 0 may hold anything there."""
+    x, ids = _rows_with(8, 3001, 1e-4, 1.0, seed=4)
+    lse, ent, _ = _state(x, 1.0, False)
+    g = torch.linspace(1, 2, 8, device="cuda")
+    h = torch.zeros(8, device="cuda")
+    h[::2] = 0.1
+    ent[1::2] = math.nan
+    got = ls.token_logprobs_grad(x, ids, lse, g, h, ent)
+    want, tol = _want(x, ids, 1.0, g, h, 0.0, torch.float32)
+    assert ((got.double() - want).abs() <= tol).all()
+
+
 def test_captured_and_on_two_streams():
     x1, i1 = _rows_with(3, 151936, 1e-4, 1.0, seed=1)
     x2, i2 = _rows_with(500, 1500, 1e-4, 1.0, seed=2)
