@@ -381,18 +381,6 @@ __global__ void __launch_bounds__(256) lm_merge_kernel(const float4* __restrict_
     }
 }
 
-bool make_map(CUtensorMap* m, const void* base, uint64_t inner, uint64_t outer, uint32_t box_outer) {
-    auto fn = encode_fn();
-    if (!fn) return false;
-    const cuuint64_t dims[2] = {inner, outer};
-    const cuuint64_t strides[1] = {inner * 2};
-    const cuuint32_t box[2] = {uint32_t(kBK), box_outer};
-    const cuuint32_t estr[2] = {1, 1};
-    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 // The two tile widths: 256 ids, or 208 when that spreads the tiles over the SMs clearly more evenly
 // (151936 ids on one row tile: 594 tiles of 256 leave two SMs a fifth tile, 731 tiles of 208 fill 148
 // SMs five times within 1%). The workspace holds records for the narrower one.
@@ -413,8 +401,8 @@ int launch_lm(const void* hidden, const void* weight, const LmArgs& a, int64_t h
               cudaStream_t stream) {
     using T = LmTile<BN, kFewRows>;
     CUtensorMap map_h, map_w;
-    if (!make_map(&map_h, hidden, uint64_t(hidden_dim), uint64_t(a.rows), uint32_t(T::kARows)) ||
-        !make_map(&map_w, weight, uint64_t(hidden_dim), uint64_t(a.n_vocab), BN))
+    if (!make_map(&map_h, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, hidden, uint64_t(hidden_dim), uint64_t(a.rows), uint32_t(T::kARows)) ||
+        !make_map(&map_w, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, weight, uint64_t(hidden_dim), uint64_t(a.n_vocab), BN))
         return LOOM_SELECT_ECUDA;
     static std::once_flag attr_once[64];
     int dev = 0;

@@ -374,18 +374,6 @@ __global__ void __launch_bounds__(I8Tile<NR, kPair>::kThreads, 1)
     }
 }
 
-bool make_map_i8(CUtensorMap* m, const void* base, uint64_t inner, uint64_t outer, uint32_t box_outer) {
-    auto fn = encode_fn();
-    if (!fn) return false;
-    const cuuint64_t dims[2] = {inner, outer};
-    const cuuint64_t strides[1] = {inner};
-    const cuuint32_t box[2] = {uint32_t(kBK), box_outer};
-    const cuuint32_t estr[2] = {1, 1};
-    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int NR, bool kPair, int kOut>
 int launch_i8(const void* hidden, const void* weight, I8Args a, int64_t hidden_dim, int sms, cudaStream_t stream) {
     using T = I8Tile<NR, kPair>;
@@ -394,9 +382,9 @@ int launch_i8(const void* hidden, const void* weight, I8Args a, int64_t hidden_d
     a.units = (a.n_vocab + kUnit - 1) / kUnit;
     const int64_t work = a.r_tiles == 1 ? a.units : a.v_tiles * a.r_tiles;
     CUtensorMap map_h, map_w, map_unit;
-    if (!make_map_i8(&map_h, hidden, uint64_t(hidden_dim), uint64_t(a.rows), T::kBRows) ||
-        !make_map_i8(&map_w, weight, uint64_t(hidden_dim), uint64_t(a.n_vocab), kIds) ||
-        !make_map_i8(&map_unit, weight, uint64_t(hidden_dim), uint64_t(a.n_vocab), kUnit))
+    if (!make_map(&map_h, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, hidden, uint64_t(hidden_dim), uint64_t(a.rows), T::kBRows) ||
+        !make_map(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, weight, uint64_t(hidden_dim), uint64_t(a.n_vocab), kIds) ||
+        !make_map(&map_unit, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, weight, uint64_t(hidden_dim), uint64_t(a.n_vocab), kUnit))
         return LOOM_SELECT_ECUDA;
     static std::atomic<bool> configured[64] = {};  // set once per device, from any host thread
     int dev = 0;

@@ -175,4 +175,18 @@ inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
+// A packed [outer, inner] matrix of `esz`-byte elements in boxes of box_outer rows by 128 bytes, with the 128-byte swizzle;
+// zeros past its ends.
+inline bool make_map(CUtensorMap* m, CUtensorMapDataType type, uint32_t esz, const void* base, uint64_t inner, uint64_t outer,
+                     uint32_t box_outer) {
+    auto fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {inner, outer};
+    const cuuint64_t strides[1] = {inner * esz};
+    const cuuint32_t box[2] = {128 / esz, box_outer};
+    const cuuint32_t estr[2] = {1, 1};
+    return fn(m, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace loom_select
