@@ -290,7 +290,8 @@ LOOM_SELECT_API int loom_lm_head_argmax(const void* hidden, const void* weight, 
  * LOOM_SELECT_MAX_TOP_LOGPROBS), positive exactly when one of out_top_ids and out_top_logp is given. T is a
  * positive, finite, normal float (LOOM_SELECT_EPARAM otherwise, as for n_top out of range). Log-probabilities are
  * accurate to 7e-5 absolute for V up to 262144, by the bound on every rounding (about 1e-6 as measured), besides 2^-22 of
- * their own size. The comparisons are exact: -0 == +0. An out_lse beyond f32's range (the lowest finite values over T < 1) is
+ * their own size; where an id has p above 0.8, its log-probability to 7e-5 and the row's entropy to 2e-4 of themselves (3e-7
+ * as measured). The comparisons are exact: -0 == +0. An out_lse beyond f32's range (the lowest finite values over T < 1) is
  * infinite, and so is a difference of two logits beyond it, whatever T.
  *   - A negative id means "no token in this row" (padding): out_logp = 0, out_rank = -1, the rest as usual.
  *     An id >= V: out_logp = NaN, out_rank = -1.

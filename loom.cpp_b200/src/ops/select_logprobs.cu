@@ -1,7 +1,8 @@
 // select_logprobs.cu -- log-probabilities of given tokens, with entropy, rank and top alternatives.
 //
 // With y = x / T over a row's n_vocab logits, m = max y, S = sum exp(y - m), A = sum exp(y - m)(y - m):
-//   lse = m + ln S,   log p(t) = (y_t - m) - ln S,   H = ln S - A / S,
+//   lse = m + ln S,   log p(t) = (y_t - m) - ln S,   H = ln S - A / S
+// (S near 1, as ln(1 + (S - 1)) from a sum without the largest element: log p keeps its digits where p is near 1),
 //   rank(t) = number of ids ahead of t in the order (x descending, id ascending),
 //   alternatives = the first n_top ids of that order with their log-probabilities.
 // One pass over the logits: each thread keeps (m, S, A) of its elements and rescales S and A when its
@@ -32,6 +33,9 @@ constexpr float kLn2 = 0.6931471805599453f;
 // Exponents are clamped here: 2^-200 is zero in f32, and zero times this is zero (a -inf logit would
 // otherwise add 0 * -inf to A).
 constexpr float kMinExp2 = -200.0f;
+
+// A row whose sum of exponentials, its largest element's 1 among them, is below this is added up without that one.
+constexpr float kNearOne = 1.25f;
 
 __device__ __forceinline__ float neg_inf() { return -__int_as_float(0x7f800000); }
 __device__ __forceinline__ float quiet_nan() { return __int_as_float(0x7fc00000); }
@@ -107,6 +111,8 @@ struct LpShared {
     float edge[32];            // the elements apart from the vectors (the first block's)
     // of the cluster's first block: what the blocks hand on
     SoftAcc acc[kBlocks * kW];  // of each warp
+    float others[kBlocks * kW];  // its sum without that of the lane with its maximum
+    int32_t lead[kBlocks * kW];  // that lane
     int32_t ahead[kBlocks * kW];
     int32_t part_cand[kBlocks];
     float m, lns;              // the row's, from the warp that has them to the one with the alternatives
@@ -152,6 +158,14 @@ __device__ __forceinline__ SoftAcc soft_reduce(SoftAcc p, int n, float c) {
         p.a += __shfl_xor_sync(0xffffffffu, p.a, o);
     }
     return p;
+}
+
+// Of the warp's states, moved to their common maximum M: the first lane that has it, and the sum of the others' s.
+__device__ __forceinline__ float soft_others(SoftAcc p, float M, float c, int32_t& lead) {
+    lead = __ffs(__ballot_sync(0xffffffffu, p.m == M && p.s > 0.0f)) - 1;
+    float s = int32_t(threadIdx.x & 31) == lead ? 0.0f : soft_move(p, M, c).s;
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
 }
 
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
@@ -441,6 +455,36 @@ __device__ __noinline__ uint64_t list_slots(const LpShare& r, LpShared<kW, true>
     return key;
 }
 
+// The sum of 2^((x - m) c) over the elements of one lane of the row, whose first vector is v, without its maximum m: read
+// again by a whole warp. (In line: as a call it cost one row of 51865 bf16 with 5 alternatives, which does not come here,
+// 1.4 us of 7.0.)
+template <int kDtype, int kU, int kNT>
+__device__ __forceinline__ float sum_without_max(const unsigned char* vec, int32_t v, int32_t v1, int32_t stride, float m, float c) {
+    const int lane = threadIdx.x & 31;
+    const int32_t n = v < v1 ? ((v1 - v + stride - 1) / stride) * kU : 0;
+    float s = 0.0f;
+    for (int32_t i0 = 0; i0 < n; i0 += 4 * 32) {
+        uint4 raw[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int32_t i = i0 + k * 32 + lane, at = v + i / kU * stride + i % kU * kNT;
+            const uint32_t none = kDtype == LOOM_SELECT_BF16 ? 0xff80ff80u : 0xff800000u;
+            raw[k] = make_uint4(none, none, none, none);
+            if (i < n && at < v1) raw[k] = ldg_stream_v4(vec + int64_t(at) * 16);
+        }
+#pragma unroll 1
+        for (int k = 0; k < 4; ++k) {
+            Vec16<kDtype> e;
+            e.unpack(k == 0 ? raw[0] : k == 1 ? raw[1] : k == 2 ? raw[2] : raw[3]);
+#pragma unroll
+            for (int q = 0; q < Vec16<kDtype>::kElems; ++q)
+                if (e.x[q] != m) s += ex2(max_nan(__fmul_rn(__fsub_rn(e.x[q], m), c), kMinExp2));
+        }
+    }
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
+}
+
 // Up to this width, and for more than 8 alternatives, the lanes of a row's one warp look through their own slots, of few
 // elements and most of them hit ([16384, 1025] f32 with 20 45.3 us, by the warp together 63.5; [8000, 8000] bf16 70.1 and
 // 65.8; with 5 [700, 2048] f32 8.6 and 7.7).
@@ -538,7 +582,7 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kU == 2 ? 8 : kU == 8
         const float x = id >= 0 ? load_global_elem<kDtype>(rowp, id) : neg_inf();
         st.add_edge(x);
         st.ahead += rank && id >= 0 && (x > xt || (x == xt && id < t));
-        if (kTop) sh.edge[lane] = x;
+        sh.edge[lane] = x;
     }
 
     float slot_top = neg_inf();  // this thread's maximum in the current slot
@@ -584,6 +628,14 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kU == 2 ? 8 : kU == 8
     if (kW > 1 && lane == 0) {
         first->acc[rank_in * kW + warp] = acc;
         first->ahead[rank_in * kW + warp] = ahead;
+    }
+    if (kW > 1 && acc.s < kNearOne) {  // (only then the row's may be)
+        int32_t lead;
+        const float others = soft_others(st.acc, acc.m, p.c, lead);
+        if (lane == 0) {
+            first->others[rank_in * kW + warp] = others;
+            first->lead[rank_in * kW + warp] = lead;
+        }
     }
     const int32_t slots = int32_t(slot_at - &sh.slot_max[warp][0][lane]) / 32;
     LpShare r{rowp, shift, v_start, v1, stride, per_slot, slots, p.n_top, 0.0f};
@@ -799,6 +851,39 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kU == 2 ? 8 : kU == 8
         }
         m = acc.m;
         lns = logf(acc.s);  // -inf for an empty row, NaN where a logit was NaN or +inf
+        if (acc.s > 0.0f && acc.s < kNearOne) {
+            // One id has nearly all of the probability, 1 / S, and ln S is a small number that the 1 in S leaves few digits
+            // of: the sum again without it, from the parts that do not hold it and the elements of the lane that does
+            // (two round trips to L2 more: [20000, 300] bf16 with 20 alternatives, such in every fifth row, 40.0 -> 44.6 us).
+            int32_t lead = 0, at = 0;
+            float rest;
+            if constexpr (kW > 1) {
+                at = 64;
+                rest = 0.0f;
+                for (int w = lane; w < C * kW; w += 32) {
+                    const SoftAcc other = sh.acc[w];
+                    if (other.m == m && other.s > 0.0f) {
+                        at = w;
+                        rest += sh.others[w];
+                        lead = sh.lead[w];
+                    } else {
+                        rest += soft_move(other, m, p.c).s;
+                    }
+                }
+                for (int o = 16; o > 0; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
+                const int32_t all = __reduce_min_sync(0xffffffffu, at);
+                lead = __shfl_sync(0xffffffffu, lead, all % 32);
+                at = all;
+            } else {
+                rest = soft_others(st.acc, m, p.c, lead);
+            }
+            const int32_t from = v0 + (at / kW) * kU * kNT + (at % kW) * 32 + lead;
+            rest += sum_without_max<kDtype, kU, kNT>(vec, from, v1, stride, m, p.c);
+            if (const float x = at == 0 ? sh.edge[lead] : m; x != m)
+                rest += ex2(fmaxf(__fmul_rn(__fsub_rn(x, m), p.c), kMinExp2));
+            lns = log1pf(rest);
+            acc.s = 1.0f + rest;
+        }
         const bool empty = acc.s == 0.0f;
         if (lane == 0) {
             if (kLast > 0) {

@@ -201,3 +201,53 @@ def test_captured_and_on_two_streams():
     torch.cuda.synchronize()
     for _, out, want, _, _ in calls:
         assert torch.equal(out, want)  # the same bits every time
+
+
+# ---- the forward call ----
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rest", [0.1, 1e-3, 1e-6, 1e-9])
+@pytest.mark.parametrize("rows,vocab,offset,T", [
+    (1, 1, 0, 1.0), (2, 9, 1, 1.0), (1, 300, 0, 0.7), (3, 900, 2, 1.0), (200, 900, 0, 1.0), (700, 1500, 3, 1.3),
+    (2100, 3001, 1, 1.0), (40, 5003, 0, 0.7), (300, 20000, 1, 1.0), (700, 12007, 0, 1.0), (700, 30011, 5, 1.0),
+    (2, 51865, 1, 1.0), (1, 151936, 0, 1.3), (20, 151936, 3, 1.0), (1, 262147, 7, 1.0),
+])
+def test_log_probability_of_a_likely_id(rows, vocab, offset, T, rest, dtype):
+    """log p = -ln S of the largest element, S = 1 + the others' exponentials: off by what the others are, 600 u (see
+    test_gpu_logprobs.py) and 3 u |d| + 4 u of each, d its distance in powers of 2, relative to themselves; and so the
+    entropy ln S + sum e |d| ln 2 / S. Then four roundings of each."""
+    x, ids = _rows_with(rows, vocab, rest, T, seed=rows + vocab, dtype=dtype, offset=offset, extra=offset)
+    lp, p, _, ent, top = _parts(x, T)
+    if vocab == 1:
+        x.fill_(1.5)
+        lp, p, _, ent, top = _parts(x, T)
+    r = ls.token_logprobs(x, ids, temperature=T, n_top=1)
+    assert torch.equal(r.top_ids, top.int()) and torch.equal(ids.long(), top[:, 0])
+    e = torch.where(p > 0, p / p.gather(1, top), 0.0).scatter(1, top, 0.0)
+    d = torch.where(e > 0, -torch.log2(e), 0.0)
+    off = e * (600 + 3 * d + 4) * U
+    want = lp.gather(1, top)[:, 0]
+    tol = off.sum(dim=1) + 4 * U * want.abs()
+    assert ((r.logp.double() - want).abs() <= tol).all() and torch.equal(r.top_logp[:, 0], r.logp)
+    tol = (off * (2 + d * math.log(2))).sum(dim=1) + 8 * U * ent[:, 0]
+    assert ((r.entropy.double() - ent[:, 0]).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [2, 700])
+@pytest.mark.parametrize("vocab", [13, 257, 4099, 20011])
+def test_the_likely_id_in_every_place(vocab, rows, dtype):
+    """At the row's ends and in the vectors that the row only partly fills."""
+    for place in (0, 1, 5, vocab // 2, vocab - 2, vocab - 1):
+        for offset in (0, 1, 3, 5):
+            g = torch.Generator(device="cuda").manual_seed(place + offset)
+            buf = torch.randn(rows * (vocab + 3) + 16, generator=g, device="cuda").to(dtype)
+            x = buf[offset:offset + rows * (vocab + 3)].view(rows, vocab + 3)[:, :vocab]
+            x[:, place] = 20.0
+            ids = torch.full((rows,), place, dtype=torch.int32, device="cuda")
+            lp, p, _, _, top = _parts(x, 1.0)
+            e = (p / p.gather(1, top)).scatter(1, top, 0.0)
+            want = lp.gather(1, top)[:, 0]
+            tol = (e * (604 - 3 * torch.log2(e.clamp(min=1e-30))) * U).sum(dim=1) + 4 * U * want.abs()
+            got = ls.token_logprobs(x, ids, n_top=2).logp
+            assert ((got.double() - want).abs() <= tol).all()
