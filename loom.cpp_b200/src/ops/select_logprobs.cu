@@ -486,7 +486,7 @@ __device__ __forceinline__ float sum_without_max(const unsigned char* vec, int32
 }
 
 // Up to this width, and for more than 8 alternatives, the lanes of a row's one warp look through their own slots, of few
-// elements and most of them hit ([16384, 1025] f32 with 20 45.3 us, by the warp together 63.5; [8000, 8000] bf16 70.1 and
+// elements and most of them hit ([16384, 1025] f32 with 20 45.3 us when it was measured (47.7 now), by the warp together 63.5; [8000, 8000] bf16 70.1 and
 // 65.8; with 5 [700, 2048] f32 8.6 and 7.7).
 constexpr int32_t kOwnSlots = 4096;
 
@@ -514,7 +514,7 @@ __device__ __forceinline__ void block_sync() {
 // every block has an SM to itself and two such steps or more to read (then 1 row of 151936 f32 8.4 us, with four 9.6, 18
 // rows 10.1 and 10.9; with less to read, one of 51865 bf16 7.8 and 7.3, 18 of 151936 bf16 10.5 and 9.9). Two for a warp's
 // row of at most two such steps, eight blocks to an SM ([20000, 300] bf16 without alternatives 15.6 us, with four 21.0;
-// [20000, 800] f32 23.5 and 19.9).
+// [20000, 800] f32 23.5 and 19.9; all of these before rows with a likely id were summed twice).
 template <int kDtype, bool kTop, int kW, int kU>
 __global__ void __launch_bounds__(kW == 1 ? 128 : kW * 32, kU == 2 ? 8 : kU == 8 ? 2 : kW < 8 ? 7 : 4)
     token_logprobs_kernel(const LpDev p) {
