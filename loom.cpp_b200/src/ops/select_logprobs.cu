@@ -486,8 +486,8 @@ __device__ __forceinline__ float sum_without_max(const unsigned char* vec, int32
 }
 
 // Up to this width, and for more than 8 alternatives, the lanes of a row's one warp look through their own slots, of few
-// elements and most of them hit ([16384, 1025] f32 with 20 45.3 us when it was measured (47.7 now), by the warp together 63.5; [8000, 8000] bf16 70.1 and
-// 65.8; with 5 [700, 2048] f32 8.6 and 7.7).
+// elements and most of them hit ([16384, 1025] f32 with 20 45.3 us when it was measured (47.7 now), by the warp together
+// 63.5; [8000, 8000] bf16 70.1 and 65.8; with 5 [700, 2048] f32 8.6 and 7.7).
 constexpr int32_t kOwnSlots = 4096;
 
 template <int kW>
